@@ -1,0 +1,501 @@
+// Causal attention of each sequence's new tokens over its paged cache (gdnr_paged_attention).
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i.k_j - max),  j <= kv - m + i
+//
+// for the m new tokens i of a sequence of kv tokens.  The G = Hq/Hk query heads of a key
+// head are rows of one tile (row r of a sequence: token r / G, head r % G), so a key
+// or value read from memory serves all of them.
+#include "gdnr_device.cuh"
+#include "gdnr_hybrid.h"
+#include "gdnr_tile.cuh"
+
+#include <algorithm>
+
+namespace gdnr {
+
+namespace {
+
+constexpr int AT_BN = 64;  // keys of a tile
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int AT_META = 8;  // ints of one CTA's record
+constexpr int AT_MAX_CTAS_PER_SM = 2;
+
+// ---------------------------------------------------------------- work split
+// A unit is (sequence, key head, tile of BM rows); its cost is the number of key tiles
+// its last row sees.  The units of the batch laid end to end are cut into equal shares,
+// one per CTA, so ragged lengths and few heads fill the machine alike.
+template <int BM>
+__device__ __forceinline__ int unit_tiles(const AttnParams& p, int kv, int m, int rt) {
+  const int last_row = min((rt + 1) * BM, m * p.G) - 1;
+  const int keys = min(kv, kv - m + last_row / p.G + 1);
+  return max(1, (keys + AT_BN - 1) / AT_BN);  // a unit without keys still writes its rows
+}
+
+struct SeqLen {
+  int q0, m, kv;
+};
+
+__device__ __forceinline__ SeqLen seq_len(const AttnParams& p, int n) {
+  SeqLen s;
+  s.q0 = min(max(p.cu[n], 0), p.T);
+  s.m = min(max(p.cu[n + 1], s.q0), p.T) - s.q0;
+  s.kv = int(min(int64_t(max(p.kv_lens[n * p.kl_s], 0)), int64_t(p.width) * p.page_size));
+  return s;
+}
+
+template <int BM>
+__device__ int64_t seq_tiles(const AttnParams& p, const SeqLen& s) {
+  const int rts = (s.m * p.G + BM - 1) / BM;
+  int64_t sum = 0;
+  for (int rt = 0; rt < rts; ++rt) sum += unit_tiles<BM>(p, s.kv, s.m, rt);
+  return sum * p.Hk;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// The unit that key tile `at` of the batch falls into (one whole warp).
+struct Unit {
+  int n, h, rt;
+  SeqLen s;
+  int64_t begin;  // first key tile of the unit
+  int tiles;
+};
+
+template <int BM>
+__device__ __forceinline__ Unit find_unit(const AttnParams& p, int64_t at, int lane) {
+  int64_t base = 0;
+  Unit u;
+  u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
+  u.s.q0 = u.s.m = u.s.kv = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    const int n = n0 + lane;
+    int64_t w = 0;
+    if (n < p.N) w = seq_tiles<BM>(p, seq_len(p, n));
+    int64_t pre = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + pre > at);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
+      u.n = n0 + src;
+      u.s = seq_len(p, u.n);
+      const int64_t per_head = __shfl_sync(0xffffffffu, w, src) / p.Hk;
+      u.h = int((at - start) / per_head);
+      u.begin = start + u.h * per_head;
+      u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, 0);
+      while (u.begin + u.tiles <= at) {
+        u.begin += u.tiles;
+        u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, ++u.rt);
+      }
+      return u;
+    }
+    base += __shfl_sync(0xffffffffu, pre, 31);
+  }
+  u.n = p.N;
+  return u;
+}
+
+// The next unit in order.
+template <int BM>
+__device__ __forceinline__ void next_unit(const AttnParams& p, Unit& u) {
+  u.begin += u.tiles;
+  ++u.rt;
+  if (u.rt * BM >= u.s.m * p.G) {
+    u.rt = 0;
+    if (++u.h == p.Hk) {
+      u.h = 0;
+      do {
+        if (++u.n >= p.N) return;
+        u.s = seq_len(p, u.n);
+      } while (u.s.m == 0);
+    }
+  }
+  u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, u.rt);
+}
+
+struct Share {
+  int64_t begin, end;
+};
+
+// Share i of `total` key tiles; at least two tiles each, so that small batches do not
+// pay for joining shares of one tile.
+__device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
+  const int64_t use = min(int64_t(ctas), (total + 1) / 2);
+  Share s;
+  if (i >= use) {
+    s.begin = s.end = total;
+    return s;
+  }
+  s.begin = total * i / use;
+  s.end = total * (i + 1) / use;
+  return s;
+}
+
+// ---------------------------------------------------------------- kernel
+// WM x WN warps: WM groups of 16 rows, each tile's keys cut over WN warps that keep
+// their own running maximum and sum and are joined at the unit's end.
+template <int D, int WM, int WN, int STAGES>
+struct AtCfg {
+  static constexpr int BM = 16 * WM;
+  static constexpr int THREADS = 32 * WM * WN;
+  static constexpr int ROWB = D * 2;
+  static constexpr int TILE = AT_BN * ROWB;
+  static constexpr int Q_BYTES = BM * ROWB;
+  static constexpr int JOIN = WN > 1 ? WN * 16 * (D + 4) * 4 : 0;
+  static constexpr int SMEM = Q_BYTES + STAGES * 2 * TILE;
+  static_assert(JOIN <= STAGES * 2 * TILE, "the join reuses the stages");
+};
+
+template <int D, int WM, int WN, int STAGES>
+__global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constant__ AttnParams p) {
+  using C = AtCfg<D, WM, WN, STAGES>;
+  constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t sh_total;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wm = warp / WN, wn = warp % WN;
+  const uint32_t q_s = smem_addr(smem), kv_s = q_s + C::Q_BYTES;
+  float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
+  int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
+
+  if (warp == 0) {
+    int64_t w = 0;
+    for (int n = lane; n < p.N; n += 32) w += seq_tiles<BM>(p, seq_len(p, n));
+    w = warp_sum64(w);
+    if (lane == 0) sh_total = w;
+  }
+  __syncthreads();
+  const int64_t total = sh_total;
+  const Share share = share_of(total, blockIdx.x, gridDim.x);
+  if (share.begin >= share.end) {
+    if (tid == 0) meta[0] = -1;
+    return;
+  }
+  Unit u = find_unit<BM>(p, share.begin, lane);
+  if (tid == 0) {
+    // record for the join: the unit this share begins in, if it begins inside it
+    meta[0] = share.begin > u.begin ? u.n : -1;
+    meta[1] = u.h;
+    meta[2] = u.rt;
+    meta[3] = int(share.begin - u.begin);              // tiles of that unit in earlier shares
+    meta[4] = int(u.begin + u.tiles - share.begin);    // tiles of it from here on
+    meta[5] = int(share.end - share.begin);
+  }
+  const float sl2 = p.scale * LOG2E;
+  for (int64_t at = share.begin; at < share.end; next_unit<BM>(p, u), at = u.begin) {
+    const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+    const int rows = u.s.m * p.G - u.rt * BM;  // rows of the sequence from this tile on
+    const int row_base = u.rt * BM;
+    const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
+    if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+    // query rows of the tile; rows beyond the sequence's are zeros
+    for (int i = tid; i < BM * CH; i += C::THREADS) {
+      const int r = i / CH, c = i % CH;
+      const bool ok = r < rows;
+      const int rr = row_base + (ok ? r : 0), tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
+      cp_async16_zfill(q_s + swz<ROWB>(r, c), p.q + int64_t(tok) * p.q_st + int64_t(hd) * p.q_sh + c * 8, ok ? 16 : 0);
+    }
+    auto load_tile = [&](int t, int stage) {
+      const uint32_t ks = kv_s + stage * 2 * C::TILE, vs = ks + C::TILE;
+      for (int i = tid; i < AT_BN * CH; i += C::THREADS) {
+        const int r = i / CH, c = i % CH;
+        const int tok = t * AT_BN + r;
+        const uint16_t *ksrc = p.k, *vsrc = p.v;
+        uint32_t bytes = 0;
+        // keys past the sequence's end are never read: what a page holds there may be anything
+        if (tok < u.s.kv) {
+          const int pi = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
+          const int off = tok - pi * p.page_size;
+          const int page = table[pi];
+          if (page >= 0 && page < p.pages) {
+            ksrc += int64_t(page) * p.k_sp + int64_t(off) * p.k_st + int64_t(u.h) * p.k_sh + c * 8;
+            vsrc += int64_t(page) * p.v_sp + int64_t(off) * p.v_st + int64_t(u.h) * p.v_sh + c * 8;
+            bytes = 16;
+          } else {
+            atomicOr(p.err, GDNR_DEVERR_BAD_SLOT);
+          }
+        }
+        cp_async16_zfill(ks + swz<ROWB>(r, c), ksrc, bytes);
+        cp_async16_zfill(vs + swz<ROWB>(r, c), vsrc, bytes);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (t0 + s < t1) load_tile(t0 + s, s);
+      cp_async_commit();
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    // last key each of this thread's two rows sees
+    int lim[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = row_base + wm * 16 + (lane >> 2) + 8 * j;
+      lim[j] = r < u.s.m * p.G ? min(u.s.kv - 1, u.s.kv - u.s.m + r / p.G) : -1;
+    }
+    for (int t = t0; t < t1; ++t) {
+      const int i = t - t0;
+      cp_async_wait<STAGES - 2>();
+      __syncthreads();
+      if (t + STAGES - 1 < t1) load_tile(t + STAGES - 1, (i + STAGES - 1) % STAGES);
+      cp_async_commit();
+      const uint32_t ks = kv_s + (i % STAGES) * 2 * C::TILE, vs = ks + C::TILE;
+      float s[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        ldsm_x4(q_s + swz<ROWB>(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)), a);
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+          uint32_t b[4];
+          ldsm_x4(ks + swz<ROWB>(wn * (AT_BN / WN) + j * 16 + ((lane >> 4) << 3) + (lane & 7), kk * 2 + ((lane >> 3) & 1)), b);
+          mma16816_bf16(s[2 * j], a, b[0], b[1]);
+          mma16816_bf16(s[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+      const int key0 = t * AT_BN + wn * (AT_BN / WN) + 2 * (lane & 3);
+      float tm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // a comparison, not an added bias: whatever a masked score is, it leaves no trace
+          s[j][e] = key0 + j * 8 + (e & 1) <= lim[e >> 1] ? s[j][e] * sl2 : -INFINITY;
+          tm[e >> 1] = fmaxf(tm[e >> 1], s[j][e]);
+        }
+      float corr[2], base[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        tm[j] = fmaxf(tm[j], __shfl_xor_sync(0xffffffffu, tm[j], 1));
+        tm[j] = fmaxf(tm[j], __shfl_xor_sync(0xffffffffu, tm[j], 2));
+        const float nm = fmaxf(mx[j], tm[j]);
+        base[j] = nm == -INFINITY ? 0.f : nm;  // a row that has seen no key yet
+        corr[j] = ex2_approx(mx[j] - base[j]);
+        mx[j] = nm;
+        sum[j] *= corr[j];
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][e] = ex2_approx(s[j][e] - base[e >> 1]);
+          sum[e >> 1] += s[j][e];
+        }
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        o[j][0] *= corr[0];
+        o[j][1] *= corr[0];
+        o[j][2] *= corr[1];
+        o[j][3] *= corr[1];
+      }
+#pragma unroll
+      for (int kk = 0; kk < NT / 2; ++kk) {
+        // weights are rounded to bf16 for the tensor cores; their sum is taken before that
+        uint32_t a[4] = {pack_bf16x2(s[2 * kk][0], s[2 * kk][1]), pack_bf16x2(s[2 * kk][2], s[2 * kk][3]),
+                         pack_bf16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_bf16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t b[4];
+          ldsm_x4_t(vs + swz<ROWB>(wn * (AT_BN / WN) + kk * 16 + (lane & 15), j * 2 + (lane >> 4)), b);
+          mma16816_bf16(o[2 * j], a, b[0], b[1]);
+          mma16816_bf16(o[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // every warp is done with the tiles and the query rows
+    const bool whole = t0 == 0 && t1 == u.tiles;
+    // a share that begins inside a unit leaves its part in slot 0, one that only ends inside in slot 1
+    float* part = ws_o + (t0 > 0 ? 0 : 1) * BM * (D + 2);
+    if constexpr (WN == 1) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = wm * 16 + (lane >> 2) + 8 * j;
+        if (r >= rows) continue;
+        if (whole) {
+          const int rr = row_base + r, tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
+          const float inv = sum[j] > 0.f ? 1.0f / sum[j] : 0.f;
+          uint16_t* dst = p.out + int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + 2 * (lane & 3);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint32_t*>(dst + c * 8) = pack_bf16x2(o[c][2 * j] * inv, o[c][2 * j + 1] * inv);
+          if (p.lse && (lane & 3) == 0)
+            p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = sum[j] > 0.f ? (mx[j] + log2f(sum[j])) * LN2 : -INFINITY;
+        } else {
+          float* dst = part + r * (D + 2);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<float2*>(dst + c * 8 + 2 * (lane & 3)) = make_float2(o[c][2 * j], o[c][2 * j + 1]);
+          if ((lane & 3) == 0) dst[D] = mx[j], dst[D + 1] = sum[j];
+        }
+      }
+    } else {
+      // join the WN warps' parts of the 16 rows through shared memory
+      static_assert(WM == 1 || WN == 1, "one of the two");
+      float* js = reinterpret_cast<float*>(smem + C::Q_BYTES);
+      constexpr int LD = D + 4;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float* dst = js + (wn * 16 + (lane >> 2) + 8 * j) * LD;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<float2*>(dst + c * 8 + 2 * (lane & 3)) = make_float2(o[c][2 * j], o[c][2 * j + 1]);
+        if ((lane & 3) == 0) dst[D] = mx[j], dst[D + 1] = sum[j];
+      }
+      __syncthreads();
+      for (int r = warp; r < 16 && r < rows; r += WM * WN) {
+        float m = -INFINITY, f[WN], l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) m = fmaxf(m, js[(w * 16 + r) * LD + D]);
+        const float b = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) {
+          f[w] = ex2_approx(js[(w * 16 + r) * LD + D] - b);
+          l += f[w] * js[(w * 16 + r) * LD + D + 1];
+        }
+        const int rr = row_base + r, tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        for (int c = lane * 2; c < D; c += 64) {
+          float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < WN; ++w) {
+            const float2 y = *reinterpret_cast<const float2*>(js + (w * 16 + r) * LD + c);
+            x.x += f[w] * y.x;
+            x.y += f[w] * y.y;
+          }
+          if (whole)
+            *reinterpret_cast<uint32_t*>(p.out + int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + c) = pack_bf16x2(x.x * inv, x.y * inv);
+          else
+            *reinterpret_cast<float2*>(part + r * (D + 2) + c) = x;
+        }
+        if (lane == 0) {
+          if (!whole)
+            part[r * (D + 2) + D] = m, part[r * (D + 2) + D + 1] = l;
+          else if (p.lse)
+            p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+        }
+      }
+      __syncthreads();  // the next unit's tiles overwrite the join
+    }
+  }
+}
+
+// Joins the parts of the units that are cut between shares.  Block (i - 1, r) looks at
+// the cut between shares i - 1 and i: where it is the first cut of its unit, the
+// block joins row r of all parts in the order of the shares (a fixed order: the
+// result does not depend on which CTA ran when).
+constexpr int AJ_WARPS = 8;
+
+template <int D, int BM>
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
+  __shared__ float sm[AJ_WARPS][D + 2];
+  const int i = blockIdx.x + 1, r = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int* metas = reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2));
+  const int* mi = metas + i * AT_META;
+  const int n = mi[0];
+  if (n < 0) return;  // no unit is cut here
+  const int before = mi[3], left = mi[4];
+  if (metas[(i - 1) * AT_META + 5] < before) return;  // the unit begins before share i - 1: not its first cut
+  const SeqLen s = seq_len(p, n);
+  const int rr = mi[2] * BM + r;
+  if (rr >= s.m * p.G) return;
+  // shares are equal but for rounding: find how many take part
+  int parts = 2;
+  for (int have = mi[5], c = i + 1; have < left; ++c, ++parts) have += metas[c * AT_META + 5];
+  constexpr int E = D / 32;
+  float m = -INFINITY, l = 0.f, x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.f;
+  for (int c = warp; c < parts; c += AJ_WARPS) {
+    const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
+    const float pm = src[D], pl = src[D + 1];
+    const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
+    const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
+    m = nm;
+    l = l * f0 + pl * f1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + src[e * 32 + lane] * f1;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sm[warp][e * 32 + lane] = x[e];
+  if (lane == 0) sm[warp][D] = m, sm[warp][D + 1] = l;
+  __syncthreads();
+  m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < AJ_WARPS; ++w) m = fmaxf(m, sm[w][D]);
+  const float b = m == -INFINITY ? 0.f : m;
+  l = 0.f;
+  float f[AJ_WARPS];
+#pragma unroll
+  for (int w = 0; w < AJ_WARPS; ++w) {
+    f[w] = ex2_approx(sm[w][D] - b);
+    l += f[w] * sm[w][D + 1];
+  }
+  const int tok = s.q0 + rr / p.G, hd = mi[1] * p.G + rr % p.G;
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  for (int c = threadIdx.x; c < D; c += AJ_WARPS * 32) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < AJ_WARPS; ++w) y += f[w] * sm[w][c];
+    p.out[int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + c] = f_to_bf16(y * inv);
+  }
+  if (p.lse && threadIdx.x == 0)
+    p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+}
+
+template <int D, int WM, int WN, int STAGES, int PER_SM>
+cudaError_t run(const AttnParams& p, cudaStream_t stream) {
+  using C = AtCfg<D, WM, WN, STAGES>;
+  static DynSmemCache cache;
+  auto kern = attn_kernel<D, WM, WN, STAGES>;
+  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
+  if (e != cudaSuccess) return e;
+  const int ctas = multiprocessor_count() * PER_SM;
+  if ((int64_t(ctas) * 2 * C::BM * (D + 2) + ctas * AT_META) * 4 > p.ws_bytes) return cudaErrorInvalidValue;
+  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int rows = int(std::min<int64_t>(C::BM, int64_t(p.max_q) * p.G));
+  attn_join_kernel<D, C::BM><<<dim3(ctas - 1, rows), AJ_WARPS * 32, 0, stream>>>(p, ctas);
+  return cudaGetLastError();
+}
+
+template <int D, int STAGES, int PER_SM>
+cudaError_t pick(const AttnParams& p, cudaStream_t stream) {
+  if (int64_t(p.max_q) * p.G <= 16) return run<D, 1, 4, STAGES, PER_SM>(p, stream);
+  return run<D, 4, 1, STAGES, PER_SM>(p, stream);
+}
+
+}  // namespace
+
+int64_t attn_workspace_bytes(int head_dim) {
+  const int64_t ctas = int64_t(multiprocessor_count()) * AT_MAX_CTAS_PER_SM;
+  return (ctas * 2 * 64 * (head_dim + 2) + ctas * AT_META) * 4;
+}
+
+cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream) {
+  if (p.D == 64) return pick<64, 3, 2>(p, stream);
+  if (p.D == 128) return pick<128, 3, 2>(p, stream);
+  return pick<256, 2, 1>(p, stream);
+}
+
+}  // namespace gdnr

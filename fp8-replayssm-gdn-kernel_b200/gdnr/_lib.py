@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 import threading
 
 import torch
@@ -126,6 +127,37 @@ class Bf16StepArgs(ctypes.Structure):
     _fields_ = [(n, Tensor) for n in ("state", "q", "k", "v", "g", "beta", "out")]
 
 
+class PrefillArgs(ctypes.Structure):
+    _fields_ = [(n, Tensor) for n in ("mixed_qkv", "a", "b", "a_log", "dt_bias", "state", "cu_seqlens",
+                                      "state_indices", "has_initial", "out")] + [
+        ("max_seqlen", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("error_flag", ctypes.c_void_p),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, Tensor) for n in ("q", "k", "v", "q_weight", "k_weight", "positions", "slots", "cos_sin", "q_out",
+                                      "k_cache", "v_cache")] + [
+        ("eps", ctypes.c_float),
+        ("weight_offset", ctypes.c_float),
+        ("interleaved", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("error_flag", ctypes.c_void_p),
+    ]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [(n, Tensor) for n in ("q", "k_cache", "v_cache", "block_table", "kv_lens", "cu_seqlens", "out",
+                                      "lse")] + [
+        ("scale", ctypes.c_float),
+        ("max_seqlen", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("error_flag", ctypes.c_void_p),
+    ]
+
+
 # symbol -> (argtypes, restype); every symbol include/gdnr.h declares
 SIGNATURES = {
     "gdnr_replay": ([ctypes.POINTER(ReplayArgs), ctypes.c_void_p], ctypes.c_int),
@@ -137,6 +169,10 @@ SIGNATURES = {
     "gdnr_quantize_vblock32": ([ctypes.POINTER(CodecArgs), ctypes.c_void_p], ctypes.c_int),
     "gdnr_dequantize_vblock32": ([ctypes.POINTER(CodecArgs), ctypes.c_void_p], ctypes.c_int),
     "gdnr_bf16_step": ([ctypes.POINTER(Bf16StepArgs), ctypes.c_void_p], ctypes.c_int),
+    "gdnr_gdn_prefill": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "gdnr_qk_norm_rope_append": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "gdnr_paged_attention": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "gdnr_paged_attention_workspace": ([ctypes.c_int32], ctypes.c_int64),
     "gdnr_last_error": ([], ctypes.c_char_p),
     "gdnr_version": ([], ctypes.c_char_p),
     "gdnr_abi_version": ([], ctypes.c_int),
@@ -207,6 +243,49 @@ def tensor_desc(t: torch.Tensor | None, require_cuda: bool = True) -> Tensor:
         d.shape[i] = s
         d.stride[i] = st
     return d
+
+
+_TENSOR_PACK = struct.Struct("@Pii8q")  # gdnr_tensor
+_ABSENT = bytes(_TENSOR_PACK.size)
+_ZEROS = tuple((0,) * (4 - n) for n in range(5))
+
+
+def pack_tensors(device_index: int, tensors) -> list[bytes]:
+    """The gdnr_tensor bytes of each tensor (None -> absent argument); all have to be on the one GPU.
+
+    The same fields as :func:`tensor_desc`, packed at once: filling a ctypes structure
+    field by field takes several microseconds a tensor, which is what a call on a few tokens
+    is made of."""
+    packed = []
+    for t in tensors:
+        if t is None:
+            packed.append(_ABSENT)
+            continue
+        if t.get_device() != device_index or device_index < 0:
+            if not t.is_cuda:
+                raise ValueError(f"libgdnr operates on CUDA tensors; got a tensor on {t.device}")
+            raise ValueError(f"tensors of one call have to be on one device; got {t.device} and cuda:{device_index}")
+        dt = _TORCH_DT.get(t.dtype)
+        if dt is None:
+            raise ValueError(f"dtype {t.dtype} is not supported by libgdnr")
+        shape = t.shape
+        n = len(shape)
+        if n > 4:
+            raise ValueError("libgdnr tensors have at most 4 dimensions")
+        packed.append(_TENSOR_PACK.pack(t.data_ptr() or 16, dt, n, *shape, *_ZEROS[n], *t.stride(), *_ZEROS[n]))
+    return packed
+
+
+def call_packed(name: str, args: bytes, device_index: int) -> None:
+    """As :func:`call`, with the argument structure as bytes."""
+    fn = getattr(load(), name)
+    if device_index == torch.cuda.current_device():
+        rc = fn(args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device_index):
+            rc = fn(args, torch.cuda.current_stream().cuda_stream)
+    if rc != OK:
+        check(rc)
 
 
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:

@@ -239,6 +239,98 @@ typedef struct {
 
 int gdnr_bf16_step(const gdnr_bf16_step_args* args, void* stream);
 
+/* ==== prompts and mixed batches of a hybrid model =========================
+ * No counterparts in the reference: what a process that serves a hybrid model
+ * (GDN layers and softmax-attention layers) calls next to the decode step above.
+ *
+ * A ragged batch of N sequences is packed: the tokens of sequence n are rows
+ * cu_seqlens[n] .. cu_seqlens[n+1]-1 of the token tensors (cu_seqlens [N+1] I32,
+ * ascending from 0; a sequence may be empty).  max_seqlen is the longest of them as far
+ * as the host knows it (0: unknown); it picks kernels and grids.  A longer sequence is
+ * reported as GDNR_DEVERR_BAD_HINT and its rows may be incomplete. */
+
+/* ---- gdnr_gdn_prefill: the gated delta rule over whole sequences ----------
+ * Per value head, token by token, with k = k_raw / sqrt(|k_raw|^2 + 1e-6), q likewise
+ * times K^-1/2, g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b):
+ *   S <- e^g S;  S <- S + beta (v - S k) k^T;  out = S q
+ * The state is float32 throughout; normalised keys are not rounded (the decode step's
+ * ring holds them in bf16).  state_indices as in gdnr_packed_decode: sequence n uses
+ * slot state_indices[n]; an index <= 0 is the null slot (out rows are zeros, no state is
+ * touched), one >= slots likewise and reported as GDNR_DEVERR_BAD_SLOT; the non-null ones
+ * must be distinct.  Without it sequence n uses slot n.  has_initial[n] == 0: the
+ * sequence starts from the zero state and its slot is only written. */
+typedef struct {
+  gdnr_tensor mixed_qkv;     /* [T, 2*H*K + HV*V] BF16, raw q | k | v */
+  gdnr_tensor a, b;          /* [T,HV] BF16|F16|F32 */
+  gdnr_tensor a_log;         /* [HV] F32 */
+  gdnr_tensor dt_bias;       /* [HV] F32 */
+  gdnr_tensor state;         /* [slots,HV,V,K] F32, in/out */
+  gdnr_tensor cu_seqlens;    /* [N+1] I32, contiguous */
+  gdnr_tensor state_indices; /* optional [N] I32 */
+  gdnr_tensor has_initial;   /* optional [N] U8 (absent: every sequence continues its slot) */
+  gdnr_tensor out;           /* [T,HV,V] BF16 */
+  int32_t max_seqlen;
+  int32_t reserved;
+  uint32_t* error_flag;
+} gdnr_prefill_args;
+
+int gdnr_gdn_prefill(const gdnr_prefill_args* args, void* stream);
+
+/* ---- gdnr_qk_norm_rope_append --------------------------------------------
+ * Per token and head: x / sqrt(mean(x^2) + eps) * (weight + weight_offset) for queries
+ * and keys (each only with its weight), the rotation of the first `rot` elements by row
+ * positions[t] of cos_sin (cos of the rot/2 angles, then sin), pairs (i, i + rot/2) or,
+ * interleaved, (2i, 2i + 1); then q to q_out, k and v to slot slots[t] (page slots[t] /
+ * page_size, row slots[t] % page_size) of the caches.  slots[t] < 0: padding, nothing
+ * is appended.  A slot past the cache sets GDNR_DEVERR_BAD_SLOT and is not
+ * written; a position outside the table sets GDNR_DEVERR_BAD_POS and leaves q and k
+ * unrotated.  Head dim D = 64, 128 or 256. */
+typedef struct {
+  gdnr_tensor q;         /* [T,Hq,D] BF16 (rows 16-byte aligned, as all below) */
+  gdnr_tensor k, v;      /* [T,Hk,D] BF16 */
+  gdnr_tensor q_weight, k_weight; /* optional [D] BF16|F32, contiguous */
+  gdnr_tensor positions; /* [T] I32 */
+  gdnr_tensor slots;     /* [T] I32, distinct where >= 0 */
+  gdnr_tensor cos_sin;   /* [P, rot] F32 */
+  gdnr_tensor q_out;     /* [T,Hq,D] BF16 (may be q itself) */
+  gdnr_tensor k_cache, v_cache; /* [pages,page_size,Hk,D] BF16, in/out */
+  float eps;
+  float weight_offset;
+  int32_t interleaved;
+  int32_t reserved;
+  uint32_t* error_flag;
+} gdnr_append_args;
+
+int gdnr_qk_norm_rope_append(const gdnr_append_args* args, void* stream);
+
+/* ---- gdnr_paged_attention --------------------------------------------------
+ * The m new tokens of a sequence (its rows of q) are the last m of its kv_lens[n]
+ * cached ones: row i attends places 0 .. kv_lens[n] - m + i (causal).  A row that
+ * sees no place is zero with lse -inf.  Query head h reads key head h / (Hq/Hk).
+ * What pages hold past a sequence's end is never used; the values of the places
+ * before it are expected to be finite.  block_table[n][j] is the page of places
+ * j*page_size ..; entries beyond the sequence's pages are not read.  A page outside the
+ * cache sets GDNR_DEVERR_BAD_SLOT and reads as zeros. */
+typedef struct {
+  gdnr_tensor q;           /* [T,Hq,D] BF16, D = 64, 128 or 256 */
+  gdnr_tensor k_cache, v_cache; /* [pages,page_size,Hk,D] BF16 */
+  gdnr_tensor block_table; /* [N,width] I32 */
+  gdnr_tensor kv_lens;     /* [N] I32 */
+  gdnr_tensor cu_seqlens;  /* [N+1] I32, contiguous */
+  gdnr_tensor out;         /* [T,Hq,D] BF16 */
+  gdnr_tensor lse;         /* optional [T,Hq] F32: log of the row's sum of exp(score) */
+  float scale;
+  int32_t max_seqlen;
+  void* workspace;         /* gdnr_paged_attention_workspace(D) bytes, 16-byte aligned, private
+                              to the call until it has run; need not be zero */
+  int64_t workspace_bytes;
+  uint32_t* error_flag;
+} gdnr_attn_args;
+
+int gdnr_paged_attention(const gdnr_attn_args* args, void* stream);
+/* Workspace bytes of gdnr_paged_attention on the current device for head dim D. */
+int64_t gdnr_paged_attention_workspace(int32_t head_dim);
+
 /* ---- misc --------------------------------------------------------------- */
 const char* gdnr_last_error(void);
 const char* gdnr_version(void);
