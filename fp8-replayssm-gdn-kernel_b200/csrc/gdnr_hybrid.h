@@ -61,6 +61,9 @@ __device__ __forceinline__ SeqRange prefill_seq(const PrefillParams& p, int n) {
 }
 
 cudaError_t launch_prefill_recurrent(const PrefillParams& p, cudaStream_t stream);
+cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream);
+// max_seqlen: 0 where the host does not know it
+cudaError_t launch_prefill(const PrefillParams& p, int max_seqlen, cudaStream_t stream);
 
 struct AppendParams {
   const uint16_t *q, *k, *v;  // [T, Hq|Hk, D] bf16

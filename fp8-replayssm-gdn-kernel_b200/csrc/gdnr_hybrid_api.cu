@@ -148,7 +148,7 @@ int gdnr_gdn_prefill(const gdnr_prefill_args* x, void* stream) {
   if (!p.err) return set_error(GDNR_ERR_CUDA, "no device error word available");
   if (n == 0) return GDNR_OK;
   if (n * HV > (int64_t(1) << 28)) return set_error(GDNR_ERR_UNSUPPORTED, "N * HV above 2^28");
-  return cuda_status(launch_prefill_recurrent(p, static_cast<cudaStream_t>(stream)), "gdnr_gdn_prefill launch");
+  return cuda_status(launch_prefill(p, x->max_seqlen, static_cast<cudaStream_t>(stream)), "gdnr_gdn_prefill launch");
 }
 
 int gdnr_qk_norm_rope_append(const gdnr_append_args* x, void* stream) {

@@ -20,6 +20,35 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t* r) {
                : "memory");
 }
 
+__device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
+               "r"(r3)
+               : "memory");
+}
+
+// Named barriers: wait for `count` threads / arrive without waiting.
+__device__ __forceinline__ void bar_sync(int id, int count) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int count) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// x as the sum of two bf16 (pairs packed): 16 bits of mantissa, an error of 2^-17 of x at most
+__device__ __forceinline__ void split_bf16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x, y);
+  const float2 h = bf16x2_to_f2(hi);
+  lo = pack_bf16x2(x - h.x, y - h.y);
+}
+
+// as the sum of three, 24 bits: float32 itself
+__device__ __forceinline__ void split3_bf16x2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = pack_bf16x2(x, y);
+  const float2 h = bf16x2_to_f2(hi);
+  const float rx = x - h.x, ry = y - h.y;
+  mid = pack_bf16x2(rx, ry);
+  const float2 m = bf16x2_to_f2(mid);
+  lo = pack_bf16x2(rx - m.x, ry - m.y);
+}
+
 // 2^x, flushing denormal results
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
