@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 // Chunks of C = 64 tokens.  With G_i the sum of the gates up to token i of the chunk, raw rows
 // K, Q, V and their inverse norms rk, rq:
 //   X = S K^T,                       R = beta (V^T - e^G rk X)
-//   N = R T^T,    T = (I + A)^-1,    A_ij = beta_i rk_i rk_j e^{G_i - G_j} k_i.k_j      (j < i)
+//   N (I + A)^T = R,                 A_ij = beta_i rk_i rk_j e^{G_i - G_j} k_i.k_j      (j < i)
 //   O = e^G rq S Q^T + N P^T,        P_ij = rq_i rk_j e^{G_i - G_j} q_i.k_j             (j <= i)
 //   S = e^{G_C} S + N diag(e^{G_C - G_j} rk_j) K
 // (N [V, C] holds the tokens' new values).  All with value rows as the rows of the matrix
@@ -140,24 +140,30 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 // from one state to the next passes through shared memory or waits for another warp.
 //
 // A CTA has 64 value rows of a head: four consumer warps of 16 rows and four producer warps
-// that load the next chunk and derive T and P of the chunk after the one being consumed.
+// that load the chunk after next and derive A and P of the next one.  N is solved for by
+// blocks of 16 tokens: the producers invert I + A's diagonal blocks, the consumers substitute
+// (N_b = R_b T_bb^T, then R_i -= N_b A_ib^T for the blocks below).
 //
-// Rounding: K, Q, V are bf16 as they come.  S, R, T, N and P meet the tensor cores as sums of
-// two bf16 (three products where both sides are split), the weighted N as a sum of three (its
-// products add up in S, which may be far smaller than their sum of sizes); this keeps the
-// float32 state within 1e-5 also where keys are alike.  The output needs it too, although it is bf16: where keys are alike, S Q^T and N P^T
-// nearly cancel, and operands rounded once left it 8e-3 off instead of 2e-3.
+// Rounding: K, Q, V are bf16 as they come.  A float32 matrix meets the tensor cores as a sum
+// of narrower ones, so that the float32 state stays within 1e-5 also where keys are alike and
+// N is what is left of large terms: S as two bf16 (against K and Q); the weighted N as
+// three (its products add up in S, which may be far smaller than their sum of
+// sizes); A, T and P, whose entries are at most about one, as two f16, and with them R and N,
+// each row brought near one by a power of two first (with two bf16 here the state was
+// 1.8e-5 off on such keys).  The output needs it too, although it is bf16: S Q^T and N P^T
+// nearly cancel there, and operands rounded once left it 8e-3 off instead of 2e-3.
 // Gates are summed in double: differences of float32 prefix sums would cancel under
 // strong decay.
 constexpr int CK_C = 64;
 constexpr int CK_ROWS = 64;
 constexpr int CK_THREADS = 256;
-constexpr int CK_LDA = 68;  // floats of a row of A and T in float32
+constexpr int CK_LDA = 20;  // floats of a row of a diagonal block
 
 struct CkTile {  // one chunk's raw rows, 16-byte chunks swizzled
   uint8_t k[CK_C * 256], q[CK_C * 256], v[CK_C * CK_ROWS * 2];
 };
 struct CkDerived {
+  // diagonal blocks of 16: T = (I + A)^-1 of the block, below them: -A
   uint8_t t_hi[CK_C * 128], t_lo[CK_C * 128], p_hi[CK_C * 128], p_lo[CK_C * 128];
   float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
   float pad[15];
@@ -165,10 +171,10 @@ struct CkDerived {
 struct CkSmem {
   CkTile tile[3];
   CkDerived der[2];
-  // A below the diagonal blocks; T's diagonal blocks in their place, its block (i, j) in block (j, i)
-  float a[CK_C * CK_LDA], y[CK_C * 20];
+  float a[CK_C * CK_LDA];  // A's diagonal blocks: warp w's at rows 16 w
   uint8_t stage[4][CK_C * 48];
   double g[CK_C];
+  float g_hi[CK_C], g_lo[CK_C];  // prefix sums of the gates in units of ln 2, in two parts
   float rk[CK_C], rq[CK_C], gbeta[CK_C];
 };
 static_assert(sizeof(CkSmem) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
@@ -196,19 +202,6 @@ __device__ __forceinline__ void ck_load(const PrefillParams& p, CkTile& tl, cons
   cp_async_commit();
 }
 
-// Four columns c..c+3 of row r of the 16 x 16 product L R (rows of both CK_LDA or ld floats apart).
-__device__ __forceinline__ void ck_mul16(const float* l, const float* rm, int ldr, float* acc) {
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const float x = l[k];
-    const float4 y = *reinterpret_cast<const float4*>(rm + k * ldr);
-    acc[0] += x * y.x;
-    acc[1] += x * y.y;
-    acc[2] += x * y.z;
-    acc[3] += x * y.w;
-  }
-}
-
 __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& r, int h, int hv, int v0, int chunks) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float neg_a = -expf(p.a_log[hv * p.al_s]), dtb = p.dt_bias[hv * p.db_s];
@@ -223,6 +216,10 @@ __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
   };
   float na, nb;
   gate_in(0, na, nb);
+  // tiles of the warp's five units; rows of units 0, 1: block warp, 4: block rb2, 2 and 3: warp 1's own, else rb2
+  const int rb2 = warp == 0 ? 3 : (warp == 1 ? 2 : warp);
+  const int unit_tile[5] = {2 * warp, 2 * warp + 1, warp < 2 ? 0 : 2 * warp - 3, warp < 2 ? 1 : 2 * warp - 2,
+                            warp == 0 ? 2 : (warp == 1 ? 0 : 2 * warp - 1)};
   for (int c = 0; c < chunks; ++c) {
     CkTile& tl = sm.tile[c % 3];
     CkDerived& dv = sm.der[c & 1];
@@ -248,96 +245,108 @@ __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
         const double y = __shfl_up_sync(0xffffffffu, x1, o);
         if (lane >= o) x0 += y, x1 += y;
       }
-      sm.g[2 * lane] = x0;
-      sm.g[2 * lane + 1] = x1;
+      // in two floats: differences of prefix sums are then exact where they matter
+      x0 *= 1.4426950408889634, x1 *= 1.4426950408889634;
+      const float h0 = float(x0), h1 = float(x1);
+      *reinterpret_cast<float2*>(&sm.g_hi[2 * lane]) = make_float2(h0, h1);
+      *reinterpret_cast<float2*>(&sm.g_lo[2 * lane]) = make_float2(float(x0 - h0), float(x1 - h1));
     }
-    {
-      // inverse norms: thread t has row t & 63 of K or Q
-      const int row = tid & 63;
-      const uint8_t* base = tid < CK_C ? tl.k : tl.q;
-      float ss = 0.f;
+    // K K^T and Q K^T on and below the diagonal: 20 tiles of 16 x 8, five a warp, the first two of them the
+    // warp's diagonal block; and Q Q^T on the diagonal.  Squared norms are diagonals.
+    float kk[5][4], qk[5][4], qq[2][4];
 #pragma unroll
-      for (int ch = 0; ch < 16; ++ch) {
-        const uint4 w = *reinterpret_cast<const uint4*>(base + swz<256>(row, ch));
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = bf16x2_to_f2(ww[i]);
-          ss += f.x * f.x + f.y * f.y;
-        }
-      }
-      (tid < CK_C ? sm.rk : sm.rq)[row] = (tid < CK_C ? 1.0f : 0.08838834764831845f) / sqrtf(ss + L2_EPS);
+      for (int j = 0; j < 5; ++j) kk[j][e] = qk[j][e] = 0.f;
+      qq[0][e] = qq[1][e] = 0.f;
     }
-    // rows 16 warp .. + 15 of K K^T and Q K^T, up to the diagonal
-    float kk[8][4], qk[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) kk[j][e] = qk[j][e] = 0.f;
     const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      uint32_t ak[4], aq[4];
-      ldsm_x4(ks + swz<256>(warp * 16 + (lane & 15), s * 2 + (lane >> 4)), ak);
-      ldsm_x4(qs + swz<256>(warp * 16 + (lane & 15), s * 2 + (lane >> 4)), aq);
+    for (int s = 0; s < 8; s += 2) {
+      uint32_t ak1[2][4], aq1[2][4], ak2[2][4], aq2[2][4], bb[5][4], bq[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j > warp) break;
-        uint32_t bb[4];
-        ldsm_x4(ks + swz<256>(j * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1)), bb);
-        mma16816_bf16(kk[2 * j], ak, bb[0], bb[1]);
-        mma16816_bf16(kk[2 * j + 1], ak, bb[2], bb[3]);
-        mma16816_bf16(qk[2 * j], aq, bb[0], bb[1]);
-        mma16816_bf16(qk[2 * j + 1], aq, bb[2], bb[3]);
+      for (int i = 0; i < 2; ++i) {
+        const int ch = (s + i) * 2 + (lane >> 4);
+        ldsm_x4(ks + swz<256>(warp * 16 + (lane & 15), ch), ak1[i]);
+        ldsm_x4(qs + swz<256>(warp * 16 + (lane & 15), ch), aq1[i]);
+        ldsm_x4(ks + swz<256>(rb2 * 16 + (lane & 15), ch), ak2[i]);
+        ldsm_x4(qs + swz<256>(rb2 * 16 + (lane & 15), ch), aq2[i]);
+        ldsm_x4(qs + swz<256>((2 * warp + i) * 8 + (lane & 7), s * 2 + (lane >> 3)), bq[i]);
       }
+#pragma unroll
+      for (int u = 0; u < 5; ++u) ldsm_x4(ks + swz<256>(unit_tile[u] * 8 + (lane & 7), s * 2 + (lane >> 3)), bb[u]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t akm[4], aqm[4];  // of units 2 and 3
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          akm[e] = warp == 1 ? ak1[i][e] : ak2[i][e];
+          aqm[e] = warp == 1 ? aq1[i][e] : aq2[i][e];
+        }
+#pragma unroll
+        for (int u = 0; u < 5; ++u) {
+          mma_bf16(kk[u], u < 2 ? ak1[i] : (u < 4 ? akm : ak2[i]), bb[u][2 * i], bb[u][2 * i + 1]);
+          mma_bf16(qk[u], u < 2 ? aq1[i] : (u < 4 ? aqm : aq2[i]), bb[u][2 * i], bb[u][2 * i + 1]);
+        }
+        mma_bf16(qq[0], aq1[i], bq[0][2 * i], bq[0][2 * i + 1]);
+        mma_bf16(qq[1], aq1[i], bq[1][2 * i], bq[1][2 * i + 1]);
+      }
+    }
+    if ((lane >> 3) == (lane & 3)) {  // the thread with elements (g, g) and (g + 8, g + 8) of its diagonal tiles
+      const int e = (lane >> 2) & 1, row = warp * 16 + (lane >> 2);
+      sm.rk[row] = 1.0f / sqrtf((e ? kk[0][1] : kk[0][0]) + L2_EPS);
+      sm.rk[row + 8] = 1.0f / sqrtf((e ? kk[1][3] : kk[1][2]) + L2_EPS);
+      sm.rq[row] = 0.08838834764831845f / sqrtf((e ? qq[0][1] : qq[0][0]) + L2_EPS);
+      sm.rq[row + 8] = 0.08838834764831845f / sqrtf((e ? qq[1][3] : qq[1][2]) + L2_EPS);
     }
     bar_sync(CK_BAR_PROD, 128);  // prefix sums and norms are in shared memory
     if (tid < CK_C) {
-      const double gi = sm.g[tid], gc = sm.g[CK_C - 1];
-      const float e = expf(float(gi)), be = sm.gbeta[tid];
+      const float gh = sm.g_hi[tid], gl = sm.g_lo[tid], ch = sm.g_hi[CK_C - 1], cl = sm.g_lo[CK_C - 1];
+      const float e = ex2_approx(gh + gl), be = sm.gbeta[tid];
       dv.beta[tid] = be;
       dv.cx[tid] = be * e * sm.rk[tid];
       dv.cq[tid] = e * sm.rq[tid];
-      dv.cs[tid] = expf(float(gc - gi)) * sm.rk[tid];
-      if (tid == 0) dv.total = expf(float(gc));
+      dv.cs[tid] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[tid];
+      if (tid == 0) dv.total = ex2_approx(ch + cl);
     }
-    {
-      const int i0 = warp * 16 + (lane >> 2);
-      const double gi[2] = {sm.g[i0], sm.g[i0 + 8]};
-      const float bk[2] = {sm.gbeta[i0] * sm.rk[i0], sm.gbeta[i0 + 8] * sm.rk[i0 + 8]}, rq[2] = {sm.rq[i0], sm.rq[i0 + 8]};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j > 2 * warp + 1) break;
-        const int col = j * 8 + 2 * (lane & 3);
-        const double gj[2] = {sm.g[col], sm.g[col + 1]};
-        const float rk[2] = {sm.rk[col], sm.rk[col + 1]};
+    for (int u = 0; u < 5; ++u) {
+      const int rb = u < 2 ? warp : (u < 4 ? (warp == 1 ? warp : rb2) : rb2);
+      const int row0 = rb * 16 + (lane >> 2), col = unit_tile[u] * 8 + 2 * (lane & 3);
+      const float2 gh = *reinterpret_cast<const float2*>(&sm.g_hi[col]), gl = *reinterpret_cast<const float2*>(&sm.g_lo[col]),
+                   rk = *reinterpret_cast<const float2*>(&sm.rk[col]);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float av[2], pv[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = i0 + 8 * hf;
-            const float d = ex2_approx(float(gi[hf] - gj[e]) * 1.4426950408889634f) * rk[e];
-            av[e] = col + e < row ? bk[hf] * d * kk[j][2 * hf + e] : 0.f;
-            pv[e] = col + e <= row ? rq[hf] * d * qk[j][2 * hf + e] : 0.f;
-          }
-          const int row = i0 + 8 * hf;
-          *reinterpret_cast<float2*>(&sm.a[row * CK_LDA + col]) = make_float2(av[0], av[1]);
-          uint32_t ph, pl;
-          split_bf16x2(pv[0], pv[1], ph, pl);
-          *reinterpret_cast<uint32_t*>(dv.p_hi + swz<128>(row, j) + 4 * (lane & 3)) = ph;
-          *reinterpret_cast<uint32_t*>(dv.p_lo + swz<128>(row, j) + 4 * (lane & 3)) = pl;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = row0 + 8 * hf;
+        const float rh = sm.g_hi[row], rl = sm.g_lo[row], bk = sm.gbeta[row] * sm.rk[row], rq = sm.rq[row];
+        const float d0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x, d1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y;
+        float a0 = bk * d0 * kk[u][2 * hf], a1 = bk * d1 * kk[u][2 * hf + 1];
+        float p0 = rq * d0 * qk[u][2 * hf], p1 = rq * d1 * qk[u][2 * hf + 1];
+        uint32_t wh, wl;
+        const uint32_t at = swz<128>(row, unit_tile[u]) + 4 * (lane & 3);
+        if (u < 2) {  // diagonal block: above the diagonal the exponentials may be anything
+          p0 = col <= row ? p0 : 0.f;
+          p1 = col + 1 <= row ? p1 : 0.f;
+          *reinterpret_cast<float2*>(&sm.a[row * CK_LDA + (col & 15)]) = make_float2(col < row ? a0 : 0.f, col + 1 < row ? a1 : 0.f);
+        } else {
+          split_f16x2(-a0, -a1, wh, wl);
+          *reinterpret_cast<uint32_t*>(dv.t_hi + at) = wh;
+          *reinterpret_cast<uint32_t*>(dv.t_lo + at) = wl;
         }
+        split_f16x2(p0, p1, wh, wl);
+        *reinterpret_cast<uint32_t*>(dv.p_hi + at) = wh;
+        *reinterpret_cast<uint32_t*>(dv.p_lo + at) = wl;
       }
     }
     __syncwarp();
-    // T = (I + A)^-1 by blocks of 16: the warp's diagonal block by substitution, lane = column
     {
+      // the warp's diagonal block of I + A inverted by substitution, lane = column (both halves of the warp alike)
+      const float* ad = sm.a + warp * 16 * CK_LDA;
+      const int cl = lane & 15;
       float x[16];
-      float* ad = sm.a + (warp * 16) * CK_LDA + warp * 16;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float s0 = i == lane ? 1.f : 0.f, s1 = 0.f;
+        float s0 = i == cl ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
         for (int j = 0; j < i; ++j) {
           if (j & 1)
@@ -347,51 +356,67 @@ __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
         }
         x[i] = s0 + s1;
       }
-      __syncwarp();
-      if (lane < 16)
+      // rows of the first half by lanes 0..15, of the second by the others
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ad[i * CK_LDA + lane] = x[i];
-    }
-    bar_sync(CK_BAR_PROD, 128);
-    // block (i, j) below: -T_ii (sum over k of A_ik T_kj), one diagonal after the other
-#pragma unroll
-    for (int d = 1; d < 4; ++d) {
-      // 64 groups of (row, four columns) a block
-      const int blocks = 4 - d;
-      for (int u = tid; u < blocks * 64; u += 128) {
-        const int bj = u >> 6, bi = bj + d, rr = (u >> 2) & 15, cc = (u & 3) * 4;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k = bj; k < bi; ++k)
-          ck_mul16(sm.a + (bi * 16 + rr) * CK_LDA + k * 16, sm.a + (bj * 16) * CK_LDA + k * 16 + cc, CK_LDA, acc);
-        *reinterpret_cast<float4*>(&sm.y[(bj * 16 + rr) * 20 + cc]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      }
-      bar_sync(CK_BAR_PROD, 128);
-      for (int u = tid; u < blocks * 64; u += 128) {
-        const int bj = u >> 6, bi = bj + d, rr = (u >> 2) & 15, cc = (u & 3) * 4;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        ck_mul16(sm.a + (bi * 16 + rr) * CK_LDA + bi * 16, sm.y + (bj * 16) * 20 + cc, 20, acc);
-        *reinterpret_cast<float4*>(&sm.a[(bj * 16 + rr) * CK_LDA + bi * 16 + cc]) =
-            make_float4(-acc[0], -acc[1], -acc[2], -acc[3]);
-      }
-      bar_sync(CK_BAR_PROD, 128);
-    }
-    // T as two bf16: thread t has half a row (what lies right of the diagonal block is never read)
-    {
-      const int row = tid >> 1, c0 = (tid & 1) * 4;
-#pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        if (c0 + ch > (row >> 4) * 2 + 1) break;
-        const int bi = row >> 4, bj = (c0 + ch) >> 1;
-        const float* src = sm.a + (bj * 16 + (row & 15)) * CK_LDA + bi * 16 + ((c0 + ch) & 1) * 8;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split_bf16x2(src[2 * i], src[2 * i + 1], hi[i], lo[i]);
-        *reinterpret_cast<uint4*>(dv.t_hi + swz<128>(row, c0 + ch)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dv.t_lo + swz<128>(row, c0 + ch)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < 8; ++i) {
+        const float v = lane < 16 ? x[i] : x[8 + i];
+        const int row = warp * 16 + i + (lane < 16 ? 0 : 8);
+        const __half hi = __float2half_rn(v);
+        const uint32_t at = swz<128>(row, warp * 2 + (cl >> 3)) + 2 * (cl & 7);
+        *reinterpret_cast<__half*>(dv.t_hi + at) = hi;
+        *reinterpret_cast<__half*>(dv.t_lo + at) = __float2half_rn(v - __half2float(hi));
       }
     }
     bar_arrive(CK_BAR_FULL + (c & 1), CK_THREADS);
   }
+}
+
+// acc [16, 64] += L M^T for L in two parts as left operands and M [64, 64] lower triangular in two parts
+// (rows of 128 bytes): hi hi + lo hi + hi lo (f16).
+__device__ __forceinline__ void ck_mul_tri(float (*acc)[4], const uint32_t (*lh)[4], const uint32_t (*ll)[4], uint32_t mh, uint32_t ml,
+                                           int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t b[4][4], bl[4][4];
+#pragma unroll
+    for (int i = j; i < 4; ++i) {
+      const uint32_t off = swz<128>(i * 16 + ((lane >> 4) << 3) + (lane & 7), j * 2 + ((lane >> 3) & 1));
+      ldsm_x4(mh + off, b[i]);
+      ldsm_x4(ml + off, bl[i]);
+    }
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+#pragma unroll
+      for (int i = 2 * j; i < 8; ++i) {
+        const uint32_t* w = part == 2 ? bl[i >> 1] : b[i >> 1];
+        mma_f16(acc[i], part == 1 ? ll[j] : lh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
+      }
+  }
+}
+
+// Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
+__device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
+  split_bf16x2(x[0][0], x[0][1], hi[0], lo[0]);
+  split_bf16x2(x[0][2], x[0][3], hi[1], lo[1]);
+  split_bf16x2(x[1][0], x[1][1], hi[2], lo[2]);
+  split_bf16x2(x[1][2], x[1][3], hi[3], lo[3]);
+}
+
+__device__ __forceinline__ void ck_left_f16(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
+  split_f16x2(x[0][0], x[0][1], hi[0], lo[0]);
+  split_f16x2(x[0][2], x[0][3], hi[1], lo[1]);
+  split_f16x2(x[1][0], x[1][1], hi[2], lo[2]);
+  split_f16x2(x[1][2], x[1][3], hi[3], lo[3]);
+}
+
+// A power of two that brings a row's largest value (over the four lanes that hold the row) into
+// [2^4, 2^5), and its inverse
+__device__ __forceinline__ void ck_row_scale(float top, float& up, float& down) {
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int e = min(max(int(__float_as_uint(top) >> 23), 8), 250);
+  up = __uint_as_float(uint32_t(258 - e) << 23);
+  down = __uint_as_float(uint32_t(e - 4) << 23);
 }
 
 __device__ void ck_consumer(const PrefillParams& p, CkSmem& sm, const SeqRange& r, int hv, int v0, int chunks, bool fresh) {
@@ -425,28 +450,28 @@ __device__ void ck_consumer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       uint32_t hi[4], lo[4];
-      split_bf16x2(S[2 * s][0], S[2 * s][1], hi[0], lo[0]);
-      split_bf16x2(S[2 * s][2], S[2 * s][3], hi[1], lo[1]);
-      split_bf16x2(S[2 * s + 1][0], S[2 * s + 1][1], hi[2], lo[2]);
-      split_bf16x2(S[2 * s + 1][2], S[2 * s + 1][3], hi[3], lo[3]);
+      ck_left(S + 2 * s, hi, lo);
+      // products that add to the same tile are kept eight apart: one takes about four times as long as it keeps the unit
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t b[4];
-        const uint32_t off = swz<256>(j * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1));
-        ldsm_x4(ks + off, b);
-        mma16816_bf16(X[2 * j], hi, b[0], b[1]);
-        mma16816_bf16(X[2 * j + 1], hi, b[2], b[3]);
-        mma16816_bf16(X[2 * j], lo, b[0], b[1]);
-        mma16816_bf16(X[2 * j + 1], lo, b[2], b[3]);
-        ldsm_x4(qs + off, b);
-        mma16816_bf16(O[2 * j], hi, b[0], b[1]);
-        mma16816_bf16(O[2 * j + 1], hi, b[2], b[3]);
-        mma16816_bf16(O[2 * j], lo, b[0], b[1]);
-        mma16816_bf16(O[2 * j + 1], lo, b[2], b[3]);
+      for (int jj = 0; jj < 4; jj += 2) {
+        uint32_t bk[2][4], bq[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t off = swz<256>((jj + j) * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1));
+          ldsm_x4(ks + off, bk[j]);
+          ldsm_x4(qs + off, bq[j]);
+        }
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_bf16(X[2 * jj + j], part ? lo : hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
+            mma_bf16(O[2 * jj + j], part ? lo : hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+          }
       }
     }
-    // R = beta V^T - (beta e^G rk) X, and its halves as the left operand
-    uint32_t rh[4][4], rl[4][4];
+    // R = beta V^T - (beta e^G rk) X
+    float top0 = 0.f, top1 = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t w[4];  // tokens 16j + t2 (+1), rows g and g + 8; tokens 16j + 8 + t2
@@ -459,40 +484,54 @@ __device__ void ck_consumer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
         const float2 v0f = bf16x2_to_f2(w[2 * hf]), v1f = bf16x2_to_f2(w[2 * hf + 1]);
         float* x = X[2 * j + hf];
         float* o = O[2 * j + hf];
-        split_bf16x2(be.x * v0f.x - cx.x * x[0], be.y * v0f.y - cx.y * x[1], rh[j][2 * hf], rl[j][2 * hf]);
-        split_bf16x2(be.x * v1f.x - cx.x * x[2], be.y * v1f.y - cx.y * x[3], rh[j][2 * hf + 1], rl[j][2 * hf + 1]);
+        x[0] = be.x * v0f.x - cx.x * x[0], x[1] = be.y * v0f.y - cx.y * x[1];
+        x[2] = be.x * v1f.x - cx.x * x[2], x[3] = be.y * v1f.y - cx.y * x[3];
+        top0 = fmaxf(top0, fmaxf(fabsf(x[0]), fabsf(x[1])));
+        top1 = fmaxf(top1, fmaxf(fabsf(x[2]), fabsf(x[3])));
         o[0] *= cq.x, o[1] *= cq.y, o[2] *= cq.x, o[3] *= cq.y;
       }
     }
+    // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
+    float up0, down0, up1, down1;
+    ck_row_scale(top0, up0, down0);
+    ck_row_scale(top1, up1, down1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      X[j][0] *= up0, X[j][1] *= up0, X[j][2] *= up1, X[j][3] *= up1;
+      O[j][0] *= up0, O[j][1] *= up0, O[j][2] *= up1, O[j][3] *= up1;
+    }
     float N[8][4];
+    uint32_t nh[4][4], nl[4][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) N[j][e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      // column j of blocks: T_jj, then -A_ij below it
+      uint32_t b[4][4], bl[4][4], rh[4], rl[4];
 #pragma unroll
       for (int i = j; i < 4; ++i) {
-        uint32_t b[4], bl[4];
         const uint32_t off = swz<128>(i * 16 + ((lane >> 4) << 3) + (lane & 7), j * 2 + ((lane >> 3) & 1));
-        ldsm_x4(th + off, b);
-        ldsm_x4(tlo + off, bl);
-        mma16816_bf16(N[2 * i], rh[j], b[0], b[1]);
-        mma16816_bf16(N[2 * i + 1], rh[j], b[2], b[3]);
-        mma16816_bf16(N[2 * i], rl[j], b[0], b[1]);
-        mma16816_bf16(N[2 * i + 1], rl[j], b[2], b[3]);
-        mma16816_bf16(N[2 * i], rh[j], bl[0], bl[1]);
-        mma16816_bf16(N[2 * i + 1], rh[j], bl[2], bl[3]);
+        ldsm_x4(th + off, b[i]);
+        ldsm_x4(tlo + off, bl[i]);
       }
-    // the state first: the next chunk waits for it
-    uint32_t nh[4][4], nl[4][4];
+      ck_left_f16(X + 2 * j, rh, rl);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      split_bf16x2(N[2 * j][0], N[2 * j][1], nh[j][0], nl[j][0]);
-      split_bf16x2(N[2 * j][2], N[2 * j][3], nh[j][1], nl[j][1]);
-      split_bf16x2(N[2 * j + 1][0], N[2 * j + 1][1], nh[j][2], nl[j][2]);
-      split_bf16x2(N[2 * j + 1][2], N[2 * j + 1][3], nh[j][3], nl[j][3]);
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          mma_f16(N[2 * j + i], part == 1 ? rl : rh, (part == 2 ? bl : b)[j][2 * i], (part == 2 ? bl : b)[j][2 * i + 1]);
+      ck_left_f16(N + 2 * j, nh[j], nl[j]);
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int i = 2 * j + 2; i < 8; ++i) {
+          const uint32_t* w = (part == 2 ? bl : b)[i >> 1];
+          mma_f16(X[i], part == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
+        }
     }
+    // the state first: the next chunk waits for it
     const float total = dv.total;
 #pragma unroll
     for (int n = 0; n < 16; ++n)
@@ -505,43 +544,29 @@ __device__ void ck_consumer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
       for (int hf = 0; hf < 2; ++hf) {
         const float2 cs = *reinterpret_cast<const float2*>(&dv.cs[j * 16 + hf * 8 + t2]);
         const float* x = N[2 * j + hf];
-        split3_bf16x2(x[0] * cs.x, x[1] * cs.y, hi[2 * hf], lo[2 * hf], rest[2 * hf]);
-        split3_bf16x2(x[2] * cs.x, x[3] * cs.y, hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
+        split3_bf16x2(x[0] * (cs.x * down0), x[1] * (cs.y * down0), hi[2 * hf], lo[2 * hf], rest[2 * hf]);
+        split3_bf16x2(x[2] * (cs.x * down1), x[3] * (cs.y * down1), hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
       }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        uint32_t b[4];
-        ldsm_x4_t(ks + swz<256>(j * 16 + (lane & 15), n * 2 + (lane >> 4)), b);
-        mma16816_bf16(S[2 * n], hi, b[0], b[1]);
-        mma16816_bf16(S[2 * n + 1], hi, b[2], b[3]);
-        mma16816_bf16(S[2 * n], lo, b[0], b[1]);
-        mma16816_bf16(S[2 * n + 1], lo, b[2], b[3]);
-        mma16816_bf16(S[2 * n], rest, b[0], b[1]);
-        mma16816_bf16(S[2 * n + 1], rest, b[2], b[3]);
+      for (int nn = 0; nn < 8; nn += 4) {
+        uint32_t b[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) ldsm_x4_t(ks + swz<256>(j * 16 + (lane & 15), (nn + n) * 2 + (lane >> 4)), b[n]);
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            mma_bf16(S[2 * nn + n], part == 0 ? hi : (part == 1 ? lo : rest), b[n >> 1][2 * (n & 1)], b[n >> 1][2 * (n & 1) + 1]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = j; i < 4; ++i) {
-        uint32_t b[4], bl[4];
-        const uint32_t off = swz<128>(i * 16 + ((lane >> 4) << 3) + (lane & 7), j * 2 + ((lane >> 3) & 1));
-        ldsm_x4(ph + off, b);
-        ldsm_x4(pl + off, bl);
-        mma16816_bf16(O[2 * i], nh[j], b[0], b[1]);
-        mma16816_bf16(O[2 * i + 1], nh[j], b[2], b[3]);
-        mma16816_bf16(O[2 * i], nl[j], b[0], b[1]);
-        mma16816_bf16(O[2 * i + 1], nl[j], b[2], b[3]);
-        mma16816_bf16(O[2 * i], nh[j], bl[0], bl[1]);
-        mma16816_bf16(O[2 * i + 1], nh[j], bl[2], bl[3]);
-      }
+    ck_mul_tri(O, nh, nl, ph, pl, lane);
     if (c + 2 < chunks) bar_arrive(CK_BAR_EMPTY + (c & 1), CK_THREADS);
     // O^T to token rows through the warp's own staging rows (48 bytes apart: no bank twice)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      stsm_x4_t(stage + (j * 16 + ((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, pack_bf16x2(O[2 * j][0], O[2 * j][1]),
-                pack_bf16x2(O[2 * j][2], O[2 * j][3]), pack_bf16x2(O[2 * j + 1][0], O[2 * j + 1][1]),
-                pack_bf16x2(O[2 * j + 1][2], O[2 * j + 1][3]));
+      stsm_x4_t(stage + (j * 16 + ((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, cvt_bf16x2(O[2 * j][0] * down0, O[2 * j][1] * down0),
+                cvt_bf16x2(O[2 * j][2] * down1, O[2 * j][3] * down1), cvt_bf16x2(O[2 * j + 1][0] * down0, O[2 * j + 1][1] * down0),
+                cvt_bf16x2(O[2 * j + 1][2] * down1, O[2 * j + 1][3] * down1));
     __syncwarp();
     const int t0 = r.begin + c * CK_C;
 #pragma unroll

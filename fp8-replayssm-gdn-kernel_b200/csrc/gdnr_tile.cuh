@@ -20,6 +20,19 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t* r) {
                : "memory");
 }
 
+// d += a b (m16n8k16, bf16).  Not volatile: the compiler may move it between the loads around it.
+__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
                "r"(r3)
@@ -32,21 +45,36 @@ __device__ __forceinline__ void bar_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
+// two floats to packed bf16 (x in the low half), one conversion
+__device__ __forceinline__ uint32_t cvt_bf16x2(float x, float y) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+
 // x as the sum of two bf16 (pairs packed): 16 bits of mantissa, an error of 2^-17 of x at most
 __device__ __forceinline__ void split_bf16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(x, y);
+  hi = cvt_bf16x2(x, y);
   const float2 h = bf16x2_to_f2(hi);
-  lo = pack_bf16x2(x - h.x, y - h.y);
+  lo = cvt_bf16x2(x - h.x, y - h.y);
+}
+
+// as the sum of two f16: 22 bits of mantissa, for values that are not far below one or above 2^15
+__device__ __forceinline__ void split_f16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack_f16x2(x - f.x, y - f.y);
 }
 
 // as the sum of three, 24 bits: float32 itself
 __device__ __forceinline__ void split3_bf16x2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  hi = pack_bf16x2(x, y);
+  hi = cvt_bf16x2(x, y);
   const float2 h = bf16x2_to_f2(hi);
   const float rx = x - h.x, ry = y - h.y;
-  mid = pack_bf16x2(rx, ry);
+  mid = cvt_bf16x2(rx, ry);
   const float2 m = bf16x2_to_f2(mid);
-  lo = pack_bf16x2(rx - m.x, ry - m.y);
+  lo = cvt_bf16x2(rx - m.x, ry - m.y);
 }
 
 // 2^x, flushing denormal results
