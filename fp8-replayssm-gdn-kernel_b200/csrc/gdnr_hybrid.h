@@ -4,6 +4,7 @@
 // (gdnr_attn.cu).  Strides are in elements.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -34,8 +35,11 @@ struct PrefillParams {
   uint16_t* out;  // [T, HV, V] bf16
   int64_t o_st, o_sh;
   int32_t N, H, HV, S, T;
+  uint8_t* images;  // chunked form: workspace, CK_IMAGE_BYTES a chunk and value head
   uint32_t* err;
 };
+
+constexpr int CK_IMAGE_BYTES = 21568;
 
 // Tokens [begin, end) of sequence n and the slot of its state; returns false for a
 // null or out-of-range slot (rows become zeros, no state is touched).
@@ -63,6 +67,7 @@ __device__ __forceinline__ SeqRange prefill_seq(const PrefillParams& p, int n) {
 cudaError_t launch_prefill_recurrent(const PrefillParams& p, cudaStream_t stream);
 cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream);
 // max_seqlen: 0 where the host does not know it
+int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen);
 cudaError_t launch_prefill(const PrefillParams& p, int max_seqlen, cudaStream_t stream);
 
 struct AppendParams {
@@ -112,5 +117,9 @@ int64_t attn_workspace_bytes(int head_dim);
 cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream);
 
 int multiprocessor_count();
+
+// Tiled map of a bf16 tensor, 128-byte swizzle (boxes of 64 innermost elements); strides in bytes, without the innermost.
+cudaError_t encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                            const uint32_t* box);
 
 }  // namespace gdnr

@@ -23,6 +23,30 @@ int multiprocessor_count() {
   return n;
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                            const uint32_t* box) {
+  static std::atomic<EncodeFn> fn{nullptr};
+  EncodeFn enc = fn.load(std::memory_order_acquire);
+  if (!enc) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return cudaErrorNotSupported;
+    enc = reinterpret_cast<EncodeFn>(ptr);
+    fn.store(enc, std::memory_order_release);
+  }
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace gdnr
 
 namespace {
@@ -148,7 +172,16 @@ int gdnr_gdn_prefill(const gdnr_prefill_args* x, void* stream) {
   if (!p.err) return set_error(GDNR_ERR_CUDA, "no device error word available");
   if (n == 0) return GDNR_OK;
   if (n * HV > (int64_t(1) << 28)) return set_error(GDNR_ERR_UNSUPPORTED, "N * HV above 2^28");
+  const int64_t need = prefill_workspace_bytes(T, n, HV, x->max_seqlen);
+  p.images = static_cast<uint8_t*>(x->workspace);
+  if (need > 0 && (!p.images || reinterpret_cast<uintptr_t>(p.images) % 16 || x->workspace_bytes < need))
+    return set_error(GDNR_ERR_ARG, "workspace: needs %lld bytes at a 16-byte aligned address", (long long)need);
+  if ((T / 64 + n) * H > (int64_t(1) << 30)) return set_error(GDNR_ERR_UNSUPPORTED, "T / 64 * H above 2^30");
   return cuda_status(launch_prefill(p, x->max_seqlen, static_cast<cudaStream_t>(stream)), "gdnr_gdn_prefill launch");
+}
+
+int64_t gdnr_gdn_prefill_workspace(int64_t tokens, int64_t sequences, int32_t value_heads, int32_t max_seqlen) {
+  return prefill_workspace_bytes(tokens, sequences, value_heads, max_seqlen);
 }
 
 int gdnr_qk_norm_rope_append(const gdnr_append_args* x, void* stream) {

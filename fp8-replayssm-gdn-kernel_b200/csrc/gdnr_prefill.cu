@@ -134,14 +134,15 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 //   N (I + A)^T = R,                 A_ij = beta_i rk_i rk_j e^{G_i - G_j} k_i.k_j      (j < i)
 //   O = e^G rq S Q^T + N P^T,        P_ij = rq_i rk_j e^{G_i - G_j} q_i.k_j             (j <= i)
 //   S = e^{G_C} S + N diag(e^{G_C - G_j} rk_j) K
-// (N [V, C] holds the tokens' new values).  All with value rows as the rows of the matrix
-// products, so a warp that owns 16 value rows of S keeps S, X, R and N in registers: the
-// accumulators of one product are the left operand of the next, and nothing of the chain
-// from one state to the next passes through shared memory or waits for another warp.
+// (N [V, C] holds the tokens' new values).
 //
-// A CTA has 64 value rows of a head: four consumer warps of 16 rows and four producer warps
-// that load the chunk after next and derive A and P of the next one.  N is solved for by
-// blocks of 16 tokens: the producers invert I + A's diagonal blocks, the consumers substitute
+// Two kernels.  The first makes what does not depend on the state, for all chunks at once: A with
+// its diagonal blocks of 16 tokens inverted, P, and the factors of each token, an image of
+// 21 KB a chunk and head in the layout the second one's shared memory has.  The second
+// walks the chunks of a sequence.  It has value rows as the rows of the matrix products: a
+// warp that owns 16 value rows of S keeps S, X, R and N in registers, the accumulators of one
+// product are the left operand of the next, and nothing of the chain from one state to
+// the next passes through shared memory or waits for another warp.  N is solved for by blocks
 // (N_b = R_b T_bb^T, then R_i -= N_b A_ib^T for the blocks below).
 //
 // Rounding: K, Q, V are bf16 as they come.  A float32 matrix meets the tensor cores as a sum
@@ -155,193 +156,228 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 // Gates are summed in double: differences of float32 prefix sums would cancel under
 // strong decay.
 constexpr int CK_C = 64;
-constexpr int CK_ROWS = 64;
-constexpr int CK_THREADS = 256;
-constexpr int CK_LDA = 20;  // floats of a row of a diagonal block
 
-struct CkTile {  // one chunk's raw rows, 16-byte chunks swizzled
-  uint8_t k[CK_C * 256], q[CK_C * 256], v[CK_C * CK_ROWS * 2];
-};
-struct CkDerived {
-  // diagonal blocks of 16: T = (I + A)^-1 of the block, below them: -A
-  uint8_t t_hi[CK_C * 128], t_lo[CK_C * 128], p_hi[CK_C * 128], p_lo[CK_C * 128];
+// Lower triangular [C, C] of f16 as its ten blocks of 16 x 16, rows of 32 bytes whose two
+// 16-byte halves change places every four rows (eight rows' equal halves cover all banks).
+constexpr int CK_TRI = 10 * 512;
+__host__ __device__ constexpr int ck_block(int i, int j) { return (i * (i + 1) / 2 + j) * 512; }
+__device__ __forceinline__ uint32_t ck_in_block(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
+
+struct CkImage {
+  // diagonal blocks: T = (I + A)^-1 of the block, below them: -A
+  uint8_t t_hi[CK_TRI], t_lo[CK_TRI], p_hi[CK_TRI], p_lo[CK_TRI];
   float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
   float pad[15];
 };
-struct CkSmem {
-  CkTile tile[3];
-  CkDerived der[2];
-  float a[CK_C * CK_LDA];  // A's diagonal blocks: warp w's at rows 16 w
-  uint8_t stage[4][CK_C * 48];
+static_assert(sizeof(CkImage) == CK_IMAGE_BYTES && sizeof(CkImage) % 16 == 0, "copied in bulk");
+
+// 64 rows of 128 bf16 as two TMA boxes of 64 columns, 128-byte swizzle: 16-byte chunk c of row r
+__device__ __forceinline__ uint32_t ck_at(int row, int c) { return uint32_t(c >> 3) * 8192u + swz<128>(row, c & 7); }
+
+__device__ __forceinline__ void ck_tma(uint32_t dst, const CUtensorMap* map, int col, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(row), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// The chunks of sequence n have the numbers ck_first(n) ..; they do not overlap, and end below T / C + N.
+__device__ __forceinline__ int ck_first(int begin, int n) { return begin / CK_C + n; }
+
+// Rows from `valid` on of a tile: what lies past the sequence's end belongs to others (it may be NaN)
+__device__ __forceinline__ void ck_zero_rows(uint8_t* tile, int boxes, int valid, int tid, int threads) {
+  for (int i = tid; i < boxes * (CK_C - valid) * 8; i += threads) {
+    const int box = i / ((CK_C - valid) * 8), j = i % ((CK_C - valid) * 8);
+    *reinterpret_cast<uint4*>(tile + box * 8192 + (valid + j / 8) * 128 + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------- chunked form, first kernel
+constexpr int CD_THREADS = 256;
+constexpr int CD_LDA = 20;  // floats of a row of a diagonal block
+
+struct CdSmem {
+  uint8_t k[CK_C * 256], q[CK_C * 256];
+  CkImage img[2];
+  float a[CK_C * CD_LDA];  // -A's diagonal blocks: warp w's at rows 16 w
   double g[CK_C];
   float g_hi[CK_C], g_lo[CK_C];  // prefix sums of the gates in units of ln 2, in two parts
   float rk[CK_C], rq[CK_C], gbeta[CK_C];
+  uint64_t bar;
 };
-static_assert(sizeof(CkSmem) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
 
-enum { CK_BAR_PROD = 1, CK_BAR_FULL = 2, CK_BAR_EMPTY = 4 };
-
-__device__ __forceinline__ void ck_load(const PrefillParams& p, CkTile& tl, const SeqRange& r, int c, int h, int hv, int v0, int tid) {
-  const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v);
-  const int t0 = r.begin + c * CK_C;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = (tid >> 4) + i * 8, ch = tid & 15;
-    const bool ok = t0 + row < r.end;
-    const uint16_t* m = p.mixed + int64_t(ok ? t0 + row : r.begin) * p.mx_s + ch * 8;
-    cp_async16_zfill(qs + swz<256>(row, ch), m + h * 128, ok ? 16 : 0);
-    cp_async16_zfill(ks + swz<256>(row, ch), m + (p.H + h) * 128, ok ? 16 : 0);
+// One CTA a chunk and key head; its value heads share the products of the raw rows.  The first
+// four warps make A (rows of K against K) and invert its diagonal blocks, the others make P
+// (rows of Q against K), the gates and the factors.
+__global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __grid_constant__ PrefillParams p,
+                                                                       const __grid_constant__ CUtensorMap map) {
+  extern __shared__ uint8_t raw[];
+  CdSmem& sm = *reinterpret_cast<CdSmem*>(raw + (-smem_addr(raw) & 1023u));
+  const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3;
+  const int id = blockIdx.x / p.H, h = blockIdx.x - id * p.H, group = p.HV / p.H;
+  // the last sequence whose first chunk is not after this one
+  int lo = 0, hi = p.N - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (ck_first(min(max(p.cu[mid], 0), p.T), mid) <= id)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (tid >> 3) + i * 16, ch = tid & 7;
-    const bool ok = t0 + row < r.end;
-    cp_async16_zfill(vs + swz<128>(row, ch), p.mixed + int64_t(ok ? t0 + row : r.begin) * p.mx_s + (2 * p.H + hv) * 128 + v0 + ch * 8,
-                     ok ? 16 : 0);
-  }
-  cp_async_commit();
-}
+  const int n = lo;
+  const SeqRange r = prefill_seq(p, n);
+  const int c = id - ck_first(r.begin, n);
+  if (r.slot < 0 || c < 0 || r.begin + c * CK_C >= r.end) return;
+  const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
 
-__device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& r, int h, int hv, int v0, int chunks) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const float neg_a = -expf(p.a_log[hv * p.al_s]), dtb = p.dt_bias[hv * p.db_s];
-  ck_load(p, sm.tile[0], r, 0, h, hv, v0, tid);
-  auto gate_in = [&](int c, float& a, float& b) {
-    const int t = r.begin + c * CK_C + tid;
+  if (tid == 0) {
+    mbar_init(&sm.bar, 1);
+    fence_mbar_init();
+    mbar_arrive_expect_tx(&sm.bar, 2 * CK_C * 256);
+    for (int b = 0; b < 2; ++b) {
+      ck_tma(smem_addr(sm.q) + b * 8192, &map, h * 128 + b * 64, t0, &sm.bar);
+      ck_tma(smem_addr(sm.k) + b * 8192, &map, (p.H + h) * 128 + b * 64, t0, &sm.bar);
+    }
+  }
+  const bool of_q = tid >= 128;
+  const int gt = tid - 128;  // token whose gates this thread makes, where in [0, C)
+  const bool gates = gt >= 0 && gt < CK_C;
+  auto gate_in = [&](int hv, float& a, float& b) {
     a = b = 0.f;
-    if (tid < CK_C && c < chunks && t < r.end) {
-      a = load_scalar(p.a, int64_t(t) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt);
-      b = load_scalar(p.b, int64_t(t) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt);
+    if (gates && gt < valid) {
+      a = load_scalar(p.a, int64_t(t0 + gt) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt) + p.dt_bias[hv * p.db_s];
+      b = load_scalar(p.b, int64_t(t0 + gt) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt);
     }
   };
   float na, nb;
-  gate_in(0, na, nb);
-  // tiles of the warp's five units; rows of units 0, 1: block warp, 4: block rb2, 2 and 3: warp 1's own, else rb2
+  gate_in(h * group, na, nb);
+  __syncthreads();  // the barrier is initialised
+  const bool ok = mbar_wait_bounded(&sm.bar, 0, p.err);
+  if (__syncthreads_or(!ok)) return;
+  if (valid < CK_C) {
+    ck_zero_rows(sm.k, 2, valid, tid, CD_THREADS);
+    ck_zero_rows(sm.q, 2, valid, tid, CD_THREADS);
+    __syncthreads();
+  }
+  // K K^T or Q K^T on and below the diagonal: 20 tiles of 16 x 8, five a warp, the first two of them the warp's
+  // diagonal block; rows of units 0, 1: block warp, 4: block rb2, 2 and 3: warp 1's own, else rb2.  And Q Q^T on
+  // the diagonal.  Squared norms are diagonals.
   const int rb2 = warp == 0 ? 3 : (warp == 1 ? 2 : warp);
   const int unit_tile[5] = {2 * warp, 2 * warp + 1, warp < 2 ? 0 : 2 * warp - 3, warp < 2 ? 1 : 2 * warp - 2,
                             warp == 0 ? 2 : (warp == 1 ? 0 : 2 * warp - 1)};
-  for (int c = 0; c < chunks; ++c) {
-    CkTile& tl = sm.tile[c % 3];
-    CkDerived& dv = sm.der[c & 1];
-    if (c >= 2) bar_sync(CK_BAR_EMPTY + (c & 1), CK_THREADS);  // the consumers are done with chunk c - 2
+  float m[5][4], qq[2][4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) m[j][e] = 0.f;
+    qq[0][e] = qq[1][e] = 0.f;
+  }
+  const uint32_t ks = smem_addr(sm.k), qs = smem_addr(sm.q), as = of_q ? qs : ks;
+#pragma unroll
+  for (int s = 0; s < 8; s += 2) {
+    uint32_t a1[2][4], a2[2][4], bb[5][4], bq[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int ch = (s + i) * 2 + (lane >> 4);
+      ldsm_x4(as + ck_at(warp * 16 + (lane & 15), ch), a1[i]);
+      ldsm_x4(as + ck_at(rb2 * 16 + (lane & 15), ch), a2[i]);
+    }
+#pragma unroll
+    for (int u = 0; u < 5; ++u) ldsm_x4(ks + ck_at(unit_tile[u] * 8 + (lane & 7), s * 2 + (lane >> 3)), bb[u]);
+    if (of_q) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ldsm_x4(qs + ck_at((2 * warp + i) * 8 + (lane & 7), s * 2 + (lane >> 3)), bq[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_bf16(qq[0], a1[i], bq[0][2 * i], bq[0][2 * i + 1]);
+        mma_bf16(qq[1], a1[i], bq[1][2 * i], bq[1][2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t am[4];  // of units 2 and 3
+#pragma unroll
+      for (int e = 0; e < 4; ++e) am[e] = warp == 1 ? a1[i][e] : a2[i][e];
+#pragma unroll
+      for (int u = 0; u < 5; ++u) mma_bf16(m[u], u < 2 ? a1[i] : (u < 4 ? am : a2[i]), bb[u][2 * i], bb[u][2 * i + 1]);
+    }
+  }
+  if ((lane >> 3) == (lane & 3)) {  // the thread with elements (g, g) and (g + 8, g + 8) of its diagonal tiles
+    const int e = (lane >> 2) & 1, row = warp * 16 + (lane >> 2);
+    const float x0 = of_q ? (e ? qq[0][1] : qq[0][0]) : (e ? m[0][1] : m[0][0]);
+    const float x1 = of_q ? (e ? qq[1][3] : qq[1][2]) : (e ? m[1][3] : m[1][2]);
+    const float gain = of_q ? 0.08838834764831845f : 1.0f;
+    (of_q ? sm.rq : sm.rk)[row] = gain * rsqrtf(x0 + L2_EPS);
+    (of_q ? sm.rq : sm.rk)[row + 8] = gain * rsqrtf(x1 + L2_EPS);
+  }
+  for (int e = 0; e < group; ++e) {
+    const int hv = h * group + e;
+    CkImage& img = sm.img[e & 1];
     const float a = na, b = nb;
-    if (c + 1 < chunks)
-      ck_load(p, sm.tile[(c + 1) % 3], r, c + 1, h, hv, v0, tid);
-    else
-      cp_async_commit();
-    gate_in(c + 1, na, nb);
-    // gates; tokens past the end neither decay nor write
-    if (tid < CK_C) {
-      const bool in = r.begin + c * CK_C + tid < r.end;
-      sm.g[tid] = in ? double(neg_a * softplus_gate(a + dtb)) : 0.0;
-      sm.gbeta[tid] = in ? sigmoid_f(b) : 0.f;
-    }
-    cp_async_wait<1>();
-    bar_sync(CK_BAR_PROD, 128);
-    if (warp == 0) {
-      double x0 = sm.g[2 * lane], x1 = x0 + sm.g[2 * lane + 1];
+    if (e + 1 < group) gate_in(hv + 1, na, nb);
+    if (gates) {  // tokens past the end neither decay nor write
+      sm.g[gt] = gt < valid ? double(-expf(p.a_log[hv * p.al_s]) * softplus_gate(a)) : 0.0;
+      sm.gbeta[gt] = gt < valid ? sigmoid_f(b) : 0.f;
+      bar_sync(1, CK_C);
+      if (warp == 0) {
+        double x0 = sm.g[2 * lane], x1 = x0 + sm.g[2 * lane + 1];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, x1, o);
-        if (lane >= o) x0 += y, x1 += y;
-      }
-      // in two floats: differences of prefix sums are then exact where they matter
-      x0 *= 1.4426950408889634, x1 *= 1.4426950408889634;
-      const float h0 = float(x0), h1 = float(x1);
-      *reinterpret_cast<float2*>(&sm.g_hi[2 * lane]) = make_float2(h0, h1);
-      *reinterpret_cast<float2*>(&sm.g_lo[2 * lane]) = make_float2(float(x0 - h0), float(x1 - h1));
-    }
-    // K K^T and Q K^T on and below the diagonal: 20 tiles of 16 x 8, five a warp, the first two of them the
-    // warp's diagonal block; and Q Q^T on the diagonal.  Squared norms are diagonals.
-    float kk[5][4], qk[5][4], qq[2][4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-      for (int j = 0; j < 5; ++j) kk[j][e] = qk[j][e] = 0.f;
-      qq[0][e] = qq[1][e] = 0.f;
-    }
-    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q);
-#pragma unroll
-    for (int s = 0; s < 8; s += 2) {
-      uint32_t ak1[2][4], aq1[2][4], ak2[2][4], aq2[2][4], bb[5][4], bq[2][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ch = (s + i) * 2 + (lane >> 4);
-        ldsm_x4(ks + swz<256>(warp * 16 + (lane & 15), ch), ak1[i]);
-        ldsm_x4(qs + swz<256>(warp * 16 + (lane & 15), ch), aq1[i]);
-        ldsm_x4(ks + swz<256>(rb2 * 16 + (lane & 15), ch), ak2[i]);
-        ldsm_x4(qs + swz<256>(rb2 * 16 + (lane & 15), ch), aq2[i]);
-        ldsm_x4(qs + swz<256>((2 * warp + i) * 8 + (lane & 7), s * 2 + (lane >> 3)), bq[i]);
-      }
-#pragma unroll
-      for (int u = 0; u < 5; ++u) ldsm_x4(ks + swz<256>(unit_tile[u] * 8 + (lane & 7), s * 2 + (lane >> 3)), bb[u]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t akm[4], aqm[4];  // of units 2 and 3
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          akm[e] = warp == 1 ? ak1[i][e] : ak2[i][e];
-          aqm[e] = warp == 1 ? aq1[i][e] : aq2[i][e];
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, x1, o);
+          if (lane >= o) x0 += y, x1 += y;
         }
-#pragma unroll
-        for (int u = 0; u < 5; ++u) {
-          mma_bf16(kk[u], u < 2 ? ak1[i] : (u < 4 ? akm : ak2[i]), bb[u][2 * i], bb[u][2 * i + 1]);
-          mma_bf16(qk[u], u < 2 ? aq1[i] : (u < 4 ? aqm : aq2[i]), bb[u][2 * i], bb[u][2 * i + 1]);
-        }
-        mma_bf16(qq[0], aq1[i], bq[0][2 * i], bq[0][2 * i + 1]);
-        mma_bf16(qq[1], aq1[i], bq[1][2 * i], bq[1][2 * i + 1]);
+        // in two floats: differences of prefix sums are then exact where they matter
+        x0 *= 1.4426950408889634, x1 *= 1.4426950408889634;
+        const float h0 = float(x0), h1 = float(x1);
+        *reinterpret_cast<float2*>(&sm.g_hi[2 * lane]) = make_float2(h0, h1);
+        *reinterpret_cast<float2*>(&sm.g_lo[2 * lane]) = make_float2(float(x0 - h0), float(x1 - h1));
       }
     }
-    if ((lane >> 3) == (lane & 3)) {  // the thread with elements (g, g) and (g + 8, g + 8) of its diagonal tiles
-      const int e = (lane >> 2) & 1, row = warp * 16 + (lane >> 2);
-      sm.rk[row] = 1.0f / sqrtf((e ? kk[0][1] : kk[0][0]) + L2_EPS);
-      sm.rk[row + 8] = 1.0f / sqrtf((e ? kk[1][3] : kk[1][2]) + L2_EPS);
-      sm.rq[row] = 0.08838834764831845f / sqrtf((e ? qq[0][1] : qq[0][0]) + L2_EPS);
-      sm.rq[row + 8] = 0.08838834764831845f / sqrtf((e ? qq[1][3] : qq[1][2]) + L2_EPS);
-    }
-    bar_sync(CK_BAR_PROD, 128);  // prefix sums and norms are in shared memory
-    if (tid < CK_C) {
-      const float gh = sm.g_hi[tid], gl = sm.g_lo[tid], ch = sm.g_hi[CK_C - 1], cl = sm.g_lo[CK_C - 1];
-      const float e = ex2_approx(gh + gl), be = sm.gbeta[tid];
-      dv.beta[tid] = be;
-      dv.cx[tid] = be * e * sm.rk[tid];
-      dv.cq[tid] = e * sm.rq[tid];
-      dv.cs[tid] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[tid];
-      if (tid == 0) dv.total = ex2_approx(ch + cl);
+    if (e >= 2 && tid == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the image's last copy has left
+    __syncthreads();
+    if (gates) {
+      const float gh = sm.g_hi[gt], gl = sm.g_lo[gt], ch = sm.g_hi[CK_C - 1], cl = sm.g_lo[CK_C - 1];
+      const float ex = ex2_approx(gh + gl), be = sm.gbeta[gt];
+      img.beta[gt] = be;
+      img.cx[gt] = be * ex * sm.rk[gt];
+      img.cq[gt] = ex * sm.rq[gt];
+      img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
+      if (gt == 0) img.total = ex2_approx(ch + cl);
     }
 #pragma unroll
     for (int u = 0; u < 5; ++u) {
       const int rb = u < 2 ? warp : (u < 4 ? (warp == 1 ? warp : rb2) : rb2);
       const int row0 = rb * 16 + (lane >> 2), col = unit_tile[u] * 8 + 2 * (lane & 3);
+      const uint32_t block = ck_block(rb, unit_tile[u] >> 1);
       const float2 gh = *reinterpret_cast<const float2*>(&sm.g_hi[col]), gl = *reinterpret_cast<const float2*>(&sm.g_lo[col]),
                    rk = *reinterpret_cast<const float2*>(&sm.rk[col]);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int row = row0 + 8 * hf;
-        const float rh = sm.g_hi[row], rl = sm.g_lo[row], bk = sm.gbeta[row] * sm.rk[row], rq = sm.rq[row];
-        const float d0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x, d1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y;
-        float a0 = bk * d0 * kk[u][2 * hf], a1 = bk * d1 * kk[u][2 * hf + 1];
-        float p0 = rq * d0 * qk[u][2 * hf], p1 = rq * d1 * qk[u][2 * hf + 1];
-        uint32_t wh, wl;
-        const uint32_t at = swz<128>(row, unit_tile[u]) + 4 * (lane & 3);
+        const float rh = sm.g_hi[row], rl = sm.g_lo[row], f = of_q ? sm.rq[row] : -sm.gbeta[row] * sm.rk[row];
+        float x0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x * f * m[u][2 * hf];
+        float x1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y * f * m[u][2 * hf + 1];
         if (u < 2) {  // diagonal block: above the diagonal the exponentials may be anything
-          p0 = col <= row ? p0 : 0.f;
-          p1 = col + 1 <= row ? p1 : 0.f;
-          *reinterpret_cast<float2*>(&sm.a[row * CK_LDA + (col & 15)]) = make_float2(col < row ? a0 : 0.f, col + 1 < row ? a1 : 0.f);
-        } else {
-          split_f16x2(-a0, -a1, wh, wl);
-          *reinterpret_cast<uint32_t*>(dv.t_hi + at) = wh;
-          *reinterpret_cast<uint32_t*>(dv.t_lo + at) = wl;
+          const int last = of_q ? row : row - 1;
+          x0 = col <= last ? x0 : 0.f;
+          x1 = col < last ? x1 : 0.f;
         }
-        split_f16x2(p0, p1, wh, wl);
-        *reinterpret_cast<uint32_t*>(dv.p_hi + at) = wh;
-        *reinterpret_cast<uint32_t*>(dv.p_lo + at) = wl;
+        if (u < 2 && !of_q) {
+          *reinterpret_cast<float2*>(&sm.a[row * CD_LDA + (col & 15)]) = make_float2(x0, x1);
+        } else {
+          uint32_t wh, wl;
+          split_f16x2(x0, x1, wh, wl);
+          const uint32_t at = block + ck_in_block(row & 15, unit_tile[u] & 1) + 4 * (lane & 3);
+          *reinterpret_cast<uint32_t*>((of_q ? img.p_hi : img.t_hi) + at) = wh;
+          *reinterpret_cast<uint32_t*>((of_q ? img.p_lo : img.t_lo) + at) = wl;
+        }
       }
     }
-    __syncwarp();
-    {
-      // the warp's diagonal block of I + A inverted by substitution, lane = column (both halves of the warp alike)
-      const float* ad = sm.a + warp * 16 * CK_LDA;
+    if (!of_q) {
+      __syncwarp();
+      // the warp's diagonal block of I + A (sm.a holds -A) inverted by substitution, lane = column (both
+      // halves of the warp alike)
+      const float* ad = sm.a + warp * 16 * CD_LDA;
       const int cl = lane & 15;
       float x[16];
 #pragma unroll
@@ -350,9 +386,9 @@ __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
 #pragma unroll
         for (int j = 0; j < i; ++j) {
           if (j & 1)
-            s1 -= ad[i * CK_LDA + j] * x[j];
+            s1 += ad[i * CD_LDA + j] * x[j];
           else
-            s0 -= ad[i * CK_LDA + j] * x[j];
+            s0 += ad[i * CD_LDA + j] * x[j];
         }
         x[i] = s0 + s1;
       }
@@ -360,39 +396,42 @@ __device__ void ck_producer(const PrefillParams& p, CkSmem& sm, const SeqRange& 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float v = lane < 16 ? x[i] : x[8 + i];
-        const int row = warp * 16 + i + (lane < 16 ? 0 : 8);
-        const __half hi = __float2half_rn(v);
-        const uint32_t at = swz<128>(row, warp * 2 + (cl >> 3)) + 2 * (cl & 7);
-        *reinterpret_cast<__half*>(dv.t_hi + at) = hi;
-        *reinterpret_cast<__half*>(dv.t_lo + at) = __float2half_rn(v - __half2float(hi));
+        const __half vh = __float2half_rn(v);
+        const uint32_t at = ck_block(warp, warp) + ck_in_block(i + (lane < 16 ? 0 : 8), cl >> 3) + 2 * (cl & 7);
+        *reinterpret_cast<__half*>(img.t_hi + at) = vh;
+        *reinterpret_cast<__half*>(img.t_lo + at) = __float2half_rn(v - __half2float(vh));
       }
     }
-    bar_arrive(CK_BAR_FULL + (c & 1), CK_THREADS);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                       p.images + (int64_t(id) * p.HV + hv) * CK_IMAGE_BYTES),
+                   "r"(smem_addr(&img)), "r"(CK_IMAGE_BYTES)
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
   }
+  if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// acc [16, 64] += L M^T for L in two parts as left operands and M [64, 64] lower triangular in two parts
-// (rows of 128 bytes): hi hi + lo hi + hi lo (f16).
-__device__ __forceinline__ void ck_mul_tri(float (*acc)[4], const uint32_t (*lh)[4], const uint32_t (*ll)[4], uint32_t mh, uint32_t ml,
-                                           int lane) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t b[4][4], bl[4][4];
-#pragma unroll
-    for (int i = j; i < 4; ++i) {
-      const uint32_t off = swz<128>(i * 16 + ((lane >> 4) << 3) + (lane & 7), j * 2 + ((lane >> 3) & 1));
-      ldsm_x4(mh + off, b[i]);
-      ldsm_x4(ml + off, bl[i]);
-    }
-#pragma unroll
-    for (int part = 0; part < 3; ++part)
-#pragma unroll
-      for (int i = 2 * j; i < 8; ++i) {
-        const uint32_t* w = part == 2 ? bl[i >> 1] : b[i >> 1];
-        mma_f16(acc[i], part == 1 ? ll[j] : lh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
-      }
-  }
-}
+// ---------------------------------------------------------------- chunked form, second kernel
+template <int NW>
+struct CsStage {  // one chunk of a CTA of NW warps
+  alignas(1024) uint8_t k[CK_C * 256];
+  uint8_t q[CK_C * 256], v[CK_C * NW * 32];
+  CkImage img;
+};
+
+constexpr int CS_STAGES = 3;
+
+template <int NW>
+struct CsSmem {
+  CsStage<NW> stage[CS_STAGES];
+  uint8_t out[NW][16 * 48];
+  uint64_t full[CS_STAGES], empty[CS_STAGES];
+};
+static_assert(sizeof(CsSmem<8>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
 
 // Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
 __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
@@ -419,170 +458,9 @@ __device__ __forceinline__ void ck_row_scale(float top, float& up, float& down) 
   down = __uint_as_float(uint32_t(e - 4) << 23);
 }
 
-__device__ void ck_consumer(const PrefillParams& p, CkSmem& sm, const SeqRange& r, int hv, int v0, int chunks, bool fresh) {
-  const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t2 = 2 * (lane & 3);
-  // S as accumulators: tile n has rows g, g + 8 of the warp's 16 and key columns 8n + t2, + 1
-  float* st = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(v0 + warp * 16 + g) * 128 + t2;
-  float S[16][4];
-#pragma unroll
-  for (int n = 0; n < 16; ++n) {
-    float2 x = make_float2(0.f, 0.f), y = x;
-    if (!fresh) {
-      x = *reinterpret_cast<const float2*>(st + n * 8);
-      y = *reinterpret_cast<const float2*>(st + 8 * 128 + n * 8);
-    }
-    S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
-  }
-  const uint32_t stage = smem_addr(sm.stage[warp]);
-  for (int c = 0; c < chunks; ++c) {
-    const CkTile& tl = sm.tile[c % 3];
-    const CkDerived& dv = sm.der[c & 1];
-    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v);
-    const uint32_t th = smem_addr(dv.t_hi), tlo = smem_addr(dv.t_lo), ph = smem_addr(dv.p_hi),
-                   pl = smem_addr(dv.p_lo);
-    bar_sync(CK_BAR_FULL + (c & 1), CK_THREADS);
-    float X[8][4], O[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) X[j][e] = O[j][e] = 0.f;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      uint32_t hi[4], lo[4];
-      ck_left(S + 2 * s, hi, lo);
-      // products that add to the same tile are kept eight apart: one takes about four times as long as it keeps the unit
-#pragma unroll
-      for (int jj = 0; jj < 4; jj += 2) {
-        uint32_t bk[2][4], bq[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t off = swz<256>((jj + j) * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1));
-          ldsm_x4(ks + off, bk[j]);
-          ldsm_x4(qs + off, bq[j]);
-        }
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma_bf16(X[2 * jj + j], part ? lo : hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
-            mma_bf16(O[2 * jj + j], part ? lo : hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
-          }
-      }
-    }
-    // R = beta V^T - (beta e^G rk) X
-    float top0 = 0.f, top1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];  // tokens 16j + t2 (+1), rows g and g + 8; tokens 16j + 8 + t2
-      ldsm_x4_t(vs + swz<128>(j * 16 + ((lane >> 4) << 3) + (lane & 7), warp * 2 + ((lane >> 3) & 1)), w);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int tok = j * 16 + hf * 8 + t2;
-        const float2 be = *reinterpret_cast<const float2*>(&dv.beta[tok]), cx = *reinterpret_cast<const float2*>(&dv.cx[tok]),
-                     cq = *reinterpret_cast<const float2*>(&dv.cq[tok]);
-        const float2 v0f = bf16x2_to_f2(w[2 * hf]), v1f = bf16x2_to_f2(w[2 * hf + 1]);
-        float* x = X[2 * j + hf];
-        float* o = O[2 * j + hf];
-        x[0] = be.x * v0f.x - cx.x * x[0], x[1] = be.y * v0f.y - cx.y * x[1];
-        x[2] = be.x * v1f.x - cx.x * x[2], x[3] = be.y * v1f.y - cx.y * x[3];
-        top0 = fmaxf(top0, fmaxf(fabsf(x[0]), fabsf(x[1])));
-        top1 = fmaxf(top1, fmaxf(fabsf(x[2]), fabsf(x[3])));
-        o[0] *= cq.x, o[1] *= cq.y, o[2] *= cq.x, o[3] *= cq.y;
-      }
-    }
-    // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
-    float up0, down0, up1, down1;
-    ck_row_scale(top0, up0, down0);
-    ck_row_scale(top1, up1, down1);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      X[j][0] *= up0, X[j][1] *= up0, X[j][2] *= up1, X[j][3] *= up1;
-      O[j][0] *= up0, O[j][1] *= up0, O[j][2] *= up1, O[j][3] *= up1;
-    }
-    float N[8][4];
-    uint32_t nh[4][4], nl[4][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) N[j][e] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // column j of blocks: T_jj, then -A_ij below it
-      uint32_t b[4][4], bl[4][4], rh[4], rl[4];
-#pragma unroll
-      for (int i = j; i < 4; ++i) {
-        const uint32_t off = swz<128>(i * 16 + ((lane >> 4) << 3) + (lane & 7), j * 2 + ((lane >> 3) & 1));
-        ldsm_x4(th + off, b[i]);
-        ldsm_x4(tlo + off, bl[i]);
-      }
-      ck_left_f16(X + 2 * j, rh, rl);
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          mma_f16(N[2 * j + i], part == 1 ? rl : rh, (part == 2 ? bl : b)[j][2 * i], (part == 2 ? bl : b)[j][2 * i + 1]);
-      ck_left_f16(N + 2 * j, nh[j], nl[j]);
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int i = 2 * j + 2; i < 8; ++i) {
-          const uint32_t* w = (part == 2 ? bl : b)[i >> 1];
-          mma_f16(X[i], part == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
-        }
-    }
-    // the state first: the next chunk waits for it
-    const float total = dv.total;
-#pragma unroll
-    for (int n = 0; n < 16; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[n][e] *= total;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t hi[4], lo[4], rest[4];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const float2 cs = *reinterpret_cast<const float2*>(&dv.cs[j * 16 + hf * 8 + t2]);
-        const float* x = N[2 * j + hf];
-        split3_bf16x2(x[0] * (cs.x * down0), x[1] * (cs.y * down0), hi[2 * hf], lo[2 * hf], rest[2 * hf]);
-        split3_bf16x2(x[2] * (cs.x * down1), x[3] * (cs.y * down1), hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
-      }
-#pragma unroll
-      for (int nn = 0; nn < 8; nn += 4) {
-        uint32_t b[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) ldsm_x4_t(ks + swz<256>(j * 16 + (lane & 15), (nn + n) * 2 + (lane >> 4)), b[n]);
-#pragma unroll
-        for (int part = 0; part < 3; ++part)
-#pragma unroll
-          for (int n = 0; n < 8; ++n)
-            mma_bf16(S[2 * nn + n], part == 0 ? hi : (part == 1 ? lo : rest), b[n >> 1][2 * (n & 1)], b[n >> 1][2 * (n & 1) + 1]);
-      }
-    }
-    ck_mul_tri(O, nh, nl, ph, pl, lane);
-    if (c + 2 < chunks) bar_arrive(CK_BAR_EMPTY + (c & 1), CK_THREADS);
-    // O^T to token rows through the warp's own staging rows (48 bytes apart: no bank twice)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      stsm_x4_t(stage + (j * 16 + ((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, cvt_bf16x2(O[2 * j][0] * down0, O[2 * j][1] * down0),
-                cvt_bf16x2(O[2 * j][2] * down1, O[2 * j][3] * down1), cvt_bf16x2(O[2 * j + 1][0] * down0, O[2 * j + 1][1] * down0),
-                cvt_bf16x2(O[2 * j + 1][2] * down1, O[2 * j + 1][3] * down1));
-    __syncwarp();
-    const int t0 = r.begin + c * CK_C;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = i * 16 + (lane >> 1);
-      if (t0 + row < r.end)
-        *reinterpret_cast<uint4*>(p.out + int64_t(t0 + row) * p.o_st + int64_t(hv) * p.o_sh + v0 + warp * 16 + (lane & 1) * 8) =
-            *reinterpret_cast<const uint4*>(sm.stage[warp] + row * 48 + (lane & 1) * 16);
-    }
-    __syncwarp();
-  }
-#pragma unroll
-  for (int n = 0; n < 16; ++n) {
-    *reinterpret_cast<float2*>(st + n * 8) = make_float2(S[n][0], S[n][1]);
-    *reinterpret_cast<float2*>(st + 8 * 128 + n * 8) = make_float2(S[n][2], S[n][3]);
-  }
+// Right operand of block (i, j) of a triangular matrix: both 8-token halves, k of 16
+__device__ __forceinline__ void ck_right(uint32_t tri, int i, int j, int lane, uint32_t* b) {
+  ldsm_x4(tri + ck_block(i, j) + ck_in_block(((lane >> 4) << 3) + (lane & 7), (lane >> 3) & 1), b);
 }
 
 // The n-th sequence from the longest down, so that no long one starts last.  One
@@ -607,44 +485,292 @@ __device__ int ck_by_length(const PrefillParams& p, int want, int lane) {
   return found;
 }
 
-__global__ void __launch_bounds__(CK_THREADS, 1) prefill_chunk_kernel(const __grid_constant__ PrefillParams p) {
+template <int NW>
+__global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
+                                                                  const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
-  CkSmem& sm = *reinterpret_cast<CkSmem*>(raw + (-smem_addr(raw) & 1023u));
-  const int heads = p.HV * (128 / CK_ROWS);
-  const int n = ck_by_length(p, blockIdx.x / heads, threadIdx.x & 31);
-  const int part = blockIdx.x % heads, hv = part / (128 / CK_ROWS), v0 = (part % (128 / CK_ROWS)) * CK_ROWS;
+  CsSmem<NW>& sm = *reinterpret_cast<CsSmem<NW>*>(raw + (-smem_addr(raw) & 1023u));
+  constexpr int PARTS = 8 / NW, ROWS = NW * 16;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int heads = p.HV * PARTS;
+  const int n = ck_by_length(p, blockIdx.x / heads, lane);
+  const int part = blockIdx.x % heads, hv = part / PARTS, v0 = (part % PARTS) * ROWS;
   const SeqRange r = prefill_seq(p, n);
   if (r.slot < 0) {  // null slot: zero rows
-    for (int i = threadIdx.x; i < (r.end - r.begin) * CK_ROWS; i += CK_THREADS)
-      p.out[int64_t(r.begin + i / CK_ROWS) * p.o_st + int64_t(hv) * p.o_sh + v0 + i % CK_ROWS] = 0;
+    for (int i = tid; i < (r.end - r.begin) * ROWS; i += NW * 32)
+      p.out[int64_t(r.begin + i / ROWS) * p.o_st + int64_t(hv) * p.o_sh + v0 + i % ROWS] = 0;
     return;
   }
   const bool fresh = p.has_init && !p.has_init[n * p.hi_s];
   if (r.begin == r.end && !fresh) return;
-  const int chunks = (r.end - r.begin + CK_C - 1) / CK_C;
-  if (threadIdx.x < 128) {
-    if (chunks) ck_producer(p, sm, r, hv / (p.HV / p.H), hv, v0, chunks);
-  } else {
-    ck_consumer(p, sm, r, hv, v0, chunks, fresh);
+  const int chunks = (r.end - r.begin + CK_C - 1) / CK_C, h = hv / (p.HV / p.H);
+  const uint8_t* images = p.images + (int64_t(ck_first(r.begin, n)) * p.HV + hv) * CK_IMAGE_BYTES;
+
+  if (tid == 0) {
+    for (int i = 0; i < CS_STAGES; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], NW);
+    }
+    fence_mbar_init();
   }
+  __syncthreads();
+  auto load = [&](int c) {  // one thread
+    CsStage<NW>& st = sm.stage[c % CS_STAGES];
+    uint64_t* bar = &sm.full[c % CS_STAGES];
+    const int row = r.begin + c * CK_C;
+    mbar_arrive_expect_tx(bar, 2 * CK_C * 256 + CK_C * NW * 32 + CK_IMAGE_BYTES);
+    for (int b = 0; b < 2; ++b) {
+      ck_tma(smem_addr(st.k) + b * 8192, &map, (p.H + h) * 128 + b * 64, row, bar);
+      ck_tma(smem_addr(st.q) + b * 8192, &map, h * 128 + b * 64, row, bar);
+    }
+    for (int b = 0; b < NW / 4; ++b) ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + v0 + b * 64, row, bar);
+    bulk_g2s(&st.img, images + int64_t(c) * p.HV * CK_IMAGE_BYTES, CK_IMAGE_BYTES, bar);
+  };
+  int issued = 0;  // of thread 0
+  if (tid == 0)
+    for (; issued < CS_STAGES - 1 && issued < chunks; ++issued) load(issued);
+
+  const int g = lane >> 2, t2 = 2 * (lane & 3);
+  // S as accumulators: tile n has rows g, g + 8 of the warp's 16 and key columns 8n + t2, + 1
+  float* st = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(v0 + warp * 16 + g) * 128 + t2;
+  float S[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float2 x = make_float2(0.f, 0.f), y = x;
+    if (!fresh) {
+      x = *reinterpret_cast<const float2*>(st + i * 8);
+      y = *reinterpret_cast<const float2*>(st + 8 * 128 + i * 8);
+    }
+    S[i][0] = x.x, S[i][1] = x.y, S[i][2] = y.x, S[i][3] = y.y;
+  }
+  const uint32_t os = smem_addr(sm.out[warp]);
+  int c = 0;
+  bool ok = true;
+  for (; c < chunks; ++c) {
+    CsStage<NW>& tl = sm.stage[c % CS_STAGES];
+    const CkImage& im = tl.img;
+    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v) + (warp >> 2) * 8192;
+    ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
+    if (!ok) break;
+    const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
+    if (valid < CK_C) {  // the last chunk
+      ck_zero_rows(tl.k, 2, valid, tid, NW * 32);
+      ck_zero_rows(tl.v, NW / 4, valid, tid, NW * 32);
+      bar_sync(1, NW * 32);
+    }
+    float X[8][4], O[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) X[j][e] = O[j][e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      uint32_t hi[4], lo[4];
+      ck_left(S + 2 * s, hi, lo);
+      // products that add to the same tile are kept eight apart: one takes three times as long as it keeps the unit
+#pragma unroll
+      for (int jj = 0; jj < 4; jj += 2) {
+        uint32_t bk[2][4], bq[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t off = ck_at((jj + j) * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1));
+          ldsm_x4(ks + off, bk[j]);
+          ldsm_x4(qs + off, bq[j]);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_bf16(X[2 * jj + j], half ? lo : hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
+            mma_bf16(O[2 * jj + j], half ? lo : hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+          }
+      }
+    }
+    if (tid == 0 && issued < chunks) {
+      // the stage of the chunk before this one, which all warps have left by now or soon
+      if (c > 0) ok = mbar_wait_bounded(&sm.empty[issued % CS_STAGES], ((c - 1) / CS_STAGES) & 1, p.err);
+      if (!ok) break;
+      load(issued++);
+    }
+    // R = beta V^T - (beta e^G rk) X
+    float top0 = 0.f, top1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];  // tokens 16j + t2 (+1), rows g and g + 8; tokens 16j + 8 + t2
+      ldsm_x4_t(vs + swz<128>(j * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)), w);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int tok = j * 16 + hf * 8 + t2;
+        const float2 be = *reinterpret_cast<const float2*>(&im.beta[tok]), cx = *reinterpret_cast<const float2*>(&im.cx[tok]),
+                     cq = *reinterpret_cast<const float2*>(&im.cq[tok]);
+        const float2 v0f = bf16x2_to_f2(w[2 * hf]), v1f = bf16x2_to_f2(w[2 * hf + 1]);
+        float* x = X[2 * j + hf];
+        float* o = O[2 * j + hf];
+        x[0] = be.x * v0f.x - cx.x * x[0], x[1] = be.y * v0f.y - cx.y * x[1];
+        x[2] = be.x * v1f.x - cx.x * x[2], x[3] = be.y * v1f.y - cx.y * x[3];
+        top0 = fmaxf(top0, fmaxf(fabsf(x[0]), fabsf(x[1])));
+        top1 = fmaxf(top1, fmaxf(fabsf(x[2]), fabsf(x[3])));
+        o[0] *= cq.x, o[1] *= cq.y, o[2] *= cq.x, o[3] *= cq.y;
+      }
+    }
+    // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
+    float up0, down0, up1, down1;
+    ck_row_scale(top0, up0, down0);
+    ck_row_scale(top1, up1, down1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      X[j][0] *= up0, X[j][1] *= up0, X[j][2] *= up1, X[j][3] *= up1;
+      O[j][0] *= up0, O[j][1] *= up0, O[j][2] *= up1, O[j][3] *= up1;
+    }
+    const uint32_t th = smem_addr(im.t_hi), tlo = smem_addr(im.t_lo), ph = smem_addr(im.p_hi), pl = smem_addr(im.p_lo);
+    float N[8][4];
+    uint32_t nh[4][4], nl[4][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) N[j][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // column j of blocks: T_jj, then -A_ij below it
+      uint32_t b[4][4], bl[4][4], rh[4], rl[4];
+#pragma unroll
+      for (int i = j; i < 4; ++i) {
+        ck_right(th, i, j, lane, b[i]);
+        ck_right(tlo, i, j, lane, bl[i]);
+      }
+      ck_left_f16(X + 2 * j, rh, rl);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          mma_f16(N[2 * j + i], q == 1 ? rl : rh, (q == 2 ? bl : b)[j][2 * i], (q == 2 ? bl : b)[j][2 * i + 1]);
+      ck_left_f16(N + 2 * j, nh[j], nl[j]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int i = 2 * j + 2; i < 8; ++i) {
+          const uint32_t* w = (q == 2 ? bl : b)[i >> 1];
+          mma_f16(X[i], q == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
+        }
+    }
+    const float total = im.total;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[i][e] *= total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t hi[4], lo[4], rest[4];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float2 cs = *reinterpret_cast<const float2*>(&im.cs[j * 16 + hf * 8 + t2]);
+        const float* x = N[2 * j + hf];
+        split3_bf16x2(x[0] * (cs.x * down0), x[1] * (cs.y * down0), hi[2 * hf], lo[2 * hf], rest[2 * hf]);
+        split3_bf16x2(x[2] * (cs.x * down1), x[3] * (cs.y * down1), hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
+      }
+#pragma unroll
+      for (int ii = 0; ii < 8; ii += 4) {
+        uint32_t b[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ldsm_x4_t(ks + ck_at(j * 16 + (lane & 15), (ii + i) * 2 + (lane >> 4)), b[i]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            mma_bf16(S[2 * ii + i], q == 0 ? hi : (q == 1 ? lo : rest), b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
+      }
+    }
+    // O += N P^T
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t b[4][4], bl[4][4];
+#pragma unroll
+      for (int i = j; i < 4; ++i) {
+        ck_right(ph, i, j, lane, b[i]);
+        ck_right(pl, i, j, lane, bl[i]);
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int i = 2 * j; i < 8; ++i) {
+          const uint32_t* w = (q == 2 ? bl : b)[i >> 1];
+          mma_f16(O[i], q == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
+        }
+    }
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.empty[c % CS_STAGES])) : "memory");
+    // O^T to token rows, 16 tokens at a time through the warp's own rows (48 bytes apart: no bank twice)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      __syncwarp();
+      stsm_x4_t(os + (((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, cvt_bf16x2(O[2 * j][0] * down0, O[2 * j][1] * down0),
+                cvt_bf16x2(O[2 * j][2] * down1, O[2 * j][3] * down1), cvt_bf16x2(O[2 * j + 1][0] * down0, O[2 * j + 1][1] * down0),
+                cvt_bf16x2(O[2 * j + 1][2] * down1, O[2 * j + 1][3] * down1));
+      __syncwarp();
+      const int row = j * 16 + (lane >> 1);
+      if (row < valid)
+        *reinterpret_cast<uint4*>(p.out + int64_t(t0 + row) * p.o_st + int64_t(hv) * p.o_sh + v0 + warp * 16 + (lane & 1) * 8) =
+            *reinterpret_cast<const uint4*>(sm.out[warp] + (lane >> 1) * 48 + (lane & 1) * 16);
+    }
+  }
+  if (!ok) {  // a wait gave up (the error word says so): the state stays, copies in flight are waited for
+    for (; c < issued; ++c) mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    *reinterpret_cast<float2*>(st + i * 8) = make_float2(S[i][0], S[i][1]);
+    *reinterpret_cast<float2*>(st + 8 * 128 + i * 8) = make_float2(S[i][2], S[i][3]);
+  }
+}
+
+template <int NW>
+cudaError_t scan(const PrefillParams& p, const CUtensorMap& map, cudaStream_t stream) {
+  static DynSmemCache cache;
+  constexpr int bytes = sizeof(CsSmem<NW>) + 1024;
+  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(prefill_scan_kernel<NW>), bytes, cache);
+  if (e != cudaSuccess) return e;
+  prefill_scan_kernel<NW><<<dim3(unsigned(int64_t(p.N) * p.HV * (8 / NW))), NW * 32, bytes, stream>>>(p, map);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream) {
-  static DynSmemCache cache;
-  constexpr int bytes = sizeof(CkSmem) + 1024;
-  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(prefill_chunk_kernel), bytes, cache);
+  CUtensorMap map;
+  // boxes of 64 columns x 64 tokens of mixed_qkv
+  const uint64_t dims[2] = {uint64_t(2 * p.H + p.HV) * 128, uint64_t(p.T)};
+  const uint64_t strides[1] = {uint64_t(p.mx_s) * 2};
+  const uint32_t box[2] = {64, CK_C};
+  cudaError_t e = encode_bf16_map(&map, p.mixed, 2, dims, strides, box);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = int64_t(p.N) * p.HV * (128 / CK_ROWS);
-  prefill_chunk_kernel<<<dim3(unsigned(blocks)), CK_THREADS, bytes, stream>>>(p);
-  return cudaGetLastError();
+  static DynSmemCache cache;
+  constexpr int bytes = sizeof(CdSmem) + 1024;
+  e = ensure_dyn_smem(reinterpret_cast<const void*>(prefill_derive_kernel), bytes, cache);
+  if (e != cudaSuccess) return e;
+  const int64_t ids = int64_t(p.T) / CK_C + p.N;
+  prefill_derive_kernel<<<dim3(unsigned(ids * p.H)), CD_THREADS, bytes, stream>>>(p, map);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // 64 value rows a CTA where that gives the machine no more CTAs than it has multiprocessors (one long prompt:
+  // the chain of chunks is what takes the time), else whole heads (two warps on each tensor unit hide one another)
+  return int64_t(p.N) * p.HV * 2 <= multiprocessor_count() ? scan<4>(p, map, stream) : scan<8>(p, map, stream);
+}
+
+// The longest sequence as the host knows it, or the mean length
+static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) {
+  const int64_t longest = max_seqlen > 0 ? max_seqlen : (tokens + sequences - 1) / sequences;
+  return longest > 8;
+}
+
+int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen) {
+  if (sequences <= 0 || tokens <= 0 || !prefill_chunked(tokens, sequences, max_seqlen)) return 0;
+  return (tokens / CK_C + sequences) * value_heads * CK_IMAGE_BYTES;
 }
 
 cudaError_t launch_prefill(const PrefillParams& p, int max_seqlen, cudaStream_t stream) {
-  // The longest sequence as the host knows it, or the mean length
-  const int longest = max_seqlen > 0 ? max_seqlen : p.T / p.N + (p.T % p.N != 0);
-  return longest <= 8 ? launch_prefill_recurrent(p, stream) : launch_prefill_chunk(p, stream);
+  if (p.T == 0 || !prefill_chunked(p.T, p.N, max_seqlen)) return launch_prefill_recurrent(p, stream);
+  return launch_prefill_chunk(p, stream);
 }
 
 cudaError_t launch_prefill_recurrent(const PrefillParams& p, cudaStream_t stream) {

@@ -132,6 +132,8 @@ class PrefillArgs(ctypes.Structure):
                                       "state_indices", "has_initial", "out")] + [
         ("max_seqlen", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
         ("error_flag", ctypes.c_void_p),
     ]
 
@@ -170,6 +172,7 @@ SIGNATURES = {
     "gdnr_dequantize_vblock32": ([ctypes.POINTER(CodecArgs), ctypes.c_void_p], ctypes.c_int),
     "gdnr_bf16_step": ([ctypes.POINTER(Bf16StepArgs), ctypes.c_void_p], ctypes.c_int),
     "gdnr_gdn_prefill": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "gdnr_gdn_prefill_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32], ctypes.c_int64),
     "gdnr_qk_norm_rope_append": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
     "gdnr_paged_attention": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
     "gdnr_paged_attention_workspace": ([ctypes.c_int32], ctypes.c_int64),

@@ -26,7 +26,7 @@ import torch
 from . import _lib
 from .ops import _err_ptr
 
-_PREFILL_TAIL = struct.Struct("@iiP")
+_PREFILL_TAIL = struct.Struct("@iiPqP")
 _APPEND_TAIL = struct.Struct("@ffiiP")
 _ATTN_TAIL = struct.Struct("@fiPqP")
 
@@ -68,7 +68,9 @@ def gdn_prefill(
     dev = mixed_qkv.get_device()
     packed = _lib.pack_tensors(dev, (mixed_qkv, a, b, A_log, dt_bias, state, cu_seqlens, state_indices,
                                      has_initial_state, out))
-    packed.append(_PREFILL_TAIL.pack(max_seqlen, 0, _err(error_flag)))
+    nbytes = _lib.load().gdnr_gdn_prefill_workspace(mixed_qkv.shape[0], cu_seqlens.shape[0] - 1, state.shape[1], max_seqlen)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=mixed_qkv.device) if nbytes > 0 else None
+    packed.append(_PREFILL_TAIL.pack(max_seqlen, 0, workspace.data_ptr() if nbytes > 0 else 0, nbytes, _err(error_flag)))
     _lib.call_packed("gdnr_gdn_prefill", b"".join(packed), dev)
     return out
 

@@ -271,10 +271,16 @@ typedef struct {
   gdnr_tensor out;           /* [T,HV,V] BF16 */
   int32_t max_seqlen;
   int32_t reserved;
+  void* workspace;           /* gdnr_gdn_prefill_workspace() bytes (may be 0), 16-byte aligned,
+                                private to the call until it has run; need not be zero */
+  int64_t workspace_bytes;
   uint32_t* error_flag;
 } gdnr_prefill_args;
 
 int gdnr_gdn_prefill(const gdnr_prefill_args* args, void* stream);
+/* Workspace bytes of gdnr_gdn_prefill for T tokens of N sequences (about 11 KB a token
+ * at 32 value heads; none for a few tokens a sequence). */
+int64_t gdnr_gdn_prefill_workspace(int64_t tokens, int64_t sequences, int32_t value_heads, int32_t max_seqlen);
 
 /* ---- gdnr_qk_norm_rope_append --------------------------------------------
  * Per token and head: x / sqrt(mean(x^2) + eps) * (weight + weight_offset) for queries
