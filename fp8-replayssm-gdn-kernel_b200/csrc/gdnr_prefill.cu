@@ -200,15 +200,14 @@ struct CdSmem {
   uint8_t k[CK_C * 256], q[CK_C * 256];
   CkImage img[2];
   float a[CK_C * CD_LDA];  // -A's diagonal blocks: warp w's at rows 16 w
-  double g[CK_C];
-  float g_hi[CK_C], g_lo[CK_C];  // prefix sums of the gates in units of ln 2, in two parts
-  float rk[CK_C], rq[CK_C], gbeta[CK_C];
+  float g_hi[2][CK_C], g_lo[2][CK_C], gbeta[2][CK_C];  // prefix sums of the gates in units of ln 2, in two parts
+  float rk[CK_C], rq[CK_C];
   uint64_t bar;
 };
 
 // One CTA a chunk and key head; its value heads share the products of the raw rows.  The first
 // four warps make A (rows of K against K) and invert its diagonal blocks, the others make P
-// (rows of Q against K), the gates and the factors.
+// (rows of Q against K) and the factors.
 __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __grid_constant__ PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
@@ -240,17 +239,40 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
     }
   }
   const bool of_q = tid >= 128;
-  const int gt = tid - 128;  // token whose gates this thread makes, where in [0, C)
-  const bool gates = gt >= 0 && gt < CK_C;
-  auto gate_in = [&](int hv, float& a, float& b) {
-    a = b = 0.f;
-    if (gates && gt < valid) {
-      a = load_scalar(p.a, int64_t(t0 + gt) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt) + p.dt_bias[hv * p.db_s];
-      b = load_scalar(p.b, int64_t(t0 + gt) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt);
+  // gates of up to two value heads, one warp each, lane: two tokens; tokens past the end neither decay nor write
+  auto make_gates = [&](int e0) {
+    const int e = tid >> 5;
+    if (e >= 2 || e0 + e >= group) return;
+    const int hv = h * group + e0 + e;
+    const float neg_a = -expf(p.a_log[hv * p.al_s]), dtb = p.dt_bias[hv * p.db_s];
+    double x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 2 * lane + i;
+      float g = 0.f, be = 0.f;
+      if (t < valid) {
+        g = neg_a * softplus_gate(load_scalar(p.a, int64_t(t0 + t) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt) + dtb);
+        be = sigmoid_f(load_scalar(p.b, int64_t(t0 + t) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt));
+      }
+      x[i] = double(g);
+      sm.gbeta[e][t] = be;
+    }
+    x[1] += x[0];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, x[1], o);
+      if (lane >= o) x[0] += y, x[1] += y;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // in two floats: differences of prefix sums are then exact where they matter
+      const double y = x[i] * 1.4426950408889634;
+      const float hi = float(y);
+      sm.g_hi[e][2 * lane + i] = hi;
+      sm.g_lo[e][2 * lane + i] = float(y - hi);
     }
   };
-  float na, nb;
-  gate_in(h * group, na, nb);
+  make_gates(0);  // while the rows are on their way
   __syncthreads();  // the barrier is initialised
   const bool ok = mbar_wait_bounded(&sm.bar, 0, p.err);
   if (__syncthreads_or(!ok)) return;
@@ -310,105 +332,93 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
     (of_q ? sm.rq : sm.rk)[row] = gain * rsqrtf(x0 + L2_EPS);
     (of_q ? sm.rq : sm.rk)[row + 8] = gain * rsqrtf(x1 + L2_EPS);
   }
-  for (int e = 0; e < group; ++e) {
-    const int hv = h * group + e;
-    CkImage& img = sm.img[e & 1];
-    const float a = na, b = nb;
-    if (e + 1 < group) gate_in(hv + 1, na, nb);
-    if (gates) {  // tokens past the end neither decay nor write
-      sm.g[gt] = gt < valid ? double(-expf(p.a_log[hv * p.al_s]) * softplus_gate(a)) : 0.0;
-      sm.gbeta[gt] = gt < valid ? sigmoid_f(b) : 0.f;
-      bar_sync(1, CK_C);
-      if (warp == 0) {
-        double x0 = sm.g[2 * lane], x1 = x0 + sm.g[2 * lane + 1];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, x1, o);
-          if (lane >= o) x0 += y, x1 += y;
-        }
-        // in two floats: differences of prefix sums are then exact where they matter
-        x0 *= 1.4426950408889634, x1 *= 1.4426950408889634;
-        const float h0 = float(x0), h1 = float(x1);
-        *reinterpret_cast<float2*>(&sm.g_hi[2 * lane]) = make_float2(h0, h1);
-        *reinterpret_cast<float2*>(&sm.g_lo[2 * lane]) = make_float2(float(x0 - h0), float(x1 - h1));
-      }
+  for (int e0 = 0; e0 < group; e0 += 2) {
+    if (e0) {  // the two images have left
+      if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      make_gates(e0);
     }
-    if (e >= 2 && tid == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the image's last copy has left
-    __syncthreads();
-    if (gates) {
-      const float gh = sm.g_hi[gt], gl = sm.g_lo[gt], ch = sm.g_hi[CK_C - 1], cl = sm.g_lo[CK_C - 1];
-      const float ex = ex2_approx(gh + gl), be = sm.gbeta[gt];
-      img.beta[gt] = be;
-      img.cx[gt] = be * ex * sm.rk[gt];
-      img.cq[gt] = ex * sm.rq[gt];
-      img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
-      if (gt == 0) img.total = ex2_approx(ch + cl);
-    }
+    __syncthreads();  // gates, norms
+    for (int e = 0; e < 2 && e0 + e < group; ++e) {
+      CkImage& img = sm.img[e];
+      const float *g_hi = sm.g_hi[e], *g_lo = sm.g_lo[e], *gbeta = sm.gbeta[e];
+      if (of_q && tid < 128 + CK_C) {
+        const int gt = tid - 128;
+        const float gh = g_hi[gt], gl = g_lo[gt], ch = g_hi[CK_C - 1], cl = g_lo[CK_C - 1];
+        const float ex = ex2_approx(gh + gl), be = gbeta[gt];
+        img.beta[gt] = be;
+        img.cx[gt] = be * ex * sm.rk[gt];
+        img.cq[gt] = ex * sm.rq[gt];
+        img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
+        if (gt == 0) img.total = ex2_approx(ch + cl);
+      }
 #pragma unroll
-    for (int u = 0; u < 5; ++u) {
-      const int rb = u < 2 ? warp : (u < 4 ? (warp == 1 ? warp : rb2) : rb2);
-      const int row0 = rb * 16 + (lane >> 2), col = unit_tile[u] * 8 + 2 * (lane & 3);
-      const uint32_t block = ck_block(rb, unit_tile[u] >> 1);
-      const float2 gh = *reinterpret_cast<const float2*>(&sm.g_hi[col]), gl = *reinterpret_cast<const float2*>(&sm.g_lo[col]),
-                   rk = *reinterpret_cast<const float2*>(&sm.rk[col]);
+      for (int u = 0; u < 5; ++u) {
+        const int rb = u < 2 ? warp : (u < 4 ? (warp == 1 ? warp : rb2) : rb2);
+        const int row0 = rb * 16 + (lane >> 2), col = unit_tile[u] * 8 + 2 * (lane & 3);
+        const uint32_t block = ck_block(rb, unit_tile[u] >> 1);
+        const float2 gh = *reinterpret_cast<const float2*>(&g_hi[col]), gl = *reinterpret_cast<const float2*>(&g_lo[col]),
+                     rk = *reinterpret_cast<const float2*>(&sm.rk[col]);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int row = row0 + 8 * hf;
-        const float rh = sm.g_hi[row], rl = sm.g_lo[row], f = of_q ? sm.rq[row] : -sm.gbeta[row] * sm.rk[row];
-        float x0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x * f * m[u][2 * hf];
-        float x1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y * f * m[u][2 * hf + 1];
-        if (u < 2) {  // diagonal block: above the diagonal the exponentials may be anything
-          const int last = of_q ? row : row - 1;
-          x0 = col <= last ? x0 : 0.f;
-          x1 = col < last ? x1 : 0.f;
-        }
-        if (u < 2 && !of_q) {
-          *reinterpret_cast<float2*>(&sm.a[row * CD_LDA + (col & 15)]) = make_float2(x0, x1);
-        } else {
-          uint32_t wh, wl;
-          split_f16x2(x0, x1, wh, wl);
-          const uint32_t at = block + ck_in_block(row & 15, unit_tile[u] & 1) + 4 * (lane & 3);
-          *reinterpret_cast<uint32_t*>((of_q ? img.p_hi : img.t_hi) + at) = wh;
-          *reinterpret_cast<uint32_t*>((of_q ? img.p_lo : img.t_lo) + at) = wl;
+        for (int hf = 0; hf < 2; ++hf) {
+          const int row = row0 + 8 * hf;
+          const float rh = g_hi[row], rl = g_lo[row], f = of_q ? sm.rq[row] : -gbeta[row] * sm.rk[row];
+          float x0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x * f * m[u][2 * hf];
+          float x1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y * f * m[u][2 * hf + 1];
+          if (u < 2) {  // diagonal block: above the diagonal the exponentials may be anything
+            const int last = of_q ? row : row - 1;
+            x0 = col <= last ? x0 : 0.f;
+            x1 = col < last ? x1 : 0.f;
+          }
+          if (u < 2 && !of_q) {
+            *reinterpret_cast<float2*>(&sm.a[row * CD_LDA + (col & 15)]) = make_float2(x0, x1);
+          } else {
+            uint32_t wh, wl;
+            split_f16x2(x0, x1, wh, wl);
+            const uint32_t at = block + ck_in_block(row & 15, unit_tile[u] & 1) + 4 * (lane & 3);
+            *reinterpret_cast<uint32_t*>((of_q ? img.p_hi : img.t_hi) + at) = wh;
+            *reinterpret_cast<uint32_t*>((of_q ? img.p_lo : img.t_lo) + at) = wl;
+          }
         }
       }
-    }
-    if (!of_q) {
-      __syncwarp();
-      // the warp's diagonal block of I + A (sm.a holds -A) inverted by substitution, lane = column (both
-      // halves of the warp alike)
-      const float* ad = sm.a + warp * 16 * CD_LDA;
-      const int cl = lane & 15;
-      float x[16];
+      if (!of_q) {
+        __syncwarp();
+        // the warp's diagonal block of I + A (sm.a holds -A) inverted by substitution, lane = column (both
+        // halves of the warp alike)
+        const float* ad = sm.a + warp * 16 * CD_LDA;
+        const int cl = lane & 15;
+        float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float s0 = i == cl ? 1.f : 0.f, s1 = 0.f;
+        for (int i = 0; i < 16; ++i) {
+          float s0 = i == cl ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) {
-          if (j & 1)
-            s1 += ad[i * CD_LDA + j] * x[j];
-          else
-            s0 += ad[i * CD_LDA + j] * x[j];
+          for (int j = 0; j < i; ++j) {
+            if (j & 1)
+              s1 += ad[i * CD_LDA + j] * x[j];
+            else
+              s0 += ad[i * CD_LDA + j] * x[j];
+          }
+          x[i] = s0 + s1;
         }
-        x[i] = s0 + s1;
-      }
-      // rows of the first half by lanes 0..15, of the second by the others
+        // rows of the first half by lanes 0..15, of the second by the others
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float v = lane < 16 ? x[i] : x[8 + i];
-        const __half vh = __float2half_rn(v);
-        const uint32_t at = ck_block(warp, warp) + ck_in_block(i + (lane < 16 ? 0 : 8), cl >> 3) + 2 * (cl & 7);
-        *reinterpret_cast<__half*>(img.t_hi + at) = vh;
-        *reinterpret_cast<__half*>(img.t_lo + at) = __float2half_rn(v - __half2float(vh));
+        for (int i = 0; i < 8; ++i) {
+          const float v = lane < 16 ? x[i] : x[8 + i];
+          const __half vh = __float2half_rn(v);
+          const uint32_t at = ck_block(warp, warp) + ck_in_block(i + (lane < 16 ? 0 : 8), cl >> 3) + 2 * (cl & 7);
+          *reinterpret_cast<__half*>(img.t_hi + at) = vh;
+          *reinterpret_cast<__half*>(img.t_lo + at) = __float2half_rn(v - __half2float(vh));
+        }
       }
+      __syncwarp();  // sm.a is the warp's own
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                       p.images + (int64_t(id) * p.HV + hv) * CK_IMAGE_BYTES),
-                   "r"(smem_addr(&img)), "r"(CK_IMAGE_BYTES)
-                   : "memory");
+      for (int e = 0; e < 2 && e0 + e < group; ++e)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                         p.images + (int64_t(id) * p.HV + h * group + e0 + e) * CK_IMAGE_BYTES),
+                     "r"(smem_addr(&sm.img[e])), "r"(CK_IMAGE_BYTES)
+                     : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
   }
@@ -416,22 +426,32 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
 }
 
 // ---------------------------------------------------------------- chunked form, second kernel
-template <int NW>
-struct CsStage {  // one chunk of a CTA of NW warps
+// NW warps; the key columns of 16 value rows are shared by KS of them (1 or 2).  With two, each
+// warp has half of S: X and S Q^T are added up through shared memory, both solve for N, and each
+// updates its half of S and makes the output of half the tokens.
+template <int NW, int KS>
+struct CsCfg {
+  static constexpr int GROUPS = NW / KS, ROWS = GROUPS * 16, PARTS = 128 / ROWS;
+  static constexpr int V_BOXES = ROWS > 64 ? 2 : 1;
+};
+
+template <int NW, int KS>
+struct CsStage {  // one chunk
   alignas(1024) uint8_t k[CK_C * 256];
-  uint8_t q[CK_C * 256], v[CK_C * NW * 32];
+  uint8_t q[CK_C * 256], v[CsCfg<NW, KS>::V_BOXES * CK_C * 128];
   CkImage img;
 };
 
 constexpr int CS_STAGES = 3;
 
-template <int NW>
+template <int NW, int KS>
 struct CsSmem {
-  CsStage<NW> stage[CS_STAGES];
+  CsStage<NW, KS> stage[CS_STAGES];
   uint8_t out[NW][16 * 48];
+  float4 swap[KS > 1 ? NW : 1][KS > 1 ? 12 : 1][32];  // a warp's X, and S Q^T of the other's tokens
   uint64_t full[CS_STAGES], empty[CS_STAGES];
 };
-static_assert(sizeof(CsSmem<8>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
+static_assert(sizeof(CsSmem<8, 1>) + 1024 <= MAX_DYN_SMEM && sizeof(CsSmem<4, 2>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
 
 // Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
 __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
@@ -485,12 +505,33 @@ __device__ int ck_by_length(const PrefillParams& p, int want, int lane) {
   return found;
 }
 
-template <int NW>
+// Column j of blocks of O += N P^T: rows of blocks 0 and 3 where `outer`, of 1 and 2 where `inner`
+__device__ __forceinline__ void ck_out_column(float (*O)[4], const uint32_t* nh, const uint32_t* nl, uint32_t ph, uint32_t pl, int j, int lane,
+                                              bool outer, bool inner) {
+  uint32_t b[4][4], bl[4][4];
+#pragma unroll
+  for (int i = j; i < 4; ++i)
+    if (i == 0 || i == 3 ? outer : inner) {
+      ck_right(ph, i, j, lane, b[i]);
+      ck_right(pl, i, j, lane, bl[i]);
+    }
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int i = 2 * j; i < 8; ++i)
+      if (i < 2 || i > 5 ? outer : inner) {
+        const uint32_t* w = (q == 2 ? bl : b)[i >> 1];
+        mma_f16(O[i], q == 1 ? nl : nh, w[2 * (i & 1)], w[2 * (i & 1) + 1]);
+      }
+}
+
+template <int NW, int KS>
 __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
                                                                   const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
-  CsSmem<NW>& sm = *reinterpret_cast<CsSmem<NW>*>(raw + (-smem_addr(raw) & 1023u));
-  constexpr int PARTS = 8 / NW, ROWS = NW * 16;
+  using C = CsCfg<NW, KS>;
+  CsSmem<NW, KS>& sm = *reinterpret_cast<CsSmem<NW, KS>*>(raw + (-smem_addr(raw) & 1023u));
+  constexpr int PARTS = C::PARTS, ROWS = C::ROWS, KT = 16 / KS;  // KT: tiles of S of a warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int heads = p.HV * PARTS;
   const int n = ck_by_length(p, blockIdx.x / heads, lane);
@@ -515,15 +556,16 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
   }
   __syncthreads();
   auto load = [&](int c) {  // one thread
-    CsStage<NW>& st = sm.stage[c % CS_STAGES];
+    CsStage<NW, KS>& st = sm.stage[c % CS_STAGES];
     uint64_t* bar = &sm.full[c % CS_STAGES];
     const int row = r.begin + c * CK_C;
-    mbar_arrive_expect_tx(bar, 2 * CK_C * 256 + CK_C * NW * 32 + CK_IMAGE_BYTES);
+    mbar_arrive_expect_tx(bar, 2 * CK_C * 256 + C::V_BOXES * CK_C * 128 + CK_IMAGE_BYTES);
     for (int b = 0; b < 2; ++b) {
       ck_tma(smem_addr(st.k) + b * 8192, &map, (p.H + h) * 128 + b * 64, row, bar);
       ck_tma(smem_addr(st.q) + b * 8192, &map, h * 128 + b * 64, row, bar);
     }
-    for (int b = 0; b < NW / 4; ++b) ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + v0 + b * 64, row, bar);
+    for (int b = 0; b < C::V_BOXES; ++b)
+      ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + (v0 & 64) + b * 64, row, bar);
     bulk_g2s(&st.img, images + int64_t(c) * p.HV * CK_IMAGE_BYTES, CK_IMAGE_BYTES, bar);
   };
   int issued = 0;  // of thread 0
@@ -531,11 +573,12 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
     for (; issued < CS_STAGES - 1 && issued < chunks; ++issued) load(issued);
 
   const int g = lane >> 2, t2 = 2 * (lane & 3);
+  const int vr = v0 + (warp % C::GROUPS) * 16, kh = KS > 1 ? warp / C::GROUPS : 0;  // the warp's value rows, its half of the keys
   // S as accumulators: tile n has rows g, g + 8 of the warp's 16 and key columns 8n + t2, + 1
-  float* st = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(v0 + warp * 16 + g) * 128 + t2;
-  float S[16][4];
+  float* st = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(vr + g) * 128 + kh * KT * 8 + t2;
+  float S[KT][4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < KT; ++i) {
     float2 x = make_float2(0.f, 0.f), y = x;
     if (!fresh) {
       x = *reinterpret_cast<const float2*>(st + i * 8);
@@ -547,15 +590,15 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
   int c = 0;
   bool ok = true;
   for (; c < chunks; ++c) {
-    CsStage<NW>& tl = sm.stage[c % CS_STAGES];
+    CsStage<NW, KS>& tl = sm.stage[c % CS_STAGES];
     const CkImage& im = tl.img;
-    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v) + (warp >> 2) * 8192;
+    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v) + (C::V_BOXES > 1 ? (vr >> 6) * 8192 : 0);
     ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
     if (!ok) break;
     const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
     if (valid < CK_C) {  // the last chunk
       ck_zero_rows(tl.k, 2, valid, tid, NW * 32);
-      ck_zero_rows(tl.v, NW / 4, valid, tid, NW * 32);
+      ck_zero_rows(tl.v, C::V_BOXES, valid, tid, NW * 32);
       bar_sync(1, NW * 32);
     }
     float X[8][4], O[8][4];
@@ -564,7 +607,7 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
 #pragma unroll
       for (int e = 0; e < 4; ++e) X[j][e] = O[j][e] = 0.f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < KT / 2; ++s) {
       uint32_t hi[4], lo[4];
       ck_left(S + 2 * s, hi, lo);
       // products that add to the same tile are kept eight apart: one takes three times as long as it keeps the unit
@@ -573,7 +616,7 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
         uint32_t bk[2][4], bq[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t off = ck_at((jj + j) * 16 + ((lane >> 4) << 3) + (lane & 7), s * 2 + ((lane >> 3) & 1));
+          const uint32_t off = ck_at((jj + j) * 16 + ((lane >> 4) << 3) + (lane & 7), kh * KT + s * 2 + ((lane >> 3) & 1));
           ldsm_x4(ks + off, bk[j]);
           ldsm_x4(qs + off, bq[j]);
         }
@@ -592,12 +635,40 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
       if (!ok) break;
       load(issued++);
     }
+    if constexpr (KS > 1) {
+      // the other half's X of all tokens and S Q^T of the tokens this warp writes out: blocks 0 and 3, or 1 and 2
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sm.swap[warp][j][lane] = make_float4(X[j][0], X[j][1], X[j][2], X[j][3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int mine = j < 2 ? j : j + 4, other = j + 2;  // tiles of blocks 0 and 3, 1 and 2
+        sm.swap[warp][8 + j][lane] = kh ? make_float4(O[mine][0], O[mine][1], O[mine][2], O[mine][3])
+                                        : make_float4(O[other][0], O[other][1], O[other][2], O[other][3]);
+      }
+      const int peer = warp ^ C::GROUPS;
+      bar_sync(2 + warp % C::GROUPS, 64);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 y = sm.swap[peer][j][lane];
+        X[j][0] += y.x, X[j][1] += y.y, X[j][2] += y.z, X[j][3] += y.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 y = sm.swap[peer][8 + j][lane];
+        float* a = O[j < 2 ? j : j + 4];
+        float* b = O[j + 2];
+        // kh 0 keeps blocks 0 and 3, kh 1 blocks 1 and 2; the other two are not used again
+        a[0] += y.x, a[1] += y.y, a[2] += y.z, a[3] += y.w;
+        b[0] += y.x, b[1] += y.y, b[2] += y.z, b[3] += y.w;
+      }
+      bar_sync(2 + warp % C::GROUPS, 64);  // read before the next chunk's overwrite it
+    }
     // R = beta V^T - (beta e^G rk) X
     float top0 = 0.f, top1 = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t w[4];  // tokens 16j + t2 (+1), rows g and g + 8; tokens 16j + 8 + t2
-      ldsm_x4_t(vs + swz<128>(j * 16 + ((lane >> 4) << 3) + (lane & 7), (warp & 3) * 2 + ((lane >> 3) & 1)), w);
+      ldsm_x4_t(vs + swz<128>(j * 16 + ((lane >> 4) << 3) + (lane & 7), ((vr & 63) >> 3) + ((lane >> 3) & 1)), w);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int tok = j * 16 + hf * 8 + t2;
@@ -655,7 +726,7 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
     }
     const float total = im.total;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[i][e] *= total;
 #pragma unroll
@@ -669,10 +740,10 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
         split3_bf16x2(x[2] * (cs.x * down1), x[3] * (cs.y * down1), hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
       }
 #pragma unroll
-      for (int ii = 0; ii < 8; ii += 4) {
+      for (int ii = 0; ii < KT / 2; ii += 4) {
         uint32_t b[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ldsm_x4_t(ks + ck_at(j * 16 + (lane & 15), (ii + i) * 2 + (lane >> 4)), b[i]);
+        for (int i = 0; i < 4; ++i) ldsm_x4_t(ks + ck_at(j * 16 + (lane & 15), kh * KT + (ii + i) * 2 + (lane >> 4)), b[i]);
 #pragma unroll
         for (int q = 0; q < 3; ++q)
 #pragma unroll
@@ -681,27 +752,19 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
       }
     }
     // O += N P^T
+    if constexpr (KS == 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t b[4][4], bl[4][4];
+      for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, true, true);
+    } else {
 #pragma unroll
-      for (int i = j; i < 4; ++i) {
-        ck_right(ph, i, j, lane, b[i]);
-        ck_right(pl, i, j, lane, bl[i]);
-      }
-#pragma unroll
-      for (int q = 0; q < 3; ++q)
-#pragma unroll
-        for (int i = 2 * j; i < 8; ++i) {
-          const uint32_t* w = (q == 2 ? bl : b)[i >> 1];
-          mma_f16(O[i], q == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
-        }
+      for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, kh == 0, kh == 1);
     }
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.empty[c % CS_STAGES])) : "memory");
     // O^T to token rows, 16 tokens at a time through the warp's own rows (48 bytes apart: no bank twice)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (KS > 1 && kh != (j == 1 || j == 2)) continue;
       __syncwarp();
       stsm_x4_t(os + (((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, cvt_bf16x2(O[2 * j][0] * down0, O[2 * j][1] * down0),
                 cvt_bf16x2(O[2 * j][2] * down1, O[2 * j][3] * down1), cvt_bf16x2(O[2 * j + 1][0] * down0, O[2 * j + 1][1] * down0),
@@ -709,7 +772,7 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
       __syncwarp();
       const int row = j * 16 + (lane >> 1);
       if (row < valid)
-        *reinterpret_cast<uint4*>(p.out + int64_t(t0 + row) * p.o_st + int64_t(hv) * p.o_sh + v0 + warp * 16 + (lane & 1) * 8) =
+        *reinterpret_cast<uint4*>(p.out + int64_t(t0 + row) * p.o_st + int64_t(hv) * p.o_sh + vr + (lane & 1) * 8) =
             *reinterpret_cast<const uint4*>(sm.out[warp] + (lane >> 1) * 48 + (lane & 1) * 16);
     }
   }
@@ -718,19 +781,20 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < KT; ++i) {
     *reinterpret_cast<float2*>(st + i * 8) = make_float2(S[i][0], S[i][1]);
     *reinterpret_cast<float2*>(st + 8 * 128 + i * 8) = make_float2(S[i][2], S[i][3]);
   }
 }
 
-template <int NW>
+template <int NW, int KS>
 cudaError_t scan(const PrefillParams& p, const CUtensorMap& map, cudaStream_t stream) {
   static DynSmemCache cache;
-  constexpr int bytes = sizeof(CsSmem<NW>) + 1024;
-  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(prefill_scan_kernel<NW>), bytes, cache);
+  constexpr int bytes = sizeof(CsSmem<NW, KS>) + 1024;
+  auto kern = prefill_scan_kernel<NW, KS>;
+  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), bytes, cache);
   if (e != cudaSuccess) return e;
-  prefill_scan_kernel<NW><<<dim3(unsigned(int64_t(p.N) * p.HV * (8 / NW))), NW * 32, bytes, stream>>>(p, map);
+  kern<<<dim3(unsigned(int64_t(p.N) * p.HV * CsCfg<NW, KS>::PARTS)), NW * 32, bytes, stream>>>(p, map);
   return cudaGetLastError();
 }
 
@@ -752,9 +816,9 @@ cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream) {
   prefill_derive_kernel<<<dim3(unsigned(ids * p.H)), CD_THREADS, bytes, stream>>>(p, map);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // 64 value rows a CTA where that gives the machine no more CTAs than it has multiprocessors (one long prompt:
-  // the chain of chunks is what takes the time), else whole heads (two warps on each tensor unit hide one another)
-  return int64_t(p.N) * p.HV * 2 <= multiprocessor_count() ? scan<4>(p, map, stream) : scan<8>(p, map, stream);
+  if (p.N * int64_t(p.HV) * 4 <= multiprocessor_count()) return scan<4, 2>(p, map, stream);
+  if (p.N * int64_t(p.HV) * 2 <= multiprocessor_count()) return scan<4, 1>(p, map, stream);
+  return scan<8, 1>(p, map, stream);
 }
 
 // The longest sequence as the host knows it, or the mean length
