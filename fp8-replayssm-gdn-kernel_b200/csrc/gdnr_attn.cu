@@ -5,9 +5,7 @@
 // for the m new tokens i of a sequence of kv tokens.  The G = Hq/Hk query heads of a key
 // head are rows of one tile (row r of a sequence: token r / G, head r % G), so a key
 // or value read from memory serves all of them.
-#include "gdnr_device.cuh"
-#include "gdnr_hybrid.h"
-#include "gdnr_tile.cuh"
+#include "gdnr_attn.cuh"
 
 #include <algorithm>
 
@@ -16,129 +14,7 @@ namespace gdnr {
 namespace {
 
 constexpr int AT_BN = 64;  // keys of a tile
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-constexpr int AT_META = 8;  // ints of one CTA's record
 constexpr int AT_MAX_CTAS_PER_SM = 2;
-
-// ---------------------------------------------------------------- work split
-// A unit is (sequence, key head, tile of BM rows); its cost is the number of key tiles
-// its last row sees.  The units of the batch laid end to end are cut into equal shares,
-// one per CTA, so ragged lengths and few heads fill the machine alike.
-template <int BM>
-__device__ __forceinline__ int unit_tiles(const AttnParams& p, int kv, int m, int rt) {
-  const int last_row = min((rt + 1) * BM, m * p.G) - 1;
-  const int keys = min(kv, kv - m + last_row / p.G + 1);
-  return max(1, (keys + AT_BN - 1) / AT_BN);  // a unit without keys still writes its rows
-}
-
-struct SeqLen {
-  int q0, m, kv;
-};
-
-__device__ __forceinline__ SeqLen seq_len(const AttnParams& p, int n) {
-  SeqLen s;
-  s.q0 = min(max(p.cu[n], 0), p.T);
-  s.m = min(max(p.cu[n + 1], s.q0), p.T) - s.q0;
-  s.kv = int(min(int64_t(max(p.kv_lens[n * p.kl_s], 0)), int64_t(p.width) * p.page_size));
-  return s;
-}
-
-template <int BM>
-__device__ int64_t seq_tiles(const AttnParams& p, const SeqLen& s) {
-  const int rts = (s.m * p.G + BM - 1) / BM;
-  int64_t sum = 0;
-  for (int rt = 0; rt < rts; ++rt) sum += unit_tiles<BM>(p, s.kv, s.m, rt);
-  return sum * p.Hk;
-}
-
-__device__ __forceinline__ int64_t warp_sum64(int64_t x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-
-// The unit that key tile `at` of the batch falls into (one whole warp).
-struct Unit {
-  int n, h, rt;
-  SeqLen s;
-  int64_t begin;  // first key tile of the unit
-  int tiles;
-};
-
-template <int BM>
-__device__ __forceinline__ Unit find_unit(const AttnParams& p, int64_t at, int lane) {
-  int64_t base = 0;
-  Unit u;
-  u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
-  u.s.q0 = u.s.m = u.s.kv = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 32) {
-    const int n = n0 + lane;
-    int64_t w = 0;
-    if (n < p.N) w = seq_tiles<BM>(p, seq_len(p, n));
-    int64_t pre = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
-      if (lane >= o) pre += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + pre > at);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
-      u.n = n0 + src;
-      u.s = seq_len(p, u.n);
-      const int64_t per_head = __shfl_sync(0xffffffffu, w, src) / p.Hk;
-      u.h = int((at - start) / per_head);
-      u.begin = start + u.h * per_head;
-      u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, 0);
-      while (u.begin + u.tiles <= at) {
-        u.begin += u.tiles;
-        u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, ++u.rt);
-      }
-      return u;
-    }
-    base += __shfl_sync(0xffffffffu, pre, 31);
-  }
-  u.n = p.N;
-  return u;
-}
-
-// The next unit in order.
-template <int BM>
-__device__ __forceinline__ void next_unit(const AttnParams& p, Unit& u) {
-  u.begin += u.tiles;
-  ++u.rt;
-  if (u.rt * BM >= u.s.m * p.G) {
-    u.rt = 0;
-    if (++u.h == p.Hk) {
-      u.h = 0;
-      do {
-        if (++u.n >= p.N) return;
-        u.s = seq_len(p, u.n);
-      } while (u.s.m == 0);
-    }
-  }
-  u.tiles = unit_tiles<BM>(p, u.s.kv, u.s.m, u.rt);
-}
-
-struct Share {
-  int64_t begin, end;
-};
-
-// Share i of `total` key tiles; at least two tiles each, so that small batches do not
-// pay for joining shares of one tile.
-__device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
-  const int64_t use = min(int64_t(ctas), (total + 1) / 2);
-  Share s;
-  if (i >= use) {
-    s.begin = s.end = total;
-    return s;
-  }
-  s.begin = total * i / use;
-  s.end = total * (i + 1) / use;
-  return s;
-}
 
 // ---------------------------------------------------------------- kernel
 // WM x WN warps: WM groups of 16 rows, each tile's keys cut over WN warps that keep
@@ -156,8 +32,9 @@ struct AtCfg {
 };
 
 template <int D, int WM, int WN, int STAGES>
-__global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constant__ AttnParams p, const AtRows of) {
   using C = AtCfg<D, WM, WN, STAGES>;
+  using T = AtTile<C::BM, AT_BN>;
   constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t sh_total;
@@ -168,9 +45,7 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
   if (warp == 0) {
-    int64_t w = 0;
-    for (int n = lane; n < p.N; n += 32) w += seq_tiles<BM>(p, seq_len(p, n));
-    w = warp_sum64(w);
+    const int64_t w = all_tiles<T>(p, of, lane);
     if (lane == 0) sh_total = w;
   }
   __syncthreads();
@@ -180,18 +55,10 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
     if (tid == 0) meta[0] = -1;
     return;
   }
-  Unit u = find_unit<BM>(p, share.begin, lane);
-  if (tid == 0) {
-    // record for the join: the unit this share begins in, if it begins inside it
-    meta[0] = share.begin > u.begin ? u.n : -1;
-    meta[1] = u.h;
-    meta[2] = u.rt;
-    meta[3] = int(share.begin - u.begin);              // tiles of that unit in earlier shares
-    meta[4] = int(u.begin + u.tiles - share.begin);    // tiles of it from here on
-    meta[5] = int(share.end - share.begin);
-  }
+  Unit u = find_unit<T>(p, of, share.begin, lane);
+  if (tid == 0) write_meta(meta, share, u);
   const float sl2 = p.scale * LOG2E;
-  for (int64_t at = share.begin; at < share.end; next_unit<BM>(p, u), at = u.begin) {
+  for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
     const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
     const int rows = u.s.m * p.G - u.rt * BM;  // rows of the sequence from this tile on
     const int row_base = u.rt * BM;
@@ -331,14 +198,12 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
         const int r = wm * 16 + (lane >> 2) + 8 * j;
         if (r >= rows) continue;
         if (whole) {
-          const int rr = row_base + r, tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
           const float inv = sum[j] > 0.f ? 1.0f / sum[j] : 0.f;
-          uint16_t* dst = p.out + int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + 2 * (lane & 3);
+          uint16_t* dst = p.out + out_at(p, u, row_base + r) + 2 * (lane & 3);
 #pragma unroll
           for (int c = 0; c < D / 8; ++c)
             *reinterpret_cast<uint32_t*>(dst + c * 8) = pack_bf16x2(o[c][2 * j] * inv, o[c][2 * j + 1] * inv);
-          if (p.lse && (lane & 3) == 0)
-            p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = sum[j] > 0.f ? (mx[j] + log2f(sum[j])) * LN2 : -INFINITY;
+          if ((lane & 3) == 0) write_lse(p, u.s, u.h, row_base + r, mx[j], sum[j]);
         } else {
           float* dst = part + r * (D + 2);
 #pragma unroll
@@ -371,7 +236,7 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
           f[w] = ex2_approx(js[(w * 16 + r) * LD + D] - b);
           l += f[w] * js[(w * 16 + r) * LD + D + 1];
         }
-        const int rr = row_base + r, tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
+        const int64_t to = out_at(p, u, row_base + r);
         const float inv = l > 0.f ? 1.0f / l : 0.f;
         for (int c = lane * 2; c < D; c += 64) {
           float2 x = make_float2(0.f, 0.f);
@@ -382,15 +247,15 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
             x.y += f[w] * y.y;
           }
           if (whole)
-            *reinterpret_cast<uint32_t*>(p.out + int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + c) = pack_bf16x2(x.x * inv, x.y * inv);
+            *reinterpret_cast<uint32_t*>(p.out + to + c) = pack_bf16x2(x.x * inv, x.y * inv);
           else
             *reinterpret_cast<float2*>(part + r * (D + 2) + c) = x;
         }
         if (lane == 0) {
           if (!whole)
             part[r * (D + 2) + D] = m, part[r * (D + 2) + D + 1] = l;
-          else if (p.lse)
-            p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+          else
+            write_lse(p, u.s, u.h, row_base + r, m, l);
         }
       }
       __syncthreads();  // the next unit's tiles overwrite the join
@@ -398,16 +263,18 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
   }
 }
 
-// Joins the parts of the units that are cut between shares.  Block (i - 1, r) looks at
+// Joins the parts of the units that are cut between shares.  Block (i - 1, y) looks at
 // the cut between shares i - 1 and i: where it is the first cut of its unit, the
-// block joins row r of all parts in the order of the shares (a fixed order: the
-// result does not depend on which CTA ran when).
+// block joins ROWS rows of all parts in the order of the shares (a fixed order: the
+// result does not depend on which CTA ran when).  The eight warps have a row each, or share one
+// row's parts: a unit of few rows may be cut into as many parts as there are shares.
 constexpr int AJ_WARPS = 8;
 
-template <int D, int BM>
-__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
+template <int D, int BM, int ROWS>
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_constant__ AttnParams p, const AtRows of, int ctas) {
+  constexpr int PER_ROW = AJ_WARPS / ROWS;
   __shared__ float sm[AJ_WARPS][D + 2];
-  const int i = blockIdx.x + 1, r = blockIdx.y;
+  const int i = blockIdx.x + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int* metas = reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2));
   const int* mi = metas + i * AT_META;
@@ -415,87 +282,133 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   if (n < 0) return;  // no unit is cut here
   const int before = mi[3], left = mi[4];
   if (metas[(i - 1) * AT_META + 5] < before) return;  // the unit begins before share i - 1: not its first cut
-  const SeqLen s = seq_len(p, n);
-  const int rr = mi[2] * BM + r;
-  if (rr >= s.m * p.G) return;
-  // shares are equal but for rounding: find how many take part
-  int parts = 2;
-  for (int have = mi[5], c = i + 1; have < left; ++c, ++parts) have += metas[c * AT_META + 5];
+  const SeqLen s = seq_len(p, n, of);
+  const int r = blockIdx.y * ROWS + warp / PER_ROW, rr = mi[2] * BM + r;
+  const bool live = r < BM && rr < s.m * p.G;
+  if (__syncthreads_or(live) == 0) return;
   constexpr int E = D / 32;
   float m = -INFINITY, l = 0.f, x[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = 0.f;
-  for (int c = warp; c < parts; c += AJ_WARPS) {
-    const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
-    const float pm = src[D], pl = src[D + 1];
-    const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
-    const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
-    m = nm;
-    l = l * f0 + pl * f1;
+  if (live) {
+    // shares are equal but for rounding: find how many take part
+    int parts = 2;
+    for (int have = mi[5], c = i + 1; have < left; ++c, ++parts) have += metas[c * AT_META + 5];
+    for (int c = warp % PER_ROW; c < parts; c += PER_ROW) {
+      const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
+      const float pm = src[D], pl = src[D + 1];
+      const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
+      const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
+      m = nm;
+      l = l * f0 + pl * f1;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + src[e * 32 + lane] * f1;
+      for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + src[e * 32 + lane] * f1;
+    }
   }
+  if constexpr (PER_ROW > 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm[warp][e * 32 + lane] = x[e];
-  if (lane == 0) sm[warp][D] = m, sm[warp][D + 1] = l;
-  __syncthreads();
-  m = -INFINITY;
+    for (int e = 0; e < E; ++e) sm[warp][e * 32 + lane] = x[e];
+    if (lane == 0) sm[warp][D] = m, sm[warp][D + 1] = l;
+    __syncthreads();
+    const int w0 = warp / PER_ROW * PER_ROW;
+    if (warp != w0) return;
+    m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < AJ_WARPS; ++w) m = fmaxf(m, sm[w][D]);
-  const float b = m == -INFINITY ? 0.f : m;
-  l = 0.f;
-  float f[AJ_WARPS];
+    for (int w = 0; w < PER_ROW; ++w) m = fmaxf(m, sm[w0 + w][D]);
+    const float b = m == -INFINITY ? 0.f : m;
+    l = 0.f;
 #pragma unroll
-  for (int w = 0; w < AJ_WARPS; ++w) {
-    f[w] = ex2_approx(sm[w][D] - b);
-    l += f[w] * sm[w][D + 1];
+    for (int e = 0; e < E; ++e) x[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < PER_ROW; ++w) {
+      const float f = ex2_approx(sm[w0 + w][D] - b);
+      l += f * sm[w0 + w][D + 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += f * sm[w0 + w][e * 32 + lane];
+    }
   }
-  const int tok = s.q0 + rr / p.G, hd = mi[1] * p.G + rr % p.G;
+  if (!live) return;
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  for (int c = threadIdx.x; c < D; c += AJ_WARPS * 32) {
-    float y = 0.f;
+  uint16_t* dst = p.out + int64_t(s.q0 + rr / p.G) * p.o_st + int64_t(mi[1] * p.G + rr % p.G) * p.o_sh;
 #pragma unroll
-    for (int w = 0; w < AJ_WARPS; ++w) y += f[w] * sm[w][c];
-    p.out[int64_t(tok) * p.o_st + int64_t(hd) * p.o_sh + c] = f_to_bf16(y * inv);
-  }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[int64_t(tok) * p.l_st + int64_t(hd) * p.l_sh] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+  for (int e = 0; e < E; ++e) dst[e * 32 + lane] = f_to_bf16(x[e] * inv);
+  if (lane == 0) write_lse(p, s, mi[1], rr, m, l);
+}
+
+template <int D, int BM, int ROWS>
+void join(const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
+  // rows a unit can have, by the longest sequence the host knows of
+  const int rows = int(std::min<int64_t>(BM, int64_t(p.max_q) * p.G));
+  attn_join_kernel<D, BM, ROWS><<<dim3(ctas - 1, (rows + ROWS - 1) / ROWS), AJ_WARPS * 32, 0, stream>>>(p, of, ctas);
+}
+
+template <int D>
+void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream_t stream) {
+  if (bm == 16)
+    join<D, 16, 1>(p, ctas, of, stream);
+  else if (bm == 64)
+    join<D, 64, 2>(p, ctas, of, stream);
+  else
+    join<D, D == 256 ? 128 : 256, 8>(p, ctas, of, stream);
 }
 
 template <int D, int WM, int WN, int STAGES, int PER_SM>
-cudaError_t run(const AttnParams& p, cudaStream_t stream) {
+cudaError_t run(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
   using C = AtCfg<D, WM, WN, STAGES>;
   static DynSmemCache cache;
   auto kern = attn_kernel<D, WM, WN, STAGES>;
   cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
   if (e != cudaSuccess) return e;
   const int ctas = multiprocessor_count() * PER_SM;
-  if ((int64_t(ctas) * 2 * C::BM * (D + 2) + ctas * AT_META) * 4 > p.ws_bytes) return cudaErrorInvalidValue;
-  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p);
+  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, of);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  const int rows = int(std::min<int64_t>(C::BM, int64_t(p.max_q) * p.G));
-  attn_join_kernel<D, C::BM><<<dim3(ctas - 1, rows), AJ_WARPS * 32, 0, stream>>>(p, ctas);
-  return cudaGetLastError();
+  return launch_attn_join(p, ctas, C::BM, of, stream);
 }
 
 template <int D, int STAGES, int PER_SM>
-cudaError_t pick(const AttnParams& p, cudaStream_t stream) {
-  if (int64_t(p.max_q) * p.G <= 16) return run<D, 1, 4, STAGES, PER_SM>(p, stream);
-  return run<D, 4, 1, STAGES, PER_SM>(p, stream);
+cudaError_t pick(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
+  if (most <= 16) return run<D, 1, 4, STAGES, PER_SM>(p, of, stream);
+  return run<D, 4, 1, STAGES, PER_SM>(p, of, stream);
 }
+
+cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
+  if (p.D == 64) return pick<64, 3, 2>(p, most, of, stream);
+  if (p.D == 128) return pick<128, 3, 2>(p, most, of, stream);
+  return pick<256, 2, 1>(p, most, of, stream);
+}
+
+// Sequences of at most so many rows (tokens times query heads of a key head) are bound by reading their keys
+// and stay on warp-level tiles.
+constexpr int AT_FEW_ROWS = 64;
 
 }  // namespace
 
+cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream) {
+  if (ctas < 2) return cudaSuccess;
+  if (p.D == 64)
+    join_of<64>(p, ctas, bm, rows, stream);
+  else if (p.D == 128)
+    join_of<128>(p, ctas, bm, rows, stream);
+  else
+    join_of<256>(p, ctas, bm, rows, stream);
+  return cudaGetLastError();
+}
+
 int64_t attn_workspace_bytes(int head_dim) {
-  const int64_t ctas = int64_t(multiprocessor_count()) * AT_MAX_CTAS_PER_SM;
-  return (ctas * 2 * 64 * (head_dim + 2) + ctas * AT_META) * 4;
+  const int64_t sms = multiprocessor_count(), ctas = sms * AT_MAX_CTAS_PER_SM;
+  const int64_t rows = std::max<int64_t>(ctas * 2 * 64, sms * 2 * attn_tc_rows(head_dim));
+  return (rows * (head_dim + 2) + ctas * AT_META) * 4;
 }
 
 cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream) {
-  if (p.D == 64) return pick<64, 3, 2>(p, stream);
-  if (p.D == 128) return pick<128, 3, 2>(p, stream);
-  return pick<256, 2, 1>(p, stream);
+  const int64_t most = std::min<int64_t>(int64_t(p.max_q) * p.G, INT32_MAX);
+  if (most <= AT_FEW_ROWS || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, stream);
+  // sequences of many rows on the tensor-memory tiles, the others, if there can be any, as above
+  if (int64_t(p.T) == int64_t(p.N) * p.max_q) return launch_attn_tc(p, 0, stream);  // all of the same length
+  cudaError_t e = launch_attn_tc(p, AT_FEW_ROWS, stream);
+  if (e != cudaSuccess) return e;
+  return small_rows(p, AT_FEW_ROWS, AtRows{0, AT_FEW_ROWS}, stream);
 }
 
 }  // namespace gdnr

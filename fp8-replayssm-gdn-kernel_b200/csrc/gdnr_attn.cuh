@@ -1,0 +1,186 @@
+// Work split of the paged-attention kernels: units, equal shares, and how a cut unit is joined.
+#pragma once
+
+#include "gdnr_device.cuh"
+#include "gdnr_hybrid.h"
+#include "gdnr_tile.cuh"
+
+namespace gdnr {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int AT_META = 8;  // ints of one CTA's record
+
+// A kernel's tiles: BM rows (token, query head) by BN keys, for the sequences whose rows are in (lo, hi].
+template <int BM_, int BN_>
+struct AtTile {
+  static constexpr int BM = BM_, BN = BN_;
+};
+
+struct AtRows {
+  int lo, hi;
+};
+
+struct SeqLen {
+  int q0, m, kv;
+};
+
+__device__ __forceinline__ SeqLen seq_len(const AttnParams& p, int n) {
+  SeqLen s;
+  s.q0 = min(max(p.cu[n], 0), p.T);
+  s.m = min(max(p.cu[n + 1], s.q0), p.T) - s.q0;
+  s.kv = int(min(int64_t(max(p.kv_lens[n * p.kl_s], 0)), int64_t(p.width) * p.page_size));
+  return s;
+}
+
+// As seq_len, without rows where the sequence is another kernel's.
+__device__ __forceinline__ SeqLen seq_len(const AttnParams& p, int n, const AtRows& r) {
+  SeqLen s = seq_len(p, n);
+  if (s.m * p.G <= r.lo || s.m * p.G > r.hi) s.m = 0;
+  return s;
+}
+
+// Keys that rows up to (not including) `rows` of a sequence see.
+__device__ __forceinline__ int keys_seen(const AttnParams& p, const SeqLen& s, int rows) {
+  return min(s.kv, s.kv - s.m + (min(rows, s.m * p.G) - 1) / p.G + 1);
+}
+
+// A unit is (sequence, key head, tile of BM rows); its cost is the number of key tiles
+// its last row sees.  The units of the batch laid end to end are cut into equal shares,
+// one per CTA, so ragged lengths and few heads fill the machine alike.
+template <class T>
+__device__ __forceinline__ int unit_tiles(const AttnParams& p, const SeqLen& s, int rt) {
+  return max(1, (keys_seen(p, s, (rt + 1) * T::BM) + T::BN - 1) / T::BN);  // a unit without keys still writes its rows
+}
+
+template <class T>
+__device__ int64_t seq_tiles(const AttnParams& p, const SeqLen& s) {
+  const int rts = (s.m * p.G + T::BM - 1) / T::BM;
+  int64_t sum = 0;
+  for (int rt = 0; rt < rts; ++rt) sum += unit_tiles<T>(p, s, rt);
+  return sum * p.Hk;
+}
+
+// Key tiles of the batch (one whole warp).
+template <class T>
+__device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& r, int lane) {
+  int64_t w = 0;
+  for (int n = lane; n < p.N; n += 32) w += seq_tiles<T>(p, seq_len(p, n, r));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+  return w;
+}
+
+struct Unit {
+  int n, h, rt;
+  SeqLen s;
+  int64_t begin;  // first key tile of the unit
+  int tiles;
+};
+
+// The unit that key tile `at` of the batch falls into (one whole warp).
+template <class T>
+__device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, int64_t at, int lane) {
+  int64_t base = 0;
+  Unit u;
+  u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
+  u.s.q0 = u.s.m = u.s.kv = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    const int n = n0 + lane;
+    int64_t w = 0;
+    if (n < p.N) w = seq_tiles<T>(p, seq_len(p, n, r));
+    int64_t pre = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + pre > at);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
+      u.n = n0 + src;
+      u.s = seq_len(p, u.n, r);
+      const int64_t per_head = __shfl_sync(0xffffffffu, w, src) / p.Hk;
+      u.h = int((at - start) / per_head);
+      u.begin = start + u.h * per_head;
+      u.tiles = unit_tiles<T>(p, u.s, 0);
+      while (u.begin + u.tiles <= at) {
+        u.begin += u.tiles;
+        u.tiles = unit_tiles<T>(p, u.s, ++u.rt);
+      }
+      return u;
+    }
+    base += __shfl_sync(0xffffffffu, pre, 31);
+  }
+  u.n = p.N;
+  return u;
+}
+
+// The next unit in order.
+template <class T>
+__device__ __forceinline__ void next_unit(const AttnParams& p, const AtRows& r, Unit& u) {
+  u.begin += u.tiles;
+  ++u.rt;
+  if (u.rt * T::BM >= u.s.m * p.G) {
+    u.rt = 0;
+    if (++u.h == p.Hk) {
+      u.h = 0;
+      do {
+        if (++u.n >= p.N) return;
+        u.s = seq_len(p, u.n, r);
+      } while (u.s.m == 0);
+    }
+  }
+  u.tiles = unit_tiles<T>(p, u.s, u.rt);
+}
+
+struct Share {
+  int64_t begin, end;
+};
+
+// Share i of `total` key tiles; at least two tiles each, so that small batches do not
+// pay for joining shares of one tile.
+__device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
+  const int64_t use = min(int64_t(ctas), (total + 1) / 2);
+  Share s;
+  if (i >= use) {
+    s.begin = s.end = total;
+    return s;
+  }
+  s.begin = total * i / use;
+  s.end = total * (i + 1) / use;
+  return s;
+}
+
+// A CTA's record for the join, in the workspace behind the parts [ctas][2][BM][D + 2]: a share that
+// begins inside a unit leaves its part of it in slot 0, one that only ends inside in slot 1.
+__device__ __forceinline__ void write_meta(int* meta, const Share& share, const Unit& u) {
+  meta[0] = share.begin > u.begin ? u.n : -1;  // the unit this share begins in, if it begins inside it
+  meta[1] = u.h;
+  meta[2] = u.rt;
+  meta[3] = int(share.begin - u.begin);            // tiles of that unit in earlier shares
+  meta[4] = int(u.begin + u.tiles - share.begin);  // tiles of it from here on
+  meta[5] = int(share.end - share.begin);
+}
+
+// Row r of a sequence: token q0 + r / G, query head h G + r % G.
+__device__ __forceinline__ int64_t out_at(const AttnParams& p, const Unit& u, int row) {
+  return int64_t(u.s.q0 + row / p.G) * p.o_st + int64_t(u.h * p.G + row % p.G) * p.o_sh;
+}
+
+__device__ __forceinline__ void write_lse(const AttnParams& p, const SeqLen& s, int h, int row, float max2, float sum) {
+  if (p.lse)
+    p.lse[int64_t(s.q0 + row / p.G) * p.l_st + int64_t(h * p.G + row % p.G) * p.l_sh] =
+        sum > 0.f ? (max2 + log2f(sum)) * LN2 : -INFINITY;
+}
+
+// Joins the parts of the units of BM rows that were cut between `ctas` shares (gdnr_attn.cu).
+cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream);
+
+// Tiles on the fifth-generation tensor cores (gdnr_attn_tc.cu): sequences of more than `lo` rows.
+bool attn_tc_takes(const AttnParams& p);
+cudaError_t launch_attn_tc(const AttnParams& p, int lo, cudaStream_t stream);
+int attn_tc_rows(int head_dim);
+
+}  // namespace gdnr

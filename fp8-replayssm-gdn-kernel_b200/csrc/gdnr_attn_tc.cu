@@ -1,0 +1,552 @@
+// Paged attention of sequences with many rows, on tcgen05.
+//
+// A CTA walks its share of the batch's (row tile, key tile) pairs.  NQ streams of 128 rows (one
+// where D = 256, whose accumulator takes half of tensor memory) share the keys and
+// values, which TMA brings page by page into a ring of tiles:
+//   load warp      keys and values of tile 0, 1, ...
+//   matrix warp    S = Q K^T into tensor memory; O += P V with P from tensor memory
+//   softmax warps  four a stream, a thread a row: S -> registers, maximum, exponentials, their sum,
+//                  P as bf16 over S
+// While one stream's softmax runs, the tensor cores work for the other (or, with one
+// stream, on the next tile's S).  The reference maximum of a row only moves when the row's maximum
+// has grown by more than 2^8 (p <= 2^8 keeps bf16's relative precision); only then O is rescaled.
+#include "gdnr_attn.cuh"
+
+#include <algorithm>
+
+namespace gdnr {
+
+namespace {
+
+template <int D>
+struct TcCfg {
+  static constexpr int NQ = D == 256 ? 1 : 2;
+  static constexpr int BN = D == 256 ? 64 : 128;
+  static constexpr int BM = 128 * NQ;
+  static constexpr int ATOMS = D / 64;                  // 64-element (128-byte) column blocks
+  static constexpr int Q_BYTES = 128 * D * 2;           // a stream
+  static constexpr int KV_BYTES = BN * D * 2;           // a tile of keys or of values
+  static constexpr int RING = D == 256 ? 5 : (D == 128 ? 5 : 8);
+  static constexpr int SOFTMAX_WARPS = 4 * NQ;
+  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
+  static constexpr int SMEM = NQ * Q_BYTES + RING * KV_BYTES + 1024;
+  // tensor memory columns: two buffers of S (P lies over the first half of its S), then O
+  static constexpr int S_COLS = BN, O_COL = 256;
+  static_assert(SMEM + 512 <= 227 * 1024, "one CTA per SM");
+};
+
+__device__ __forceinline__ uint64_t tc_desc_k(uint32_t addr) {  // rows of 128 bytes, 128-byte swizzle, K contiguous
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+
+// K in rows of 128 bytes (64 elements of N), 128-byte swizzle: groups of eight rows 1024 bytes apart, column blocks
+// `lbo` bytes apart
+__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr, uint32_t lbo) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+// f32 accumulator, bf16 operands, M = 128; B with N contiguous where `bn`
+__host__ __device__ constexpr uint32_t tc_idesc(int n, bool bn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (bn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define TC_R8(o) "=f"(r[o]), "=f"(r[o + 1]), "=f"(r[o + 2]), "=f"(r[o + 3]), "=f"(r[o + 4]), "=f"(r[o + 5]), "=f"(r[o + 6]), "=f"(r[o + 7])
+#define TC_W8(o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+
+// 32 columns of the thread's lane; the values are there after tc_wait_ld
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : TC_R8(0), TC_R8(8), TC_R8(16), TC_R8(24)
+      : "r"(addr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::TC_W8(0),
+      TC_W8(8), TC_W8(16), TC_W8(24), "r"(addr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap* map, int c, int h, int off, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(c), "r"(h), "r"(off), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+struct TcBars {
+  uint64_t kv_full[8], kv_empty[8];
+  uint64_t q_full[2];   // softmax warps -> matrix warp: the stream's query rows are in shared memory
+  uint64_t s_full[2];   // matrix warp -> softmax warps: S of the buffer is complete
+  uint64_t p_full[2];   // softmax warps -> matrix warp: P of the buffer is written (and O rescaled)
+  uint64_t o_full;      // one stream: PV of a key tile is complete (what O must wait for before it is rescaled)
+  uint64_t done[2];     // matrix warp -> softmax warps: the stream's last PV of a unit is complete
+  int abort;
+  uint32_t tmem;
+  int64_t total;
+};
+
+// Waits of a whole warp; they give up after a second, or when another warp has: then every role leaves its loop.
+struct TcWait {
+  uint32_t* err;
+  volatile int* abort;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    bool ok = mbar_try_wait(smem_addr(bar), parity);
+    if (!ok) ok = slow(bar, parity);
+    return __all_sync(0xffffffffu, ok);
+  }
+  __device__ __noinline__ bool slow(uint64_t* bar, uint32_t parity) const {
+    const uint32_t a = smem_addr(bar);
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1; it < WAIT_LIMIT_ITERS; ++it) {
+      if (mbar_try_wait(a, parity)) return true;
+      if ((it & 63u) == 0) {
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
+      }
+    }
+    *abort = 1;
+    atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
+    return false;
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
+    attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                   const AtRows of) {
+  using C = TcCfg<D>;
+  using T = AtTile<C::BM, C::BN>;
+  constexpr int NQ = C::NQ, BN = C::BN, BM = C::BM;
+  extern __shared__ uint8_t raw[];
+  __shared__ TcBars bars;
+  const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u, kv_base = base + NQ * C::Q_BYTES;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
+  int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
+
+  if (warp == 0) {
+    const int64_t w = all_tiles<T>(p, of, lane);
+    if (lane == 0) bars.total = w;
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bars.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid == 64) {
+    for (int i = 0; i < C::RING; ++i) {
+      mbar_init(&bars.kv_full[i], 1);
+      mbar_init(&bars.kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], 4);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.done[i], 1);
+    }
+    mbar_init(&bars.o_full, 1);
+    bars.abort = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const Share share = share_of(bars.total, blockIdx.x, gridDim.x);
+  const TcWait wait{p.err, &bars.abort};
+  Unit u;
+  u.n = p.N;
+  if (share.begin < share.end) {
+    u = find_unit<T>(p, of, share.begin, lane);
+    if (tid == 0) write_meta(meta, share, u);
+  } else if (tid == 0) {
+    meta[0] = -1;
+  }
+
+  // key tiles [t0, t1) of the unit are this share's; stream q sees the first seen(q) tiles of the unit
+  auto seen = [&](int q) {
+    const int rows = u.rt * BM + (q + 1) * 128;
+    if (u.rt * BM + q * 128 >= u.s.m * p.G) return 0;
+    return max(0, (keys_seen(p, u.s, rows) + BN - 1) / BN);
+  };
+
+  if (warp == C::SOFTMAX_WARPS + 1) {
+    // ------------------------------------------------------------ load warp
+    uint32_t slot = 0;  // tiles requested so far
+    bool ok = true;
+    constexpr int PER_SLOT = BN;
+    const int box = min(p.page_size, BN), boxes = PER_SLOT / box * C::ATOMS;
+    for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
+      const int t0 = int(at - u.begin);
+      int t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      int most = seen(0);
+      if (NQ > 1) most = max(most, seen(1));
+      t1 = min(t1, most);
+      const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
+      for (int t = t0; ok && t < t1; ++t) {
+        // where this lane's boxes come from: a page past the sequence's end, or outside the cache, reads as zeros
+        const int atom = lane % C::ATOMS, part = lane / C::ATOMS, tok = t * BN + part * box;
+        int page = p.pages, off = 0;
+        if (lane < boxes && tok < u.s.kv) {
+          const int pi = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
+          off = tok - pi * p.page_size;
+          page = table[pi];
+          if (page < 0 || page >= p.pages) {
+            page = p.pages, off = 0;
+            atomicOr(p.err, GDNR_DEVERR_BAD_SLOT);
+          }
+        }
+        for (int kv = 0; kv < 2; ++kv, ++slot) {
+          const uint32_t s = slot % C::RING;
+          if (slot >= C::RING) ok = wait(&bars.kv_empty[s], (slot / C::RING - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[s], C::KV_BYTES);
+          __syncwarp();
+          if (lane < boxes)
+            tc_tma(kv_base + s * C::KV_BYTES + atom * (BN * 128) + part * box * 128, kv ? &vmap : &kmap, atom * 64, u.h, off, page,
+                   &bars.kv_full[s]);
+        }
+      }
+    }
+    if (!ok)  // copies in flight end before the CTA does
+      for (uint32_t k = slot > C::RING ? slot - C::RING : 0; k < slot; ++k) {
+        const uint64_t t = globaltimer_ns();
+        while (!mbar_try_wait(smem_addr(&bars.kv_full[k % C::RING]), (k / C::RING) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
+        }
+      }
+  } else if (warp == C::SOFTMAX_WARPS) {
+    // ------------------------------------------------------------ matrix warp
+    uint32_t slot = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // tiles consumed; phases of q_full, p_full
+    constexpr uint32_t QK = tc_idesc(BN, false), PV = tc_idesc(D, true);
+    bool ok = true;
+    auto kv_wait = [&](uint32_t k) { return wait(&bars.kv_full[k % C::RING], (k / C::RING) & 1); };
+    auto kv_addr = [&](uint32_t k) { return kv_base + (k % C::RING) * C::KV_BYTES; };
+    auto score = [&](int q, int buf, uint32_t k) {  // S[buf] = Q_q K^T
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        tc_mma_ss(tmem + buf * C::S_COLS, tc_desc_k(base + q * C::Q_BYTES + (i >> 2) * 16384 + (i & 3) * 32),
+                  tc_desc_k(kv_addr(k) + (i >> 2) * (BN * 128) + (i & 3) * 32), QK, i > 0);
+      tc_commit(&bars.s_full[buf]);
+    };
+    auto weigh = [&](int q, int buf, uint32_t k, bool first, bool last) {  // O_q += P[buf] V
+#pragma unroll
+      for (int i = 0; i < BN / 16; ++i)
+        tc_mma_ts(tmem + C::O_COL + q * D, tmem + buf * C::S_COLS + i * 8, tc_desc_mn(kv_addr(k) + i * 2048, BN * 128), PV,
+                  !first || i > 0);
+      if (NQ == 1) tc_commit(&bars.o_full);
+      if (last) tc_commit(&bars.done[q]);
+    };
+    for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
+      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      int end[2] = {min(t1, seen(0)), NQ > 1 ? min(t1, seen(1)) : 0};
+      const int last = max(end[0], end[1]);
+      if (last <= t0) continue;
+      for (int q = 0; q < NQ && ok; ++q)
+        if (end[q] > t0) ok = wait(&bars.q_full[q], nq[q]++ & 1);
+      // tile t: keys in slot k0 + 2 (t - t0), values in the next one
+      const uint32_t k0 = slot;
+      // the last page may end inside the tile: what its rows past the end hold (it may be NaN) must not meet a weight of zero
+      auto clean = [&](int t, uint32_t k) {
+        const int from = u.s.kv - t * BN;
+        if (from >= BN) return;
+        for (int i = lane; i < (BN - from) * C::ATOMS * 8; i += 32) {
+          const int row = from + i / (C::ATOMS * 8), j = i % (C::ATOMS * 8);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv_addr(k) + (j >> 3) * (BN * 128) + row * 128 + (j & 7) * 16), "r"(0)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      };
+      auto free_slot = [&](uint32_t k) {
+        if (lane == 0) tc_commit(&bars.kv_empty[k % C::RING]);
+      };
+      if constexpr (NQ == 2) {
+        // S0(t), S1(t); then for each stream P(t) V(t) and S(t + 1)
+        if (ok) ok = kv_wait(k0);
+        if (ok && lane == 0)
+          for (int q = 0; q < 2; ++q)
+            if (end[q] > t0) score(q, q, k0);
+        free_slot(k0);
+        for (int t = t0; t < last && ok; ++t) {
+          const uint32_t kk = k0 + 2 * (t + 1 - t0), kv = k0 + 2 * (t - t0) + 1;
+          ok = kv_wait(kv);
+          if (!ok) break;
+          clean(t, kv);
+          bool have_k = false;
+          for (int q = 0; q < 2 && ok; ++q) {
+            if (t >= end[q]) continue;
+            ok = wait(&bars.p_full[q], np[q]++ & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) weigh(q, q, kv, t == t0, t + 1 == end[q]);
+            if (t + 1 < end[q]) {
+              if (!have_k) ok = kv_wait(kk), have_k = true;
+              if (!ok) break;
+              if (lane == 0) score(q, q, kk);
+            }
+            __syncwarp();
+          }
+          free_slot(kv);
+          if (t + 1 < last) free_slot(kk);
+        }
+      } else {
+        // S(t + 1) is issued before P(t) V(t), into the other buffer
+        if (ok) ok = kv_wait(k0);
+        if (ok && lane == 0) score(0, t0 & 1, k0);
+        free_slot(k0);
+        for (int t = t0; t < last && ok; ++t) {
+          const uint32_t kk = k0 + 2 * (t + 1 - t0), kv = k0 + 2 * (t - t0) + 1;
+          if (t + 1 < last) {
+            ok = kv_wait(kk);
+            if (!ok) break;
+            if (lane == 0) score(0, (t + 1) & 1, kk);
+            __syncwarp();
+          }
+          ok = kv_wait(kv);
+          if (!ok) break;
+          clean(t, kv);
+          ok = wait(&bars.p_full[t & 1], np[t & 1]++ & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) weigh(0, t & 1, kv, t == t0, t + 1 == last);
+          __syncwarp();
+          free_slot(kv);
+          if (t + 1 < last) free_slot(kk);
+        }
+      }
+      slot = k0 + 2 * (last - t0);
+    }
+    if (!ok) {  // tensor-core work in flight ends before its memory is given back
+      const uint64_t t = globaltimer_ns();
+      while (globaltimer_ns() - t < 1000000) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const int q = NQ > 1 ? warp >> 2 : 0, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t(warp & 3) << 21;  // the warp's tensor memory lanes (bits 16..)
+    const uint32_t q_smem = base + q * C::Q_BYTES, o_mem = tmem + lanes + C::O_COL + q * D;
+    const float sl2 = p.scale * LOG2E;
+    uint32_t ns[2] = {0, 0}, no = 0, nd = 0;  // phases of s_full, o_full, done
+    bool ok = true;
+    for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
+      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const int end = min(t1, seen(q));
+      const int row = u.rt * BM + q * 128 + r;  // row of the sequence
+      const bool live = row < u.s.m * p.G;
+      const int lim = live ? min(u.s.kv - 1, u.s.kv - u.s.m + row / p.G) : -1;  // last key the row sees
+      if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+      float mx = -INFINITY, sum = 0.f;
+      if (end > t0) {
+        // 16 lanes (D = 128) copy a row; rows past the sequence's are zeros
+        constexpr int CH = D / 8;
+        for (int i = lane; i < 32 * CH; i += 32) {
+          const int rr = (warp & 3) * 32 + i / CH, c = i % CH, srow = u.rt * BM + q * 128 + rr;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (srow < u.s.m * p.G)
+            x = *reinterpret_cast<const uint4*>(p.q + int64_t(u.s.q0 + srow / p.G) * p.q_st + int64_t(u.h * p.G + srow % p.G) * p.q_sh + c * 8);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (c >> 3) * 16384 + swz<128>(rr, c & 7)), "r"(x.x), "r"(x.y),
+                       "r"(x.z), "r"(x.w)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc_arrive(&bars.q_full[q]);
+      }
+      const int warp_lim = __reduce_min_sync(0xffffffffu, lim);
+      for (int t = t0; t < end; ++t) {
+        const int buf = NQ > 1 ? q : t & 1;
+        ok = wait(&bars.s_full[buf], ns[buf]++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_mem = tmem + lanes + buf * C::S_COLS;
+        float s[BN];
+#pragma unroll
+        for (int i = 0; i < BN / 32; ++i) tc_ld32(s_mem + i * 32, s + i * 32);
+        tc_wait_ld();
+        if (warp_lim < t * BN + BN - 1) {  // some row of the warp does not see the whole tile
+          const int left = lim - t * BN;
+#pragma unroll
+          for (int i = 0; i < BN; ++i) s[i] = i <= left ? s[i] : -INFINITY;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < BN; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+        const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+        if (t == t0) {
+          mx = tm;
+        } else if (__any_sync(0xffffffffu, tm > mx + 8.0f)) {
+          // O is at rest once the previous tile's PV is; its phase cannot pass before this tile's P
+          if constexpr (NQ == 1) {
+            ok = wait(&bars.o_full, (no - 1) & 1);
+            if (!ok) break;
+          }
+          tc_fence_after();
+          const bool grow = tm > mx + 8.0f;
+          const float f = grow ? ex2_approx(mx - tm) : 1.0f;
+          if (grow) mx = tm;
+          sum *= f;
+#pragma unroll 1
+          for (int i = 0; i < D; i += 32) {
+            float o[32];
+            tc_ld32(o_mem + i, o);
+            tc_wait_ld();
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * f);
+            tc_st32(o_mem + i, w);
+          }
+        }
+        const float b = mx == -INFINITY ? 0.f : mx;  // a row that has seen no key yet
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < BN / 64; ++i) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = ex2_approx(fmaf(s[i * 64 + 2 * j], sl2, -b)), y = ex2_approx(fmaf(s[i * 64 + 2 * j + 1], sl2, -b));
+            part[(2 * j) & 3] += x;
+            part[(2 * j + 1) & 3] += y;
+            // weights are rounded to bf16 for the tensor cores; their sum is taken before that
+            w[j] = cvt_bf16x2(x, y);
+          }
+          tc_st32(s_mem + i * 32, w);
+        }
+        tc_wait_st();
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc_arrive(&bars.p_full[buf]);
+        ++no;
+      }
+      if (!ok) break;
+      const bool any = end > t0;
+      if (any) {
+        ok = wait(&bars.done[q], nd++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool whole = t0 == 0 && t1 == u.tiles;
+      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+      uint16_t* dst = live ? p.out + out_at(p, u, row) : nullptr;
+      float* part = ws_o + ((t0 > 0 ? 0 : 1) * BM + q * 128 + r) * (D + 2);
+#pragma unroll 1
+      for (int i = 0; i < D; i += 32) {
+        float o[32];
+        if (any) {
+          tc_ld32(o_mem + i, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.f;
+        }
+        if (live && whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(dst + i + j * 8) =
+                make_uint4(cvt_bf16x2(o[8 * j] * inv, o[8 * j + 1] * inv), cvt_bf16x2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                           cvt_bf16x2(o[8 * j + 4] * inv, o[8 * j + 5] * inv), cvt_bf16x2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+        } else if (live) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) *reinterpret_cast<float2*>(part + i + j * 2) = make_float2(o[2 * j], o[2 * j + 1]);
+        }
+        __syncwarp();
+      }
+      if (live) {
+        if (whole)
+          write_lse(p, u.s, u.h, row, mx, sum);
+        else
+          part[D] = mx, part[D + 1] = sum;
+      }
+      tc_fence_before();  // O has been read before the next unit's first P is announced
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <int D>
+cudaError_t run_tc(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
+  using C = TcCfg<D>;
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[4] = {uint64_t(D), uint64_t(p.Hk), uint64_t(p.page_size), uint64_t(p.pages)};
+    const uint64_t strides[3] = {uint64_t(i ? p.v_sh : p.k_sh) * 2, uint64_t(i ? p.v_st : p.k_st) * 2, uint64_t(i ? p.v_sp : p.k_sp) * 2};
+    const uint32_t box[4] = {64, 1, uint32_t(std::min(p.page_size, C::BN)), 1};
+    cudaError_t e = encode_bf16_map(&maps[i], i ? p.v : p.k, 4, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
+  static DynSmemCache cache;
+  auto kern = attn_tc_kernel<D>;
+  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
+  if (e != cudaSuccess) return e;
+  const int ctas = multiprocessor_count();
+  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], of);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_attn_join(p, ctas, C::BM, of, stream);
+}
+
+}  // namespace
+
+int attn_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
+
+// Pages that tiles of keys are made of without a remainder (16 rows at least, so that a box is whole swizzle
+// patterns), and scores that grow with the dot product.  Strides of one-element dims may be anything: they are
+// not taken.
+bool attn_tc_takes(const AttnParams& p) {
+  const int bn = p.D == 256 ? 64 : 128;
+  if (p.page_size < 16 || (p.page_size < bn ? bn % p.page_size != 0 : p.page_size % bn != 0)) return false;
+  const int64_t strides[6] = {p.k_sh, p.k_st, p.k_sp, p.v_sh, p.v_st, p.v_sp};
+  for (int64_t s : strides)
+    if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
+  return p.scale > 0.f && p.pages > 0;
+}
+
+cudaError_t launch_attn_tc(const AttnParams& p, int lo, cudaStream_t stream) {
+  const AtRows of{lo, INT32_MAX};
+  if (p.D == 64) return run_tc<64>(p, of, stream);
+  if (p.D == 128) return run_tc<128>(p, of, stream);
+  return run_tc<256>(p, of, stream);
+}
+
+}  // namespace gdnr
