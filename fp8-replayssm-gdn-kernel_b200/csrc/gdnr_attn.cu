@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
     return;
   }
   Unit u = find_unit<T>(p, of, share.begin, lane);
-  if (tid == 0) write_meta(meta, share, u);
+  if (tid == 0) write_meta(meta, share, u, total, gridDim.x);
   const float sl2 = p.scale * LOG2E;
   for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
     const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
@@ -68,8 +68,9 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
     for (int i = tid; i < BM * CH; i += C::THREADS) {
       const int r = i / CH, c = i % CH;
       const bool ok = r < rows;
-      const int rr = row_base + (ok ? r : 0), tok = u.s.q0 + rr / p.G, hd = u.h * p.G + rr % p.G;
-      cp_async16_zfill(q_s + swz<ROWB>(r, c), p.q + int64_t(tok) * p.q_st + int64_t(hd) * p.q_sh + c * 8, ok ? 16 : 0);
+      const int rr = row_base + (ok ? r : 0), tk = token_of(p, rr);
+      cp_async16_zfill(q_s + swz<ROWB>(r, c), p.q + int64_t(u.s.q0 + tk) * p.q_st + int64_t(u.h * p.G + rr - tk * p.G) * p.q_sh + c * 8,
+                       ok ? 16 : 0);
     }
     auto load_tile = [&](int t, int stage) {
       const uint32_t ks = kv_s + stage * 2 * C::TILE, vs = ks + C::TILE;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int r = row_base + wm * 16 + (lane >> 2) + 8 * j;
-      lim[j] = r < u.s.m * p.G ? min(u.s.kv - 1, u.s.kv - u.s.m + r / p.G) : -1;
+      lim[j] = r < u.s.m * p.G ? min(u.s.kv - 1, u.s.kv - u.s.m + token_of(p, r)) : -1;
     }
     for (int t = t0; t < t1; ++t) {
       const int i = t - t0;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   const int* mi = metas + i * AT_META;
   const int n = mi[0];
   if (n < 0) return;  // no unit is cut here
-  const int before = mi[3], left = mi[4];
+  const int before = mi[3];
   if (metas[(i - 1) * AT_META + 5] < before) return;  // the unit begins before share i - 1: not its first cut
   const SeqLen s = seq_len(p, n, of);
   const int r = blockIdx.y * ROWS + warp / PER_ROW, rr = mi[2] * BM + r;
@@ -291,18 +292,28 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = 0.f;
   if (live) {
-    // shares are equal but for rounding: find how many take part
-    int parts = 2;
-    for (int have = mi[5], c = i + 1; have < left; ++c, ++parts) have += metas[c * AT_META + 5];
-    for (int c = warp % PER_ROW; c < parts; c += PER_ROW) {
-      const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
-      const float pm = src[D], pl = src[D + 1];
-      const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
-      const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
-      m = nm;
-      l = l * f0 + pl * f1;
+    const int parts = mi[6] - i + 2;  // shares i - 1 .. the one of the unit's last tile
+    constexpr int AHEAD = 4;
+    for (int c0 = warp % PER_ROW; c0 < parts; c0 += PER_ROW * AHEAD) {
+      float y[AHEAD][E], pm[AHEAD], pl[AHEAD];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + src[e * 32 + lane] * f1;
+      for (int a = 0; a < AHEAD; ++a) {
+        const int c = c0 + a * PER_ROW;
+        pm[a] = -INFINITY, pl[a] = 0.f;
+        const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
+        if (c < parts) pm[a] = src[D], pl[a] = src[D + 1];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[a][e] = c < parts ? src[e * 32 + lane] : 0.f;
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const float nm = fmaxf(m, pm[a]), b = nm == -INFINITY ? 0.f : nm;
+        const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm[a] - b);
+        m = nm;
+        l = l * f0 + pl[a] * f1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + y[a][e] * f1;
+      }
     }
   }
   if constexpr (PER_ROW > 1) {
@@ -329,7 +340,8 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   }
   if (!live) return;
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  uint16_t* dst = p.out + int64_t(s.q0 + rr / p.G) * p.o_st + int64_t(mi[1] * p.G + rr % p.G) * p.o_sh;
+  const int tk = token_of(p, rr);
+  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(mi[1] * p.G + rr - tk * p.G) * p.o_sh;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e * 32 + lane] = f_to_bf16(x[e] * inv);
   if (lane == 0) write_lse(p, s, mi[1], rr, m, l);

@@ -40,9 +40,14 @@ __device__ __forceinline__ SeqLen seq_len(const AttnParams& p, int n, const AtRo
   return s;
 }
 
+// row / G: a multiplication where that is exact for every row (the host checks)
+__device__ __forceinline__ int token_of(const AttnParams& p, int row) {
+  return p.g_magic ? int(__umulhi(uint32_t(row), p.g_magic)) : row / p.G;
+}
+
 // Keys that rows up to (not including) `rows` of a sequence see.
 __device__ __forceinline__ int keys_seen(const AttnParams& p, const SeqLen& s, int rows) {
-  return min(s.kv, s.kv - s.m + (min(rows, s.m * p.G) - 1) / p.G + 1);
+  return min(s.kv, s.kv - s.m + token_of(p, min(rows, s.m * p.G) - 1) + 1);
 }
 
 // A unit is (sequence, key head, tile of BM rows); its cost is the number of key tiles
@@ -53,19 +58,32 @@ __device__ __forceinline__ int unit_tiles(const AttnParams& p, const SeqLen& s, 
   return max(1, (keys_seen(p, s, (rt + 1) * T::BM) + T::BN - 1) / T::BN);  // a unit without keys still writes its rows
 }
 
+// A warp looks at 32 / per sequences at a time with `per` lanes each, so that one long sequence does not
+// keep a single lane busy.
+__device__ __forceinline__ int lanes_per_seq(int n) { return n >= 32 ? 1 : (n > 16 ? 1 : (n > 8 ? 2 : (n > 4 ? 4 : (n > 2 ? 8 : (n > 1 ? 16 : 32))))); }
+
+// Key tiles of sequence n (0 past the last), in each of its `per` lanes.
 template <class T>
-__device__ int64_t seq_tiles(const AttnParams& p, const SeqLen& s) {
-  const int rts = (s.m * p.G + T::BM - 1) / T::BM;
+__device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const AtRows& r, int n, int per, int lane) {
   int64_t sum = 0;
-  for (int rt = 0; rt < rts; ++rt) sum += unit_tiles<T>(p, s, rt);
+  if (n < p.N) {
+    const SeqLen s = seq_len(p, n, r);
+    const int rts = (s.m * p.G + T::BM - 1) / T::BM;
+    for (int rt = lane & (per - 1); rt < rts; rt += per) sum += unit_tiles<T>(p, s, rt);
+  }
+  for (int o = per >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum * p.Hk;
 }
 
 // Key tiles of the batch (one whole warp).
 template <class T>
 __device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& r, int lane) {
+  const int per = lanes_per_seq(p.N), step = 32 / per;
   int64_t w = 0;
-  for (int n = lane; n < p.N; n += 32) w += seq_tiles<T>(p, seq_len(p, n, r));
+  for (int n0 = 0; n0 < p.N; n0 += step) {
+    const int64_t x = seq_tiles<T>(p, r, n0 + lane / per, per, lane);
+    if ((lane & (per - 1)) == 0) w += x;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
   return w;
@@ -81,35 +99,46 @@ struct Unit {
 // The unit that key tile `at` of the batch falls into (one whole warp).
 template <class T>
 __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, int64_t at, int lane) {
+  const int per = lanes_per_seq(p.N), step = 32 / per;
   int64_t base = 0;
   Unit u;
   u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
   u.s.q0 = u.s.m = u.s.kv = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 32) {
-    const int n = n0 + lane;
-    int64_t w = 0;
-    if (n < p.N) w = seq_tiles<T>(p, seq_len(p, n, r));
+  for (int n0 = 0; n0 < p.N; n0 += step) {
+    const int64_t w = seq_tiles<T>(p, r, n0 + lane / per, per, lane);
     int64_t pre = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = per; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
       if (lane >= o) pre += v;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, base + pre > at);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
-      u.n = n0 + src;
+      int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
+      u.n = n0 + src / per;
       u.s = seq_len(p, u.n, r);
       const int64_t per_head = __shfl_sync(0xffffffffu, w, src) / p.Hk;
       u.h = int((at - start) / per_head);
-      u.begin = start + u.h * per_head;
-      u.tiles = unit_tiles<T>(p, u.s, 0);
-      while (u.begin + u.tiles <= at) {
-        u.begin += u.tiles;
-        u.tiles = unit_tiles<T>(p, u.s, ++u.rt);
+      start += u.h * per_head;
+      const int rts = (u.s.m * p.G + T::BM - 1) / T::BM;
+      for (int rt0 = 0; rt0 < rts; rt0 += 32) {
+        const int mine = rt0 + lane < rts ? unit_tiles<T>(p, u.s, rt0 + lane) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, start + sum > at);
+        if (in) {
+          const int l = __ffs(in) - 1;
+          u.rt = rt0 + l;
+          u.tiles = __shfl_sync(0xffffffffu, mine, l);
+          u.begin = start + __shfl_sync(0xffffffffu, sum - mine, l);
+          return u;
+        }
+        start += __shfl_sync(0xffffffffu, sum, 31);
       }
-      return u;
     }
     base += __shfl_sync(0xffffffffu, pre, 31);
   }
@@ -155,24 +184,30 @@ __device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
 
 // A CTA's record for the join, in the workspace behind the parts [ctas][2][BM][D + 2]: a share that
 // begins inside a unit leaves its part of it in slot 0, one that only ends inside in slot 1.
-__device__ __forceinline__ void write_meta(int* meta, const Share& share, const Unit& u) {
+__device__ __forceinline__ void write_meta(int* meta, const Share& share, const Unit& u, int64_t total, int ctas) {
   meta[0] = share.begin > u.begin ? u.n : -1;  // the unit this share begins in, if it begins inside it
   meta[1] = u.h;
   meta[2] = u.rt;
   meta[3] = int(share.begin - u.begin);            // tiles of that unit in earlier shares
   meta[4] = int(u.begin + u.tiles - share.begin);  // tiles of it from here on
   meta[5] = int(share.end - share.begin);
+  // the share of the unit's last tile: the last one that begins at or before it
+  const int64_t use = min(int64_t(ctas), (total + 1) / 2), last = u.begin + u.tiles - 1;
+  int64_t c = last * use / total;
+  while (c + 1 < use && total * (c + 1) / use <= last) ++c;
+  meta[6] = int(c);
 }
 
 // Row r of a sequence: token q0 + r / G, query head h G + r % G.
 __device__ __forceinline__ int64_t out_at(const AttnParams& p, const Unit& u, int row) {
-  return int64_t(u.s.q0 + row / p.G) * p.o_st + int64_t(u.h * p.G + row % p.G) * p.o_sh;
+  const int t = token_of(p, row);
+  return int64_t(u.s.q0 + t) * p.o_st + int64_t(u.h * p.G + row - t * p.G) * p.o_sh;
 }
 
 __device__ __forceinline__ void write_lse(const AttnParams& p, const SeqLen& s, int h, int row, float max2, float sum) {
-  if (p.lse)
-    p.lse[int64_t(s.q0 + row / p.G) * p.l_st + int64_t(h * p.G + row % p.G) * p.l_sh] =
-        sum > 0.f ? (max2 + log2f(sum)) * LN2 : -INFINITY;
+  if (!p.lse) return;
+  const int t = token_of(p, row);
+  p.lse[int64_t(s.q0 + t) * p.l_st + int64_t(h * p.G + row - t * p.G) * p.l_sh] = sum > 0.f ? (max2 + log2f(sum)) * LN2 : -INFINITY;
 }
 
 // Joins the parts of the units of BM rows that were cut between `ctas` shares (gdnr_attn.cu).

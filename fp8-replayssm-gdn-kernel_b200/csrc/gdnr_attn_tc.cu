@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   u.n = p.N;
   if (share.begin < share.end) {
     u = find_unit<T>(p, of, share.begin, lane);
-    if (tid == 0) write_meta(meta, share, u);
+    if (tid == 0) write_meta(meta, share, u, bars.total, gridDim.x);
   } else if (tid == 0) {
     meta[0] = -1;
   }
@@ -368,20 +368,30 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       const int end = min(t1, seen(q));
       const int row = u.rt * BM + q * 128 + r;  // row of the sequence
       const bool live = row < u.s.m * p.G;
-      const int lim = live ? min(u.s.kv - 1, u.s.kv - u.s.m + row / p.G) : -1;  // last key the row sees
+      const int lim = live ? min(u.s.kv - 1, u.s.kv - u.s.m + token_of(p, row)) : -1;  // last key the row sees
       if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
       float mx = -INFINITY, sum = 0.f;
       if (end > t0) {
-        // 16 lanes (D = 128) copy a row; rows past the sequence's are zeros
+        // D / 8 lanes copy a row, eight loads in flight; rows past the sequence's are zeros
         constexpr int CH = D / 8;
-        for (int i = lane; i < 32 * CH; i += 32) {
-          const int rr = (warp & 3) * 32 + i / CH, c = i % CH, srow = u.rt * BM + q * 128 + rr;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (srow < u.s.m * p.G)
-            x = *reinterpret_cast<const uint4*>(p.q + int64_t(u.s.q0 + srow / p.G) * p.q_st + int64_t(u.h * p.G + srow % p.G) * p.q_sh + c * 8);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (c >> 3) * 16384 + swz<128>(rr, c & 7)), "r"(x.x), "r"(x.y),
-                       "r"(x.z), "r"(x.w)
-                       : "memory");
+#pragma unroll 1
+        for (int i0 = lane; i0 < 32 * CH; i0 += 256) {
+          uint4 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * 32, rr = (warp & 3) * 32 + i / CH, srow = u.rt * BM + q * 128 + rr, tk = token_of(p, srow);
+            x[j] = make_uint4(0, 0, 0, 0);
+            if (srow < u.s.m * p.G)
+              x[j] = *reinterpret_cast<const uint4*>(p.q + int64_t(u.s.q0 + tk) * p.q_st + int64_t(u.h * p.G + srow - tk * p.G) * p.q_sh +
+                                                     i % CH * 8);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * 32, rr = (warp & 3) * 32 + i / CH, c = i % CH;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (c >> 3) * 16384 + swz<128>(rr, c & 7)), "r"(x[j].x),
+                         "r"(x[j].y), "r"(x[j].z), "r"(x[j].w)
+                         : "memory");
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();

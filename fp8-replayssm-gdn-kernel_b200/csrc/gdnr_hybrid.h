@@ -108,6 +108,7 @@ struct AttnParams {
   int64_t l_st, l_sh;
   float scale;
   int32_t N, T, Hq, Hk, G, D, pages, page_size, page_shift, width, max_q;
+  uint32_t g_magic;  // row / G = high half of row * g_magic; 0: divide
   float* ws;
   int64_t ws_bytes;
   uint32_t* err;

@@ -299,6 +299,8 @@ int gdnr_paged_attention(const gdnr_attn_args* x, void* stream) {
   p.page_shift = -1;
   for (int s = 0; s < 30; ++s)
     if (ps == (int64_t(1) << s)) p.page_shift = s;
+  // row * (G magic - 2^32) has to stay below 2^32 for rows up to T * G
+  if (p.G > 1 && T * p.G * p.G < (int64_t(1) << 32)) p.g_magic = uint32_t(((int64_t(1) << 32) + p.G - 1) / p.G);
   p.max_q = x->max_seqlen > 0 ? x->max_seqlen : int(T);
   p.err = x->error_flag ? x->error_flag : default_error_word();
   if (!p.err) return set_error(GDNR_ERR_CUDA, "no device error word available");
