@@ -347,6 +347,47 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   if (lane == 0) write_lse(p, s, mi[1], rr, m, l);
 }
 
+// The same for parts that lie in columns of BM rows (the tcgen05 kernel's: its threads have a row each).  Block
+// (i - 1, y) has 32 rows, a lane each; its warps share the D columns.
+template <int D, int BM>
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const __grid_constant__ AttnParams p, const AtRows of, int ctas) {
+  constexpr int COLS = D / AJ_WARPS;
+  const int i = blockIdx.x + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int* metas = reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2));
+  const int* mi = metas + i * AT_META;
+  const int n = mi[0];
+  if (n < 0 || metas[(i - 1) * AT_META + 5] < mi[3]) return;  // no unit is cut here, or not for the first time
+  const SeqLen s = seq_len(p, n, of);
+  const int r = blockIdx.y * 32 + lane, rr = mi[2] * BM + r;
+  if (rr >= s.m * p.G) return;
+  float m = -INFINITY, l = 0.f, x[COLS];
+#pragma unroll
+  for (int e = 0; e < COLS; ++e) x[e] = 0.f;
+  const int parts = mi[6] - i + 2;
+  for (int c = 0; c < parts; ++c) {
+    const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
+    const float pm = src[D * BM], pl = src[(D + 1) * BM];
+    float y[COLS];
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) y[e] = src[(warp * COLS + e) * BM];
+    const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
+    const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
+    m = nm;
+    l = l * f0 + pl * f1;
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) x[e] = x[e] * f0 + y[e] * f1;
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const int tk = token_of(p, rr);
+  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(mi[1] * p.G + rr - tk * p.G) * p.o_sh + warp * COLS;
+#pragma unroll
+  for (int e = 0; e < COLS; e += 8)
+    *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16x2(x[e] * inv, x[e + 1] * inv), pack_bf16x2(x[e + 2] * inv, x[e + 3] * inv),
+                                                    pack_bf16x2(x[e + 4] * inv, x[e + 5] * inv), pack_bf16x2(x[e + 6] * inv, x[e + 7] * inv));
+  if (warp == 0) write_lse(p, s, mi[1], rr, m, l);
+}
+
 template <int D, int BM, int ROWS>
 void join(const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
   // rows a unit can have, by the longest sequence the host knows of
@@ -361,7 +402,7 @@ void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream
   else if (bm == 64)
     join<D, 64, 2>(p, ctas, of, stream);
   else
-    join<D, D == 256 ? 128 : 256, 8>(p, ctas, of, stream);
+    attn_join_columns_kernel<D, D == 256 ? 128 : 256><<<dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), AJ_WARPS * 32, 0, stream>>>(p, of, ctas);
 }
 
 template <int D, int WM, int WN, int STAGES, int PER_SM>

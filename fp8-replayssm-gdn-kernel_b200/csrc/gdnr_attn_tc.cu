@@ -3,7 +3,7 @@
 // A CTA walks its share of the batch's (row tile, key tile) pairs.  NQ streams of 128 rows (one
 // where D = 256, whose accumulator takes half of tensor memory) share the keys and
 // values, which TMA brings page by page into a ring of tiles:
-//   load warp      keys and values of tile 0, 1, ...
+//   load warp      query rows of each unit, keys and values of tile 0, 1, ...
 //   matrix warp    S = Q K^T into tensor memory; O += P V with P from tensor memory
 //   softmax warps  four a stream, a thread a row: S -> registers, maximum, exponentials, their sum,
 //                  P as bf16 over S
@@ -28,7 +28,11 @@ struct TcCfg {
   static constexpr int KV_BYTES = BN * D * 2;           // a tile of keys or of values
   static constexpr int RING = D == 256 ? 5 : (D == 128 ? 5 : 8);
   static constexpr int SOFTMAX_WARPS = 4 * NQ;
-  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
+  // two streams: whole groups of four warps, and registers are handed from the last one (two of its warps have no
+  // role) to the softmax warps, whose rows of S live in them: 256 x 200 + 128 x 104 <= 384 x 168, what the block is
+  // launched with
+  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + (NQ == 2 ? 4 : 2));
+  static constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 104;
   static constexpr int SMEM = NQ * Q_BYTES + RING * KV_BYTES + 1024;
   // tensor memory columns: two buffers of S (P lies over the first half of its S), then O
   static constexpr int S_COLS = BN, O_COL = 256;
@@ -88,11 +92,18 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, float* r) {
       : "memory");
 }
 
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tc_ld16(uint32_t addr, float* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::TC_W8(0),
-      TC_W8(8), TC_W8(16), TC_W8(24), "r"(addr)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : TC_R8(0), TC_R8(8)
+      : "r"(addr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TC_W8(0),
+      TC_W8(8), "r"(addr)
       : "memory");
 }
 
@@ -106,13 +117,53 @@ __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
+__device__ __forceinline__ void tc_tma3(uint32_t dst, const CUtensorMap* map, int c, int h, int token, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(c), "r"(h), "r"(token), "r"(smem_addr(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void tc_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// Two floats in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+template <bool DO, int REGS>
+__device__ __forceinline__ void tc_regs_dec() {
+  if constexpr (DO) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
 struct TcBars {
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t q_full[2];   // softmax warps -> matrix warp: the stream's query rows are in shared memory
+  uint64_t q_full[2];   // the stream's query rows are in shared memory
+  uint64_t q_free[2];   // matrix warp -> load warp: the stream's last Q K^T of a unit is complete
   uint64_t s_full[2];   // matrix warp -> softmax warps: S of the buffer is complete
   uint64_t p_full[2];   // softmax warps -> matrix warp: P of the buffer is written (and O rescaled)
   uint64_t o_full;      // one stream: PV of a key tile is complete (what O must wait for before it is rescaled)
@@ -131,7 +182,7 @@ struct TcWait {
     if (!ok) ok = slow(bar, parity);
     return __all_sync(0xffffffffu, ok);
   }
-  __device__ __noinline__ bool slow(uint64_t* bar, uint32_t parity) const {
+  __device__ __forceinline__ bool slow(uint64_t* bar, uint32_t parity) const {
     const uint32_t a = smem_addr(bar);
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1; it < WAIT_LIMIT_ITERS; ++it) {
@@ -150,7 +201,7 @@ struct TcWait {
 template <int D>
 __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                   const AtRows of) {
+                   const __grid_constant__ CUtensorMap qmap, const AtRows of, const int q_tma) {
   using C = TcCfg<D>;
   using T = AtTile<C::BM, C::BN>;
   constexpr int NQ = C::NQ, BN = C::BN, BM = C::BM;
@@ -173,7 +224,8 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       mbar_init(&bars.kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.q_full[i], 4);
+      mbar_init(&bars.q_full[i], q_tma ? 1 : 4);
+      mbar_init(&bars.q_free[i], 1);
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.done[i], 1);
@@ -206,7 +258,8 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
 
   if (warp == C::SOFTMAX_WARPS + 1) {
     // ------------------------------------------------------------ load warp
-    uint32_t slot = 0;  // tiles requested so far
+    tc_regs_dec<C::NQ == 2, C::OTHER_REGS>();
+    uint32_t slot = 0, nq[2] = {0, 0};  // tiles and query tiles requested so far
     bool ok = true;
     constexpr int PER_SLOT = BN;
     const int box = min(p.page_size, BN), boxes = PER_SLOT / box * C::ATOMS;
@@ -217,6 +270,17 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       if (NQ > 1) most = max(most, seen(1));
       t1 = min(t1, most);
       const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
+      for (int q = 0; q_tma && q < NQ && ok; ++q) {
+        if (min(t1, seen(q)) <= t0) continue;
+        if (nq[q]) ok = wait(&bars.q_free[q], (nq[q] - 1) & 1);
+        if (!ok) break;
+        ++nq[q];
+        if (lane == 0) mbar_arrive_expect_tx(&bars.q_full[q], C::Q_BYTES);
+        __syncwarp();
+        // rows past the sequence's end are another's: their results are not written
+        if (lane < C::ATOMS)
+          tc_tma3(base + q * C::Q_BYTES + lane * 16384, &qmap, lane * 64, u.h * p.G, u.s.q0 + token_of(p, u.rt * BM + q * 128), &bars.q_full[q]);
+      }
       for (int t = t0; ok && t < t1; ++t) {
         // where this lane's boxes come from: a page past the sequence's end, or outside the cache, reads as zeros
         const int atom = lane % C::ATOMS, part = lane / C::ATOMS, tok = t * BN + part * box;
@@ -242,25 +306,33 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         }
       }
     }
-    if (!ok)  // copies in flight end before the CTA does
+    if (!ok) {  // copies in flight end before the CTA does
+      for (int q = 0; q < NQ; ++q) {
+        const uint64_t t = globaltimer_ns();
+        while (nq[q] && !mbar_try_wait(smem_addr(&bars.q_full[q]), (nq[q] - 1) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
+        }
+      }
       for (uint32_t k = slot > C::RING ? slot - C::RING : 0; k < slot; ++k) {
         const uint64_t t = globaltimer_ns();
         while (!mbar_try_wait(smem_addr(&bars.kv_full[k % C::RING]), (k / C::RING) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
         }
       }
+    }
   } else if (warp == C::SOFTMAX_WARPS) {
     // ------------------------------------------------------------ matrix warp
+    tc_regs_dec<C::NQ == 2, C::OTHER_REGS>();
     uint32_t slot = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // tiles consumed; phases of q_full, p_full
     constexpr uint32_t QK = tc_idesc(BN, false), PV = tc_idesc(D, true);
     bool ok = true;
     auto kv_wait = [&](uint32_t k) { return wait(&bars.kv_full[k % C::RING], (k / C::RING) & 1); };
     auto kv_addr = [&](uint32_t k) { return kv_base + (k % C::RING) * C::KV_BYTES; };
-    auto score = [&](int q, int buf, uint32_t k) {  // S[buf] = Q_q K^T
+    auto score = [&](int q, int buf, uint32_t k, bool last) {  // S[buf] = Q_q K^T
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
         tc_mma_ss(tmem + buf * C::S_COLS, tc_desc_k(base + q * C::Q_BYTES + (i >> 2) * 16384 + (i & 3) * 32),
                   tc_desc_k(kv_addr(k) + (i >> 2) * (BN * 128) + (i & 3) * 32), QK, i > 0);
       tc_commit(&bars.s_full[buf]);
+      if (last) tc_commit(&bars.q_free[q]);
     };
     auto weigh = [&](int q, int buf, uint32_t k, bool first, bool last) {  // O_q += P[buf] V
 #pragma unroll
@@ -299,7 +371,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         if (ok) ok = kv_wait(k0);
         if (ok && lane == 0)
           for (int q = 0; q < 2; ++q)
-            if (end[q] > t0) score(q, q, k0);
+            if (end[q] > t0) score(q, q, k0, t0 + 1 == end[q]);
         free_slot(k0);
         for (int t = t0; t < last && ok; ++t) {
           const uint32_t kk = k0 + 2 * (t + 1 - t0), kv = k0 + 2 * (t - t0) + 1;
@@ -316,7 +388,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
             if (t + 1 < end[q]) {
               if (!have_k) ok = kv_wait(kk), have_k = true;
               if (!ok) break;
-              if (lane == 0) score(q, q, kk);
+              if (lane == 0) score(q, q, kk, t + 2 == end[q]);
             }
             __syncwarp();
           }
@@ -326,14 +398,14 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       } else {
         // S(t + 1) is issued before P(t) V(t), into the other buffer
         if (ok) ok = kv_wait(k0);
-        if (ok && lane == 0) score(0, t0 & 1, k0);
+        if (ok && lane == 0) score(0, t0 & 1, k0, t0 + 1 == last);
         free_slot(k0);
         for (int t = t0; t < last && ok; ++t) {
           const uint32_t kk = k0 + 2 * (t + 1 - t0), kv = k0 + 2 * (t - t0) + 1;
           if (t + 1 < last) {
             ok = kv_wait(kk);
             if (!ok) break;
-            if (lane == 0) score(0, (t + 1) & 1, kk);
+            if (lane == 0) score(0, (t + 1) & 1, kk, t + 2 == last);
             __syncwarp();
           }
           ok = kv_wait(kv);
@@ -355,8 +427,9 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       while (globaltimer_ns() - t < 1000000) {
       }
     }
-  } else {
+  } else if (warp < C::SOFTMAX_WARPS) {
     // ------------------------------------------------------------ softmax warps
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
     const int q = NQ > 1 ? warp >> 2 : 0, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // the warp's tensor memory lanes (bits 16..)
     const uint32_t q_smem = base + q * C::Q_BYTES, o_mem = tmem + lanes + C::O_COL + q * D;
@@ -371,7 +444,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       const int lim = live ? min(u.s.kv - 1, u.s.kv - u.s.m + token_of(p, row)) : -1;  // last key the row sees
       if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
       float mx = -INFINITY, sum = 0.f;
-      if (end > t0) {
+      if (end > t0 && !q_tma) {
         // D / 8 lanes copy a row, eight loads in flight; rows past the sequence's are zeros
         constexpr int CH = D / 8;
 #pragma unroll 1
@@ -415,7 +488,11 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < BN; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+        for (int i = 4; i + 8 <= BN; i += 8)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[BN - 4 + j]);
         const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
         if (t == t0) {
           mx = tm;
@@ -431,33 +508,35 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
           if (grow) mx = tm;
           sum *= f;
 #pragma unroll 1
-          for (int i = 0; i < D; i += 32) {
-            float o[32];
-            tc_ld32(o_mem + i, o);
+          for (int i = 0; i < D; i += 16) {
+            float o[16];
+            tc_ld16(o_mem + i, o);
             tc_wait_ld();
-            uint32_t w[32];
+            uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * f);
-            tc_st32(o_mem + i, w);
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * f);
+            tc_st16(o_mem + i, w);
           }
         }
         const float b = mx == -INFINITY ? 0.f : mx;  // a row that has seen no key yet
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t part[2] = {0, 0};  // pairs of sums
+        const uint64_t sl2_2 = pack2(sl2, sl2), nb2 = pack2(-b, -b);
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) {
-          uint32_t w[32];
+        for (int i = 0; i < BN / 32; ++i) {
+          uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = ex2_approx(fmaf(s[i * 64 + 2 * j], sl2, -b)), y = ex2_approx(fmaf(s[i * 64 + 2 * j + 1], sl2, -b));
-            part[(2 * j) & 3] += x;
-            part[(2 * j + 1) & 3] += y;
+          for (int j = 0; j < 16; ++j) {
+            const float2 e = unpack2(fma2(pack2(s[i * 32 + 2 * j], s[i * 32 + 2 * j + 1]), sl2_2, nb2));
+            const float x = ex2_approx(e.x), y = ex2_approx(e.y);
+            part[j & 1] = add2(part[j & 1], pack2(x, y));
             // weights are rounded to bf16 for the tensor cores; their sum is taken before that
             w[j] = cvt_bf16x2(x, y);
           }
-          tc_st32(s_mem + i * 32, w);
+          tc_st16(s_mem + i * 16, w);
         }
         tc_wait_st();
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        const float2 add = unpack2(add2(part[0], part[1]));
+        sum += add.x + add.y;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) tc_arrive(&bars.p_full[buf]);
@@ -473,7 +552,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       const bool whole = t0 == 0 && t1 == u.tiles;
       const float inv = sum > 0.f ? 1.0f / sum : 0.f;
       uint16_t* dst = live ? p.out + out_at(p, u, row) : nullptr;
-      float* part = ws_o + ((t0 > 0 ? 0 : 1) * BM + q * 128 + r) * (D + 2);
+      float* part = ws_o + (t0 > 0 ? 0 : 1) * BM * (D + 2) + q * 128 + r;  // columns of BM rows
 #pragma unroll 1
       for (int i = 0; i < D; i += 32) {
         float o[32];
@@ -492,7 +571,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
                            cvt_bf16x2(o[8 * j + 4] * inv, o[8 * j + 5] * inv), cvt_bf16x2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
         } else if (live) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) *reinterpret_cast<float2*>(part + i + j * 2) = make_float2(o[2 * j], o[2 * j + 1]);
+          for (int j = 0; j < 32; ++j) part[(i + j) * BM] = o[j];
         }
         __syncwarp();
       }
@@ -500,11 +579,13 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         if (whole)
           write_lse(p, u.s, u.h, row, mx, sum);
         else
-          part[D] = mx, part[D + 1] = sum;
+          part[D * BM] = mx, part[(D + 1) * BM] = sum;
       }
       tc_fence_before();  // O has been read before the next unit's first P is announced
       __syncwarp();
     }
+  } else {
+    tc_regs_dec<C::NQ == 2, C::OTHER_REGS>();
   }
   tc_fence_before();
   __syncthreads();
@@ -530,7 +611,17 @@ cudaError_t run_tc(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
   cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
   if (e != cudaSuccess) return e;
   const int ctas = multiprocessor_count();
-  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], of);
+  // query rows by TMA where a tile is whole tokens: boxes of 64 elements x G heads x 128 / G tokens
+  CUtensorMap qmap = maps[0];
+  const int q_tma = 128 % p.G == 0 && p.q_st > 0 && p.q_sh > 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
+  if (q_tma) {
+    const uint64_t dims[3] = {uint64_t(D), uint64_t(p.Hq), uint64_t(p.T)};
+    const uint64_t strides[2] = {uint64_t(p.q_sh) * 2, uint64_t(p.q_st) * 2};
+    const uint32_t box[3] = {64, uint32_t(p.G), uint32_t(128 / p.G)};
+    e = encode_bf16_map(&qmap, p.q, 3, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], qmap, of, q_tma);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_attn_join(p, ctas, C::BM, of, stream);
