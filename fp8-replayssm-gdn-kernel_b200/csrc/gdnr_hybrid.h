@@ -85,7 +85,7 @@ struct AppendParams {
   int64_t qo_st, qo_sh;
   uint16_t *kc, *vc;  // [pages, page_size, Hk, D]
   int64_t kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh;
-  int32_t T, Hq, Hk, D, rot, P, pages, page_size, inter;
+  int32_t T, Hq, Hk, D, rot, P, pages, page_size, page_shift, inter, tb_vec;
   float eps, w_off;
   uint32_t* err;
 };

@@ -90,6 +90,13 @@ bool touches(const gdnr_tensor& a, const gdnr_tensor& b) {
   return overlaps(a, b);
 }
 
+// log2 of a power of two, -1 of anything else
+int shift_of(int64_t x) {
+  for (int s = 0; s < 31; ++s)
+    if (x == (int64_t(1) << s)) return s;
+  return -1;
+}
+
 // cu_seqlens [N+1]; N out
 int check_seqlens(const gdnr_tensor& t, int64_t* n) {
   CHECK(check_tensor(t, "cu_seqlens", 1, HY_I32, 1, nullptr));
@@ -202,11 +209,13 @@ int gdnr_qk_norm_rope_append(const gdnr_append_args* x, void* stream) {
   if (present(x->q_weight)) {
     CHECK(check_tensor(x->q_weight, "q_weight", 1, HY_WEIGHT, 2, want_d));
     CHECK(check_inner_contiguous(x->q_weight, "q_weight"));
+    CHECK(check_aligned16(x->q_weight, "q_weight", 0));
     p.qw = x->q_weight.data, p.qw_dt = x->q_weight.dtype;
   }
   if (present(x->k_weight)) {
     CHECK(check_tensor(x->k_weight, "k_weight", 1, HY_WEIGHT, 2, want_d));
     CHECK(check_inner_contiguous(x->k_weight, "k_weight"));
+    CHECK(check_aligned16(x->k_weight, "k_weight", 0));
     p.kw = x->k_weight.data, p.kw_dt = x->k_weight.dtype;
   }
   CHECK(check_tensor(x->positions, "positions", 1, HY_I32, 1, want_t));
@@ -241,11 +250,13 @@ int gdnr_qk_norm_rope_append(const gdnr_append_args* x, void* stream) {
   p.vc_sp = x->v_cache.stride[0], p.vc_st = x->v_cache.stride[1], p.vc_sh = x->v_cache.stride[2];
   p.T = int(T), p.Hq = int(Hq), p.Hk = int(Hk), p.D = int(D), p.rot = int(rot), p.P = int(x->cos_sin.shape[0]);
   p.pages = int(pages), p.page_size = int(ps), p.inter = x->interleaved;
+  p.page_shift = shift_of(ps);
+  p.tb_vec = reinterpret_cast<uintptr_t>(p.table) % 16 == 0 && p.tb_s % 4 == 0 && (rot / 2) % 8 == 0;
   p.eps = x->eps, p.w_off = x->weight_offset;
   p.err = x->error_flag ? x->error_flag : default_error_word();
   if (!p.err) return set_error(GDNR_ERR_CUDA, "no device error word available");
   if (T == 0 || Hq + Hk == 0) return GDNR_OK;
-  if (T * (Hq + 2 * Hk) > (int64_t(1) << 33)) return set_error(GDNR_ERR_UNSUPPORTED, "T * heads above 2^33");
+  if (T * (Hq + 2 * Hk) > (int64_t(1) << 31)) return set_error(GDNR_ERR_UNSUPPORTED, "T * heads above 2^31");
   return cuda_status(launch_append(p, static_cast<cudaStream_t>(stream)), "gdnr_qk_norm_rope_append launch");
 }
 
@@ -296,9 +307,7 @@ int gdnr_paged_attention(const gdnr_attn_args* x, void* stream) {
   p.scale = x->scale;
   p.N = int(n), p.T = int(T), p.Hq = int(Hq), p.Hk = int(Hk), p.G = int(Hq / Hk), p.D = int(D);
   p.pages = int(pages), p.page_size = int(ps), p.width = int(x->block_table.shape[1]);
-  p.page_shift = -1;
-  for (int s = 0; s < 30; ++s)
-    if (ps == (int64_t(1) << s)) p.page_shift = s;
+  p.page_shift = shift_of(ps);
   // row * (G magic - 2^32) has to stay below 2^32 for rows up to T * G
   if (p.G > 1 && T * p.G * p.G < (int64_t(1) << 32)) p.g_magic = uint32_t(((int64_t(1) << 32) + p.G - 1) / p.G);
   p.max_q = x->max_seqlen > 0 ? x->max_seqlen : int(T);

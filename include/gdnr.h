@@ -294,7 +294,7 @@ int64_t gdnr_gdn_prefill_workspace(int64_t tokens, int64_t sequences, int32_t va
 typedef struct {
   gdnr_tensor q;         /* [T,Hq,D] BF16 (rows 16-byte aligned, as all below) */
   gdnr_tensor k, v;      /* [T,Hk,D] BF16 */
-  gdnr_tensor q_weight, k_weight; /* optional [D] BF16|F32, contiguous */
+  gdnr_tensor q_weight, k_weight; /* optional [D] BF16|F32, contiguous, 16-byte aligned */
   gdnr_tensor positions; /* [T] I32 */
   gdnr_tensor slots;     /* [T] I32, distinct where >= 0 */
   gdnr_tensor cos_sin;   /* [P, rot] F32 */
