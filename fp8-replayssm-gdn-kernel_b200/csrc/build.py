@@ -1,4 +1,4 @@
-"""Build libgdnr.so (all CUDA sources of this directory) for sm_100a.
+"""Build libgdnr.so (all CUDA sources of this directory) for sm_100a, and the host call path (_host).
 
     python fp8-replayssm-gdn-kernel_b200/csrc/build.py [--verbose-ptxas] [--force]
 
@@ -16,12 +16,15 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = pathlib.Path(__file__).resolve().parent
 PKG = HERE.parent / "gdnr"
 INCLUDE = HERE.parent.parent / "include"
 BUILD = HERE / "_build"
 TARGET = PKG / "libgdnr.so"
+HOST_SOURCE = HERE / "gdnr_host.cpp"
+HOST_TARGET = PKG / "_host.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2", "--expt-relaxed-constexpr"]
@@ -51,11 +54,30 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> pathlib.Path:
             cmd += ["-Xptxas", "-v"]
         print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_host(force)
     if force or not TARGET.exists() or any(o.stat().st_mtime > TARGET.stat().st_mtime for o in objects):
         cmd = [nvcc(), *ARCH, "-shared", "-o", str(TARGET), *map(str, objects), "-lcuda"]
         print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
     return TARGET
+
+
+def build_host(force: bool = False) -> pathlib.Path:
+    """gdnr/_host.so: the CPython module over torch's C++ tensors (g++, no device code)."""
+    newest = max(HOST_SOURCE.stat().st_mtime, (INCLUDE / "gdnr.h").stat().st_mtime)
+    if not force and HOST_TARGET.exists() and HOST_TARGET.stat().st_mtime >= newest:
+        return HOST_TARGET
+    import torch
+
+    root = pathlib.Path(torch.__file__).resolve().parent
+    cuda = pathlib.Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", str(cuda / "include"), str(HOST_SOURCE), "-o", str(HOST_TARGET),
+           "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return HOST_TARGET
 
 
 def main() -> None:

@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
-import struct
 import threading
 
 import torch
@@ -248,47 +247,37 @@ def tensor_desc(t: torch.Tensor | None, require_cuda: bool = True) -> Tensor:
     return d
 
 
-_TENSOR_PACK = struct.Struct("@Pii8q")  # gdnr_tensor
-_ABSENT = bytes(_TENSOR_PACK.size)
-_ZEROS = tuple((0,) * (4 - n) for n in range(5))
+_addresses: dict[str, int] = {}
 
 
-def pack_tensors(device_index: int, tensors) -> list[bytes]:
-    """The gdnr_tensor bytes of each tensor (None -> absent argument); all have to be on the one GPU.
+def call_tensors(name: str, tensors: tuple, tail: bytes) -> None:
+    """Entry point ``name`` on the current stream of the tensors' device, with that device current.
 
-    The same fields as :func:`tensor_desc`, packed at once: filling a ctypes structure
-    field by field takes several microseconds a tensor, which is what a call on a few tokens
-    is made of."""
-    packed = []
-    for t in tensors:
-        if t is None:
-            packed.append(_ABSENT)
-            continue
-        if t.get_device() != device_index or device_index < 0:
-            if not t.is_cuda:
-                raise ValueError(f"libgdnr operates on CUDA tensors; got a tensor on {t.device}")
-            raise ValueError(f"tensors of one call have to be on one device; got {t.device} and cuda:{device_index}")
-        dt = _TORCH_DT.get(t.dtype)
-        if dt is None:
-            raise ValueError(f"dtype {t.dtype} is not supported by libgdnr")
-        shape = t.shape
-        n = len(shape)
-        if n > 4:
-            raise ValueError("libgdnr tensors have at most 4 dimensions")
-        packed.append(_TENSOR_PACK.pack(t.data_ptr() or 16, dt, n, *shape, *_ZEROS[n], *t.stride(), *_ZEROS[n]))
-    return packed
-
-
-def call_packed(name: str, args: bytes, device_index: int) -> None:
-    """As :func:`call`, with the argument structure as bytes."""
-    fn = getattr(load(), name)
-    if device_index == torch.cuda.current_device():
-        rc = fn(args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device_index):
-            rc = fn(args, torch.cuda.current_stream().cuda_stream)
+    ``tensors`` (None: absent) and ``tail`` are the fields of its argument structure: the
+    gdnr_tensor views are filled by the compiled call path (csrc/gdnr_host.cpp), which refuses tensors
+    that are not on one CUDA device."""
+    address = _addresses.get(name)
+    if address is None:
+        address = _addresses[name] = ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+    rc = _host().call(address, tensors, tail)
     if rc != OK:
         check(rc)
+
+
+_host_module = None
+
+
+def _host():
+    global _host_module
+    if _host_module is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RuntimeError(
+                "gdnr/_host.so is missing or does not fit this torch: build it with "
+                f"`python fp8-replayssm-gdn-kernel_b200/csrc/build.py` ({e})") from e
+        _host_module = module
+    return _host_module
 
 
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:

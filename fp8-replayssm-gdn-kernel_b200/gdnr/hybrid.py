@@ -63,15 +63,11 @@ def gdn_prefill(
     The state can be handed to the decode step with :meth:`gdnr.ReplayState.load_state`.
     """
     if out is None:
-        out = torch.empty(mixed_qkv.shape[0], state.shape[1], state.shape[2], dtype=torch.bfloat16,
-                          device=mixed_qkv.device)
-    dev = mixed_qkv.get_device()
-    packed = _lib.pack_tensors(dev, (mixed_qkv, a, b, A_log, dt_bias, state, cu_seqlens, state_indices,
-                                     has_initial_state, out))
+        out = mixed_qkv.new_empty((mixed_qkv.shape[0], state.shape[1], state.shape[2]), dtype=torch.bfloat16)
     nbytes = _lib.load().gdnr_gdn_prefill_workspace(mixed_qkv.shape[0], cu_seqlens.shape[0] - 1, state.shape[1], max_seqlen)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=mixed_qkv.device) if nbytes > 0 else None
-    packed.append(_PREFILL_TAIL.pack(max_seqlen, 0, workspace.data_ptr() if nbytes > 0 else 0, nbytes, _err(error_flag)))
-    _lib.call_packed("gdnr_gdn_prefill", b"".join(packed), dev)
+    workspace = mixed_qkv.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _lib.call_tensors("gdnr_gdn_prefill", (mixed_qkv, a, b, A_log, dt_bias, state, cu_seqlens, state_indices, has_initial_state, out),
+                      _PREFILL_TAIL.pack(max_seqlen, 0, workspace.data_ptr() if nbytes > 0 else 0, nbytes, _err(error_flag)))
     return out
 
 
@@ -103,11 +99,9 @@ def qk_norm_rope_append(
     [pages,page_size,Hk,D]; a negative slot is padding.  ``q_out`` may be ``q`` itself.
     """
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dev = q.get_device()
-    packed = _lib.pack_tensors(dev, (q, k, v, q_weight, k_weight, positions, slots, cos_sin, q_out, k_cache, v_cache))
-    packed.append(_APPEND_TAIL.pack(eps, weight_offset, 1 if interleaved else 0, 0, _err(error_flag)))
-    _lib.call_packed("gdnr_qk_norm_rope_append", b"".join(packed), dev)
+        q_out = q.new_empty(q.shape)
+    _lib.call_tensors("gdnr_qk_norm_rope_append", (q, k, v, q_weight, k_weight, positions, slots, cos_sin, q_out, k_cache, v_cache),
+                      _APPEND_TAIL.pack(eps, weight_offset, 1 if interleaved else 0, 0, _err(error_flag)))
     return q_out
 
 
@@ -136,15 +130,13 @@ def paged_attention(
     """
     head_dim = q.shape[-1]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    dev = q.get_device()
-    packed = _lib.pack_tensors(dev, (q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, out, lse))
-    nbytes = _workspace_bytes(dev, head_dim)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    packed.append(_ATTN_TAIL.pack(head_dim ** -0.5 if scale is None else scale, max_seqlen, workspace.data_ptr(), nbytes,
-                                  _err(error_flag)))
-    _lib.call_packed("gdnr_paged_attention", b"".join(packed), dev)
+        out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    nbytes = _workspace_bytes(q.get_device(), head_dim)
+    workspace = q.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call_tensors("gdnr_paged_attention", (q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, out, lse),
+                      _ATTN_TAIL.pack(head_dim ** -0.5 if scale is None else scale, max_seqlen, workspace.data_ptr(), nbytes,
+                                      _err(error_flag)))
     return (out, lse) if return_lse else out
 
 

@@ -184,10 +184,9 @@ def test_structs_match_c(tmp_path):
 
 
 def test_packed_bytes_are_the_structure():
-    """The packed form of the calls against the ctypes structures, for the tails."""
+    """The tails that the calls pack against the ctypes structures."""
     from gdnr import hybrid
 
     for cls, tail, tensors in ((_lib.PrefillArgs, hybrid._PREFILL_TAIL, 10), (_lib.AppendArgs, hybrid._APPEND_TAIL, 11),
                                (_lib.AttnArgs, hybrid._ATTN_TAIL, 8)):
         assert ctypes.sizeof(cls) == tensors * ctypes.sizeof(_lib.Tensor) + tail.size
-    assert _lib._TENSOR_PACK.size == ctypes.sizeof(_lib.Tensor)
