@@ -264,6 +264,308 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
   }
 }
 
+// ---------------------------------------------------------------- kernel, pages by TMA
+// The same tiles and the same split, with the keys and values requested by a warp of its own page by page
+// (attn_kernel's threads spend four fifths of their instructions on copying: 64 sequences of 4 k keys took
+// 135 us).  Needs page sizes that are multiples of 8.
+template <int D, int WM, int WN, int STAGES>
+struct AsCfg {
+  static constexpr int BM = 16 * WM, CONSUMERS = 32 * WM * WN, THREADS = CONSUMERS + 32;
+  static constexpr int ROWB = D * 2, ATOMS = D / 64, TILE = AT_BN * ROWB, Q_BYTES = BM * ROWB;
+  // the first kilobyte: AsShared; the stages begin at the second, a multiple of 1024 bytes (two CTAs of 115,712 bytes
+  // are what a multiprocessor holds: there is no room to align by hand)
+  static constexpr int SMEM = 1024 + STAGES * 2 * TILE + Q_BYTES;
+  static_assert(WN == 1 || WN * 16 * D * 4 <= 2 * TILE, "the join uses the last tile's stage");
+};
+
+struct AsShared {
+  uint64_t full[8], empty[8];
+  int64_t total;
+  int abort;
+  float ml[4][16][2];  // maximum and sum of the rows of each warp's keys
+};
+static_assert(sizeof(AsShared) <= 1024, "the first kilobyte");
+
+template <int D, int WM, int WN, int STAGES>
+__global__ void __launch_bounds__(32 * WM * WN + 32)
+    attn_stream_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const AtRows of) {
+  using C = AsCfg<D, WM, WN, STAGES>;
+  using T = AtTile<C::BM, AT_BN>;
+  constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
+  extern __shared__ __align__(1024) uint8_t raw[];
+  AsShared& sh = *reinterpret_cast<AsShared*>(raw);
+  uint64_t *const full = sh.full, *const empty = sh.empty;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t kv_s = smem_addr(raw) + 1024, q_s = kv_s + STAGES * 2 * C::TILE;
+  if (kv_s & 1023u) {  // the swizzled tiles would not be where the products look for them
+    if (tid == 0) atomicOr(p.err, GDNR_DEVERR_LAYOUT);
+    return;
+  }
+  float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
+  int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
+
+  if (warp == 0) {
+    const int64_t w = all_tiles<T>(p, of, lane);
+    if (lane == 0) sh.total = w;
+  } else if (tid == 32) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], WM * WN);
+    }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int64_t total = sh.total;
+  const Share share = share_of(total, blockIdx.x, gridDim.x);
+  if (share.begin >= share.end) {
+    if (tid == 0) meta[0] = -1;
+    return;
+  }
+  const WarpWait wait{p.err, &sh.abort};
+  Unit u = find_unit<T>(p, of, share.begin, lane);
+  uint32_t k = 0;  // tiles requested or consumed so far
+  bool ok = true;
+
+  if (warp == WM * WN) {
+    for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
+      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
+      for (int t = t0; t < t1; ++t, ++k) {
+        const KvBox b = kv_box<AT_BN, C::ATOMS>(p, u, table, t, lane);
+        const uint32_t s = k % STAGES, to = kv_s + s * 2 * C::TILE;
+        if (k >= STAGES) ok = wait(&empty[s], (k / STAGES - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * C::TILE);
+        __syncwarp();
+        if (b.live) {
+          kv_tma(to + b.to, &kmap, b.col, u.h, b.off, b.page, &full[s]);
+          kv_tma(to + C::TILE + b.to, &vmap, b.col, u.h, b.off, b.page, &full[s]);
+        }
+      }
+    }
+    if (!ok)  // copies in flight end before the CTA does
+      for (uint32_t j = k > STAGES ? k - STAGES : 0; j < k; ++j) {
+        const uint64_t t = globaltimer_ns();
+        while (!mbar_try_wait(smem_addr(&full[j % STAGES]), (j / STAGES) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
+        }
+      }
+    return;
+  }
+
+  if (tid == 0) write_meta(meta, share, u, total, gridDim.x);
+  const int wm = warp / WN, wn = warp % WN;
+  const float sl2 = p.scale * LOG2E;
+  for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
+    const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+    const int row_base = u.rt * BM, rows = u.s.m * p.G - row_base;  // rows of the sequence from this tile on
+    if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+    // query rows of the tile; rows beyond the sequence's are zeros
+    for (int i = tid; i < BM * CH; i += C::CONSUMERS) {
+      const int r = i / CH, c = i % CH;
+      const bool in = r < rows;
+      const int rr = row_base + (in ? r : 0), tk = token_of(p, rr);
+      cp_async16_zfill(q_s + swz<ROWB>(r, c), p.q + int64_t(u.s.q0 + tk) * p.q_st + int64_t(u.h * p.G + rr - tk * p.G) * p.q_sh + c * 8,
+                       in ? 16 : 0);
+    }
+    cp_async_commit();
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    int lim[2];  // last key each of this thread's two rows sees
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = row_base + wm * 16 + (lane >> 2) + 8 * j;
+      lim[j] = r < u.s.m * p.G ? min(u.s.kv - 1, u.s.kv - u.s.m + token_of(p, r)) : -1;
+    }
+    const int low = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));
+    cp_async_wait<0>();
+    bar_sync(1, C::CONSUMERS);
+    for (int t = t0; t < t1; ++t, ++k) {
+      const uint32_t st = k % STAGES, ks = kv_s + st * 2 * C::TILE, vs = ks + C::TILE;
+      ok = wait(&full[st], (k / STAGES) & 1);
+      if (!ok) return;
+      // the last page may end inside the tile: what its rows past the end hold (it may be NaN) must not meet a weight of zero
+      const int from = u.s.kv - t * AT_BN;
+      if (from < AT_BN) {
+        const int r0 = WN > 1 ? wn * (AT_BN / WN) : 0, r1 = WN > 1 ? r0 + AT_BN / WN : AT_BN;
+        const int first = max(from, r0), step = WN > 1 ? 32 : C::CONSUMERS;
+        for (int i = WN > 1 ? lane : tid; i < (r1 - first) * CH; i += step) {
+          const int r = first + i / CH, c = i % CH;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (c >> 3) * (AT_BN * 128) + r * 128 + (c & 7) * 16), "r"(0)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (WN > 1)
+          __syncwarp();
+        else
+          bar_sync(1, C::CONSUMERS);
+      }
+      float s[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        ldsm_x4(q_s + swz<ROWB>(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)), a);
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+          uint32_t b[4];
+          const int r = wn * (AT_BN / WN) + j * 16 + ((lane >> 4) << 3) + (lane & 7), c = kk * 2 + ((lane >> 3) & 1);
+          ldsm_x4(ks + (c >> 3) * (AT_BN * 128) + swz<128>(r, c & 7), b);
+          mma_bf16(s[2 * j], a, b[0], b[1]);
+          mma_bf16(s[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+      const int key0 = t * AT_BN + wn * (AT_BN / WN) + 2 * (lane & 3);
+      if (low < t * AT_BN + AT_BN - 1) {  // some row does not see the whole tile
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            // a comparison, not an added bias: whatever a masked score is, it leaves no trace
+            s[j][e] = key0 + j * 8 + (e & 1) <= lim[e >> 1] ? s[j][e] * sl2 : -INFINITY;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] *= sl2;
+      }
+      float base[2];
+      bool grow = false;
+      float nm[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float tm = fmaxf(s[0][2 * j], s[0][2 * j + 1]);
+#pragma unroll
+        for (int i = 1; i < NT; ++i) tm = fmaxf(tm, fmaxf(s[i][2 * j], s[i][2 * j + 1]));
+        tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
+        nm[j] = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
+        grow = grow || nm[j] > mx[j] + 8.0f;
+      }
+      // the reference maximum moves only when a row's has grown by more than 2^8 (weights then keep their
+      // relative precision), so that O is rarely rescaled
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float m = fmaxf(mx[j], nm[j]), f = ex2_approx(mx[j] - (m == -INFINITY ? 0.f : m));
+          mx[j] = m;
+          sum[j] *= f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) o[i][2 * j] *= f, o[i][2 * j + 1] *= f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) base[j] = mx[j] == -INFINITY ? 0.f : mx[j];  // a row that has seen no key yet
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][e] = ex2_approx(s[j][e] - base[e >> 1]);
+          sum[e >> 1] += s[j][e];
+        }
+#pragma unroll
+      for (int kk = 0; kk < NT / 2; ++kk) {
+        // weights are rounded to bf16 for the tensor cores; their sum is taken before that
+        const uint32_t a[4] = {cvt_bf16x2(s[2 * kk][0], s[2 * kk][1]), cvt_bf16x2(s[2 * kk][2], s[2 * kk][3]),
+                               cvt_bf16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]), cvt_bf16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t b[4];
+          const int r = wn * (AT_BN / WN) + kk * 16 + (lane & 15), c = j * 2 + (lane >> 4);
+          ldsm_x4_t(vs + (c >> 3) * (AT_BN * 128) + swz<128>(r, c & 7), b);
+          mma_bf16(o[2 * j], a, b[0], b[1]);
+          mma_bf16(o[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && (WN == 1 || t + 1 < t1)) mbar_arrive(&empty[st]);  // the join below uses the last one
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+    }
+    bar_sync(1, C::CONSUMERS);  // every warp is done with the query rows and the last tile
+    const bool whole = t0 == 0 && t1 == u.tiles;
+    float* part = ws_o + (t0 > 0 ? 0 : 1) * BM * (D + 2);
+    if constexpr (WN == 1) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = wm * 16 + (lane >> 2) + 8 * j;
+        if (r >= rows) continue;
+        if (whole) {
+          const float inv = sum[j] > 0.f ? 1.0f / sum[j] : 0.f;
+          uint16_t* dst = p.out + out_at(p, u, row_base + r) + 2 * (lane & 3);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint32_t*>(dst + c * 8) = cvt_bf16x2(o[c][2 * j] * inv, o[c][2 * j + 1] * inv);
+          if ((lane & 3) == 0) write_lse(p, u.s, u.h, row_base + r, mx[j], sum[j]);
+        } else {
+          float* dst = part + r * (D + 2);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<float2*>(dst + c * 8 + 2 * (lane & 3)) = make_float2(o[c][2 * j], o[c][2 * j + 1]);
+          if ((lane & 3) == 0) dst[D] = mx[j], dst[D + 1] = sum[j];
+        }
+      }
+    } else {
+      // join the WN warps' parts of the 16 rows in the last tile's stage, [WN][16][D] floats, columns changed by row
+      static_assert(WM == 1 || WN == 1, "one of the two");
+      const uint32_t st = (k - 1) % STAGES;
+      float* js = reinterpret_cast<float*>(raw + 1024 + st * 2 * C::TILE);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = (lane >> 2) + 8 * j;
+        float* dst = js + (wn * 16 + r) * D;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<float2*>(dst + ((c * 8 + 2 * (lane & 3)) ^ ((r & 7) * 8))) = make_float2(o[c][2 * j], o[c][2 * j + 1]);
+        if ((lane & 3) == 0) sh.ml[wn][r][0] = mx[j], sh.ml[wn][r][1] = sum[j];
+      }
+      bar_sync(1, C::CONSUMERS);
+      for (int r = warp; r < 16 && r < rows; r += WM * WN) {
+        float m = -INFINITY, f[WN], l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) m = fmaxf(m, sh.ml[w][r][0]);
+        const float b = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) {
+          f[w] = ex2_approx(sh.ml[w][r][0] - b);
+          l += f[w] * sh.ml[w][r][1];
+        }
+        const int64_t to = out_at(p, u, row_base + r);
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int c = lane * 2; c < D; c += 64) {
+          float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < WN; ++w) {
+            const float2 y = *reinterpret_cast<const float2*>(js + (w * 16 + r) * D + (c ^ ((r & 7) * 8)));
+            x.x += f[w] * y.x;
+            x.y += f[w] * y.y;
+          }
+          if (whole)
+            *reinterpret_cast<uint32_t*>(p.out + to + c) = cvt_bf16x2(x.x * inv, x.y * inv);
+          else
+            *reinterpret_cast<float2*>(part + r * (D + 2) + c) = x;
+        }
+        if (lane == 0) {
+          if (!whole)
+            part[r * (D + 2) + D] = m, part[r * (D + 2) + D + 1] = l;
+          else
+            write_lse(p, u.s, u.h, row_base + r, m, l);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes there again
+      bar_sync(1, C::CONSUMERS);
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+  }
+}
+
 // Joins the parts of the units that are cut between shares.  Block (i - 1, y) looks at
 // the cut between shares i - 1 and i: where it is the first cut of its unit, the
 // block joins ROWS rows of all parts in the order of the shares (a fixed order: the
@@ -419,16 +721,34 @@ cudaError_t run(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
   return launch_attn_join(p, ctas, C::BM, of, stream);
 }
 
+template <int D, int WM, int WN, int STAGES, int PER_SM>
+cudaError_t run_stream(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
+  using C = AsCfg<D, WM, WN, STAGES>;
+  CUtensorMap maps[2];
+  cudaError_t e = encode_kv_maps(p, AT_BN, maps);
+  if (e != cudaSuccess) return e;
+  static DynSmemCache cache;
+  auto kern = attn_stream_kernel<D, WM, WN, STAGES>;
+  e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
+  if (e != cudaSuccess) return e;
+  const int ctas = multiprocessor_count() * PER_SM;
+  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], of);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_attn_join(p, ctas, C::BM, of, stream);
+}
+
 template <int D, int STAGES, int PER_SM>
 cudaError_t pick(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
-  if (most <= 16) return run<D, 1, 4, STAGES, PER_SM>(p, of, stream);
-  return run<D, 4, 1, STAGES, PER_SM>(p, of, stream);
+  if (kv_tma_takes(p)) return most <= 16 ? run_stream<D, 1, 4, STAGES, PER_SM>(p, of, stream) : run_stream<D, 4, 1, STAGES, PER_SM>(p, of, stream);
+  constexpr int S = D == 256 ? 2 : 3;  // pages of any size
+  return most <= 16 ? run<D, 1, 4, S, PER_SM>(p, of, stream) : run<D, 4, 1, S, PER_SM>(p, of, stream);
 }
 
 cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
-  if (p.D == 64) return pick<64, 3, 2>(p, most, of, stream);
+  if (p.D == 64) return pick<64, 6, 2>(p, most, of, stream);
   if (p.D == 128) return pick<128, 3, 2>(p, most, of, stream);
-  return pick<256, 2, 1>(p, most, of, stream);
+  return pick<256, 3, 1>(p, most, of, stream);
 }
 
 // Sequences of at most so many rows (tokens times query heads of a key head) are bound by reading their keys
@@ -436,6 +756,25 @@ cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, cudaStre
 constexpr int AT_FEW_ROWS = 64;
 
 }  // namespace
+
+// Strides of one-element dims may be anything: they are not taken.
+bool kv_tma_takes(const AttnParams& p) {
+  const int64_t strides[6] = {p.k_sh, p.k_st, p.k_sp, p.v_sh, p.v_st, p.v_sp};
+  for (int64_t s : strides)
+    if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
+  return p.page_size % 8 == 0 && p.pages > 0;
+}
+
+cudaError_t encode_kv_maps(const AttnParams& p, int bn, CUtensorMap* maps) {
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[4] = {uint64_t(p.D), uint64_t(p.Hk), uint64_t(p.page_size), uint64_t(p.pages)};
+    const uint64_t strides[3] = {uint64_t(i ? p.v_sh : p.k_sh) * 2, uint64_t(i ? p.v_st : p.k_st) * 2, uint64_t(i ? p.v_sp : p.k_sp) * 2};
+    const uint32_t box[4] = {64, 1, uint32_t(std::min(p.page_size & -p.page_size, bn)), 1};
+    const cudaError_t e = encode_bf16_map(&maps[i], i ? p.v : p.k, 4, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
 
 cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream) {
   if (ctas < 2) return cudaSuccess;

@@ -210,6 +210,76 @@ __device__ __forceinline__ void write_lse(const AttnParams& p, const SeqLen& s, 
   p.lse[int64_t(s.q0 + t) * p.l_st + int64_t(h * p.G + row - t * p.G) * p.l_sh] = sum > 0.f ? (max2 + log2f(sum)) * LN2 : -INFINITY;
 }
 
+// ---------------------------------------------------------------- keys and values by TMA
+// Tiles of BN keys as boxes of 64 elements by gcd(page_size, BN) rows of one page: whole 8-row swizzle patterns
+// where the page size is a multiple of 8.
+bool kv_tma_takes(const AttnParams& p);
+cudaError_t encode_kv_maps(const AttnParams& p, int bn, CUtensorMap* maps);
+
+__device__ __forceinline__ void kv_tma(uint32_t dst, const CUtensorMap* map, int c, int h, int off, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(c), "r"(h), "r"(off), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// Waits of a whole warp; they give up after a second, or when another warp has: then every role leaves its loop.
+struct WarpWait {
+  uint32_t* err;
+  volatile int* abort;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    bool ok = mbar_try_wait(smem_addr(bar), parity);
+    if (!ok) ok = slow(bar, parity);
+    return __all_sync(0xffffffffu, ok);
+  }
+  __device__ __forceinline__ bool slow(uint64_t* bar, uint32_t parity) const {
+    const uint32_t a = smem_addr(bar);
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1; it < WAIT_LIMIT_ITERS; ++it) {
+      if (mbar_try_wait(a, parity)) return true;
+      if ((it & 63u) == 0) {
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
+      }
+    }
+    *abort = 1;
+    atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
+    return false;
+  }
+};
+
+// The box of tile t that a lane requests: a page past the sequence's end, or outside the cache, reads as zeros
+// (its coordinate lies past the map).
+struct KvBox {
+  bool live;
+  int col, off, page;
+  uint32_t to;  // byte offset in the tile [ATOMS][BN][128 bytes]
+};
+
+template <int BN, int ATOMS>
+__device__ __forceinline__ KvBox kv_box(const AttnParams& p, const Unit& u, const int32_t* table, int t, int lane) {
+  const int rows = min(p.page_size & -p.page_size, BN), atom = lane % ATOMS, part = lane / ATOMS, tok = t * BN + part * rows;
+  KvBox b;
+  b.live = part * rows < BN;
+  b.col = atom * 64;
+  b.to = atom * (BN * 128) + part * rows * 128;
+  b.page = p.pages, b.off = 0;
+  if (b.live && tok < u.s.kv) {
+    const int pi = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
+    b.page = table[pi];
+    b.off = tok - pi * p.page_size;
+    if (b.page < 0 || b.page >= p.pages) {
+      b.page = p.pages, b.off = 0;
+      atomicOr(p.err, GDNR_DEVERR_BAD_SLOT);
+    }
+  }
+  return b;
+}
+
 // Joins the parts of the units of BM rows that were cut between `ctas` shares (gdnr_attn.cu).
 cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream);
 

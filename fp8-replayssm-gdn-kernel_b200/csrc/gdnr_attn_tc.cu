@@ -110,22 +110,11 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap* map, int c, int h, int off, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(c), "r"(h), "r"(off), "r"(page), "r"(smem_addr(bar))
-      : "memory");
-}
-
 __device__ __forceinline__ void tc_tma3(uint32_t dst, const CUtensorMap* map, int c, int h, int token, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(c), "r"(h), "r"(token), "r"(smem_addr(bar))
       : "memory");
-}
-
-__device__ __forceinline__ void tc_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -150,31 +139,6 @@ struct TcBars {
   int abort;
   uint32_t tmem;
   int64_t total;
-};
-
-// Waits of a whole warp; they give up after a second, or when another warp has: then every role leaves its loop.
-struct TcWait {
-  uint32_t* err;
-  volatile int* abort;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    bool ok = mbar_try_wait(smem_addr(bar), parity);
-    if (!ok) ok = slow(bar, parity);
-    return __all_sync(0xffffffffu, ok);
-  }
-  __device__ __forceinline__ bool slow(uint64_t* bar, uint32_t parity) const {
-    const uint32_t a = smem_addr(bar);
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t it = 1; it < WAIT_LIMIT_ITERS; ++it) {
-      if (mbar_try_wait(a, parity)) return true;
-      if ((it & 63u) == 0) {
-        if (*abort) return false;
-        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
-      }
-    }
-    *abort = 1;
-    atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
-    return false;
-  }
 };
 
 template <int D>
@@ -218,7 +182,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   const Share share = share_of(bars.total, blockIdx.x, gridDim.x);
-  const TcWait wait{p.err, &bars.abort};
+  const WarpWait wait{p.err, &bars.abort};
   Unit u;
   u.n = p.N;
   if (share.begin < share.end) {
@@ -240,8 +204,6 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     tc_regs_dec<C::NQ == 2, C::OTHER_REGS>();
     uint32_t slot = 0, nq[2] = {0, 0};  // tiles and query tiles requested so far
     bool ok = true;
-    constexpr int PER_SLOT = BN;
-    const int box = min(p.page_size, BN), boxes = PER_SLOT / box * C::ATOMS;
     for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
       const int t0 = int(at - u.begin);
       int t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
@@ -261,27 +223,15 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
           tc_tma3(base + q * C::Q_BYTES + lane * 16384, &qmap, lane * 64, u.h * p.G, u.s.q0 + token_of(p, u.rt * BM + q * 128), &bars.q_full[q]);
       }
       for (int t = t0; ok && t < t1; ++t) {
-        // where this lane's boxes come from: a page past the sequence's end, or outside the cache, reads as zeros
-        const int atom = lane % C::ATOMS, part = lane / C::ATOMS, tok = t * BN + part * box;
-        int page = p.pages, off = 0;
-        if (lane < boxes && tok < u.s.kv) {
-          const int pi = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
-          off = tok - pi * p.page_size;
-          page = table[pi];
-          if (page < 0 || page >= p.pages) {
-            page = p.pages, off = 0;
-            atomicOr(p.err, GDNR_DEVERR_BAD_SLOT);
-          }
-        }
+        const KvBox b = kv_box<BN, C::ATOMS>(p, u, table, t, lane);
         for (int kv = 0; kv < 2; ++kv, ++slot) {
           const uint32_t s = slot % C::RING;
           if (slot >= C::RING) ok = wait(&bars.kv_empty[s], (slot / C::RING - 1) & 1);
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[s], C::KV_BYTES);
           __syncwarp();
-          if (lane < boxes)
-            tc_tma(kv_base + s * C::KV_BYTES + atom * (BN * 128) + part * box * 128, kv ? &vmap : &kmap, atom * 64, u.h, off, page,
-                   &bars.kv_full[s]);
+          if (b.live)
+            kv_tma(kv_base + s * C::KV_BYTES + b.to, kv ? &vmap : &kmap, b.col, u.h, b.off, b.page, &bars.kv_full[s]);
         }
       }
     }
@@ -447,7 +397,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) tc_arrive(&bars.q_full[q]);
+        if (lane == 0) mbar_arrive(&bars.q_full[q]);
       }
       const int warp_lim = __reduce_min_sync(0xffffffffu, lim);
       for (int t = t0; t < end; ++t) {
@@ -518,7 +468,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         sum += add.x + add.y;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc_arrive(&bars.p_full[buf]);
+        if (lane == 0) mbar_arrive(&bars.p_full[buf]);
         ++no;
       }
       if (!ok) break;
@@ -578,16 +528,11 @@ template <int D>
 cudaError_t run_tc(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
   using C = TcCfg<D>;
   CUtensorMap maps[2];
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t dims[4] = {uint64_t(D), uint64_t(p.Hk), uint64_t(p.page_size), uint64_t(p.pages)};
-    const uint64_t strides[3] = {uint64_t(i ? p.v_sh : p.k_sh) * 2, uint64_t(i ? p.v_st : p.k_st) * 2, uint64_t(i ? p.v_sp : p.k_sp) * 2};
-    const uint32_t box[4] = {64, 1, uint32_t(std::min(p.page_size, C::BN)), 1};
-    cudaError_t e = encode_bf16_map(&maps[i], i ? p.v : p.k, 4, dims, strides, box);
-    if (e != cudaSuccess) return e;
-  }
+  cudaError_t e = encode_kv_maps(p, C::BN, maps);
+  if (e != cudaSuccess) return e;
   static DynSmemCache cache;
   auto kern = attn_tc_kernel<D>;
-  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
+  e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
   if (e != cudaSuccess) return e;
   const int ctas = multiprocessor_count();
   // query rows by TMA where a tile is whole tokens: boxes of 64 elements x G heads x 128 / G tokens
@@ -610,17 +555,8 @@ cudaError_t run_tc(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
 
 int attn_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 
-// Pages that tiles of keys are made of without a remainder (16 rows at least, so that a box is whole swizzle
-// patterns), and scores that grow with the dot product.  Strides of one-element dims may be anything: they are
-// not taken.
-bool attn_tc_takes(const AttnParams& p) {
-  const int bn = p.D == 256 ? 64 : 128;
-  if (p.page_size < 16 || (p.page_size < bn ? bn % p.page_size != 0 : p.page_size % bn != 0)) return false;
-  const int64_t strides[6] = {p.k_sh, p.k_st, p.k_sp, p.v_sh, p.v_st, p.v_sp};
-  for (int64_t s : strides)
-    if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
-  return p.scale > 0.f && p.pages > 0;
-}
+// Scores that grow with the dot product: the maximum is taken before the scale
+bool attn_tc_takes(const AttnParams& p) { return p.scale > 0.f && kv_tma_takes(p); }
 
 cudaError_t launch_attn_tc(const AttnParams& p, int lo, cudaStream_t stream) {
   const AtRows of{lo, INT32_MAX};
