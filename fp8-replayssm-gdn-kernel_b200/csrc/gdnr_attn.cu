@@ -579,14 +579,11 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   __shared__ float sm[AJ_WARPS][D + 2];
   const int i = blockIdx.x + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int* metas = reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2));
-  const int* mi = metas + i * AT_META;
-  const int n = mi[0];
-  if (n < 0) return;  // no unit is cut here
-  const int before = mi[3];
-  if (metas[(i - 1) * AT_META + 5] < before) return;  // the unit begins before share i - 1: not its first cut
-  const SeqLen s = seq_len(p, n, of);
-  const int r = blockIdx.y * ROWS + warp / PER_ROW, rr = mi[2] * BM + r;
+  griddep_wait();
+  CutUnit cut;
+  if (!cut_unit(reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2)), i, cut)) return;
+  const SeqLen s = seq_len(p, cut.n, of);
+  const int r = blockIdx.y * ROWS + warp / PER_ROW, rr = cut.rt * BM + r;
   const bool live = r < BM && rr < s.m * p.G;
   if (__syncthreads_or(live) == 0) return;
   constexpr int E = D / 32;
@@ -594,7 +591,7 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = 0.f;
   if (live) {
-    const int parts = mi[6] - i + 2;  // shares i - 1 .. the one of the unit's last tile
+    const int parts = cut.parts;
     constexpr int AHEAD = 4;
     for (int c0 = warp % PER_ROW; c0 < parts; c0 += PER_ROW * AHEAD) {
       float y[AHEAD][E], pm[AHEAD], pl[AHEAD];
@@ -643,10 +640,10 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   if (!live) return;
   const float inv = l > 0.f ? 1.0f / l : 0.f;
   const int tk = token_of(p, rr);
-  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(mi[1] * p.G + rr - tk * p.G) * p.o_sh;
+  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(cut.h * p.G + rr - tk * p.G) * p.o_sh;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e * 32 + lane] = f_to_bf16(x[e] * inv);
-  if (lane == 0) write_lse(p, s, mi[1], rr, m, l);
+  if (lane == 0) write_lse(p, s, cut.h, rr, m, l);
 }
 
 // The same for parts that lie in columns of BM rows (the tcgen05 kernel's: its threads have a row each).  Block
@@ -656,45 +653,67 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const 
   constexpr int COLS = D / AJ_WARPS;
   const int i = blockIdx.x + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int* metas = reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2));
-  const int* mi = metas + i * AT_META;
-  const int n = mi[0];
-  if (n < 0 || metas[(i - 1) * AT_META + 5] < mi[3]) return;  // no unit is cut here, or not for the first time
-  const SeqLen s = seq_len(p, n, of);
-  const int r = blockIdx.y * 32 + lane, rr = mi[2] * BM + r;
+  griddep_wait();
+  CutUnit cut;
+  if (!cut_unit(reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2)), i, cut)) return;
+  const SeqLen s = seq_len(p, cut.n, of);
+  const int r = blockIdx.y * 32 + lane, rr = cut.rt * BM + r;
   if (rr >= s.m * p.G) return;
   float m = -INFINITY, l = 0.f, x[COLS];
 #pragma unroll
   for (int e = 0; e < COLS; ++e) x[e] = 0.f;
-  const int parts = mi[6] - i + 2;
-  for (int c = 0; c < parts; ++c) {
+  // the next part is on its way while one is added
+  float next[COLS], nm, nl;
+  auto request = [&](int c) {
     const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
-    const float pm = src[D * BM], pl = src[(D + 1) * BM];
-    float y[COLS];
+    nm = src[D * BM], nl = src[(D + 1) * BM];
 #pragma unroll
-    for (int e = 0; e < COLS; ++e) y[e] = src[(warp * COLS + e) * BM];
-    const float nm = fmaxf(m, pm), b = nm == -INFINITY ? 0.f : nm;
+    for (int e = 0; e < COLS; ++e) next[e] = src[(warp * COLS + e) * BM];
+  };
+  request(0);
+  for (int c = 0; c < cut.parts; ++c) {
+    float y[COLS];
+    const float pm = nm, pl = nl;
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) y[e] = next[e];
+    if (c + 1 < cut.parts) request(c + 1);
+    const float top = fmaxf(m, pm), b = top == -INFINITY ? 0.f : top;
     const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
-    m = nm;
+    m = top;
     l = l * f0 + pl * f1;
 #pragma unroll
     for (int e = 0; e < COLS; ++e) x[e] = x[e] * f0 + y[e] * f1;
   }
   const float inv = l > 0.f ? 1.0f / l : 0.f;
   const int tk = token_of(p, rr);
-  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(mi[1] * p.G + rr - tk * p.G) * p.o_sh + warp * COLS;
+  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(cut.h * p.G + rr - tk * p.G) * p.o_sh + warp * COLS;
 #pragma unroll
   for (int e = 0; e < COLS; e += 8)
     *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16x2(x[e] * inv, x[e + 1] * inv), pack_bf16x2(x[e + 2] * inv, x[e + 3] * inv),
                                                     pack_bf16x2(x[e + 4] * inv, x[e + 5] * inv), pack_bf16x2(x[e + 6] * inv, x[e + 7] * inv));
-  if (warp == 0) write_lse(p, s, mi[1], rr, m, l);
+  if (warp == 0) write_lse(p, s, cut.h, rr, m, l);
+}
+
+// The join may be set up while the kernel before it still runs; it waits for that one's results (griddep_wait).
+template <class K>
+void launch_join(K kern, dim3 grid, const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(AJ_WARPS * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, p, of, ctas);
 }
 
 template <int D, int BM, int ROWS>
 void join(const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
   // rows a unit can have, by the longest sequence the host knows of
   const int rows = int(std::min<int64_t>(BM, int64_t(p.max_q) * p.G));
-  attn_join_kernel<D, BM, ROWS><<<dim3(ctas - 1, (rows + ROWS - 1) / ROWS), AJ_WARPS * 32, 0, stream>>>(p, of, ctas);
+  launch_join(attn_join_kernel<D, BM, ROWS>, dim3(ctas - 1, (rows + ROWS - 1) / ROWS), p, ctas, of, stream);
 }
 
 template <int D>
@@ -704,7 +723,7 @@ void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream
   else if (bm == 64)
     join<D, 64, 2>(p, ctas, of, stream);
   else
-    attn_join_columns_kernel<D, D == 256 ? 128 : 256><<<dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), AJ_WARPS * 32, 0, stream>>>(p, of, ctas);
+    launch_join(attn_join_columns_kernel<D, D == 256 ? 128 : 256>, dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), p, ctas, of, stream);
 }
 
 template <int D, int WM, int WN, int STAGES, int PER_SM>

@@ -185,17 +185,27 @@ __device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
 // A CTA's record for the join, in the workspace behind the parts [ctas][2][BM][D + 2]: a share that
 // begins inside a unit leaves its part of it in slot 0, one that only ends inside in slot 1.
 __device__ __forceinline__ void write_meta(int* meta, const Share& share, const Unit& u, int64_t total, int ctas) {
-  meta[0] = share.begin > u.begin ? u.n : -1;  // the unit this share begins in, if it begins inside it
-  meta[1] = u.h;
-  meta[2] = u.rt;
-  meta[3] = int(share.begin - u.begin);            // tiles of that unit in earlier shares
-  meta[4] = int(u.begin + u.tiles - share.begin);  // tiles of it from here on
-  meta[5] = int(share.end - share.begin);
   // the share of the unit's last tile: the last one that begins at or before it
   const int64_t use = min(int64_t(ctas), (total + 1) / 2), last = u.begin + u.tiles - 1;
   int64_t c = last * use / total;
   while (c + 1 < use && total * (c + 1) / use <= last) ++c;
-  meta[6] = int(c);
+  int4* const to = reinterpret_cast<int4*>(meta);
+  // the unit this share begins in, if it begins inside it (else n = -1), and its tiles in earlier shares
+  to[0] = make_int4(share.begin > u.begin ? u.n : -1, u.h, u.rt, int(share.begin - u.begin));
+  to[1] = make_int4(int(c), int(share.end - share.begin), 0, 0);
+}
+
+// What a join's block reads of share i: false where no unit is cut between shares i - 1 and i, or not for the
+// first time.
+struct CutUnit {
+  int n, h, rt, parts;  // parts: shares i - 1 .. the one of the unit's last tile
+};
+
+__device__ __forceinline__ bool cut_unit(const int* metas, int i, CutUnit& c) {
+  const int4 a = *reinterpret_cast<const int4*>(metas + i * AT_META), b = *reinterpret_cast<const int4*>(metas + i * AT_META + 4);
+  const int before = metas[(i - 1) * AT_META + 5];  // tiles of the share before
+  c.n = a.x, c.h = a.y, c.rt = a.z, c.parts = b.x - i + 2;
+  return a.x >= 0 && before >= a.w;  // else the unit begins before share i - 1
 }
 
 // Row r of a sequence: token q0 + r / G, query head h G + r % G.
