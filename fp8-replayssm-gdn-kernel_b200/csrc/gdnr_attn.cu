@@ -34,7 +34,7 @@ struct AtCfg {
 template <int D, int WM, int WN, int STAGES>
 __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constant__ AttnParams p, const AtRows of) {
   using C = AtCfg<D, WM, WN, STAGES>;
-  using T = AtTile<C::BM, AT_BN>;
+  using T = AtTile<C::BM, AT_BN, 1>;
   constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t sh_total;
@@ -50,16 +50,18 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
   }
   __syncthreads();
   const int64_t total = sh_total;
-  const Share share = share_of(total, blockIdx.x, gridDim.x);
+  const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   if (share.begin >= share.end) {
     if (tid == 0) meta[0] = -1;
     return;
   }
   Unit u = find_unit<T>(p, of, share.begin, lane);
-  if (tid == 0) write_meta(meta, share, u, total, gridDim.x);
+  if (tid == 0) write_meta<T>(meta, share, u, total, gridDim.x);
   const float sl2 = p.scale * LOG2E;
   for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-    const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+    const Tiles part_of = tiles_of<T>(share, u);
+    const int t0 = part_of.begin, t1 = part_of.end;
+    if (t1 <= t0) continue;
     const int rows = u.s.m * p.G - u.rt * BM;  // rows of the sequence from this tile on
     const int row_base = u.rt * BM;
     const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
     attn_stream_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const AtRows of) {
   using C = AsCfg<D, WM, WN, STAGES>;
-  using T = AtTile<C::BM, AT_BN>;
+  using T = AtTile<C::BM, AT_BN, 1>;
   constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
   extern __shared__ __align__(1024) uint8_t raw[];
   AsShared& sh = *reinterpret_cast<AsShared*>(raw);
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   }
   __syncthreads();
   const int64_t total = sh.total;
-  const Share share = share_of(total, blockIdx.x, gridDim.x);
+  const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   if (share.begin >= share.end) {
     if (tid == 0) meta[0] = -1;
     return;
@@ -330,7 +332,9 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
 
   if (warp == WM * WN) {
     for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const Tiles part_of = tiles_of<T>(share, u);
+      const int t0 = part_of.begin, t1 = part_of.end;
+      if (t1 <= t0) continue;
       const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
       for (int t = t0; t < t1; ++t, ++k) {
         const KvBox b = kv_box<AT_BN, C::ATOMS>(p, u, table, t, lane);
@@ -354,11 +358,13 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
     return;
   }
 
-  if (tid == 0) write_meta(meta, share, u, total, gridDim.x);
+  if (tid == 0) write_meta<T>(meta, share, u, total, gridDim.x);
   const int wm = warp / WN, wn = warp % WN;
   const float sl2 = p.scale * LOG2E;
   for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-    const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+    const Tiles part_of = tiles_of<T>(share, u);
+    const int t0 = part_of.begin, t1 = part_of.end;
+    if (t1 <= t0) continue;
     const int row_base = u.rt * BM, rows = u.s.m * p.G - row_base;  // rows of the sequence from this tile on
     if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
     // query rows of the tile; rows beyond the sequence's are zeros

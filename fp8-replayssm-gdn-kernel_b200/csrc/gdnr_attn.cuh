@@ -12,9 +12,10 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int AT_META = 8;  // ints of one CTA's record
 
 // A kernel's tiles: BM rows (token, query head) by BN keys, for the sequences whose rows are in (lo, hi].
-template <int BM_, int BN_>
+// OVER: what beginning and ending a unit costs, in tiles.
+template <int BM_, int BN_, int OVER_>
 struct AtTile {
-  static constexpr int BM = BM_, BN = BN_;
+  static constexpr int BM = BM_, BN = BN_, OVER = OVER_;
 };
 
 struct AtRows {
@@ -51,8 +52,9 @@ __device__ __forceinline__ int keys_seen(const AttnParams& p, const SeqLen& s, i
 }
 
 // A unit is (sequence, key head, tile of BM rows); its cost is the number of key tiles
-// its last row sees.  The units of the batch laid end to end are cut into equal shares,
-// one per CTA, so ragged lengths and few heads fill the machine alike.
+// its last row sees, and OVER places before them.  The units of the batch laid end to end are cut into
+// equal shares, one per CTA, so ragged lengths and few heads fill the machine alike.  A cut among a unit's
+// first OVER places leaves the unit whole, to the later share.
 template <class T>
 __device__ __forceinline__ int unit_tiles(const AttnParams& p, const SeqLen& s, int rt) {
   return max(1, (keys_seen(p, s, (rt + 1) * T::BM) + T::BN - 1) / T::BN);  // a unit without keys still writes its rows
@@ -62,20 +64,20 @@ __device__ __forceinline__ int unit_tiles(const AttnParams& p, const SeqLen& s, 
 // keep a single lane busy.
 __device__ __forceinline__ int lanes_per_seq(int n) { return n >= 32 ? 1 : (n > 16 ? 1 : (n > 8 ? 2 : (n > 4 ? 4 : (n > 2 ? 8 : (n > 1 ? 16 : 32))))); }
 
-// Key tiles of sequence n (0 past the last), in each of its `per` lanes.
+// Places of sequence n (0 past the last), in each of its `per` lanes.
 template <class T>
 __device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const AtRows& r, int n, int per, int lane) {
   int64_t sum = 0;
   if (n < p.N) {
     const SeqLen s = seq_len(p, n, r);
     const int rts = (s.m * p.G + T::BM - 1) / T::BM;
-    for (int rt = lane & (per - 1); rt < rts; rt += per) sum += unit_tiles<T>(p, s, rt);
+    for (int rt = lane & (per - 1); rt < rts; rt += per) sum += T::OVER + unit_tiles<T>(p, s, rt);
   }
   for (int o = per >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum * p.Hk;
 }
 
-// Key tiles of the batch (one whole warp).
+// Places of the batch (one whole warp).
 template <class T>
 __device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& r, int lane) {
   const int per = lanes_per_seq(p.N), step = 32 / per;
@@ -92,11 +94,11 @@ __device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& 
 struct Unit {
   int n, h, rt;
   SeqLen s;
-  int64_t begin;  // first key tile of the unit
+  int64_t begin;  // first place of the unit
   int tiles;
 };
 
-// The unit that key tile `at` of the batch falls into (one whole warp).
+// The unit that place `at` of the batch falls into (one whole warp).
 template <class T>
 __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, int64_t at, int lane) {
   const int per = lanes_per_seq(p.N), step = 32 / per;
@@ -122,7 +124,7 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
       start += u.h * per_head;
       const int rts = (u.s.m * p.G + T::BM - 1) / T::BM;
       for (int rt0 = 0; rt0 < rts; rt0 += 32) {
-        const int mine = rt0 + lane < rts ? unit_tiles<T>(p, u.s, rt0 + lane) : 0;
+        const int mine = rt0 + lane < rts ? T::OVER + unit_tiles<T>(p, u.s, rt0 + lane) : 0;
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -133,7 +135,7 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
         if (in) {
           const int l = __ffs(in) - 1;
           u.rt = rt0 + l;
-          u.tiles = __shfl_sync(0xffffffffu, mine, l);
+          u.tiles = __shfl_sync(0xffffffffu, mine, l) - T::OVER;
           u.begin = start + __shfl_sync(0xffffffffu, sum - mine, l);
           return u;
         }
@@ -149,7 +151,7 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
 // The next unit in order.
 template <class T>
 __device__ __forceinline__ void next_unit(const AttnParams& p, const AtRows& r, Unit& u) {
-  u.begin += u.tiles;
+  u.begin += T::OVER + u.tiles;
   ++u.rt;
   if (u.rt * T::BM >= u.s.m * p.G) {
     u.rt = 0;
@@ -168,31 +170,56 @@ struct Share {
   int64_t begin, end;
 };
 
-// Share i of `total` key tiles; at least two tiles each, so that small batches do not
-// pay for joining shares of one tile.
+// Shares of `total` places: no more than units of one tile would give, so that small batches do not pay for joining.
+template <class T>
+__device__ __forceinline__ int64_t shares(int64_t total, int ctas) {
+  return min(int64_t(ctas), (total + T::OVER) / (T::OVER + 1));
+}
+
+// Share i: sizes differ by one at most, the larger ones first.
+template <class T>
 __device__ __forceinline__ Share share_of(int64_t total, int i, int ctas) {
-  const int64_t use = min(int64_t(ctas), (total + 1) / 2);
+  const int64_t use = shares<T>(total, ctas);
   Share s;
   if (i >= use) {
     s.begin = s.end = total;
     return s;
   }
-  s.begin = total * i / use;
-  s.end = total * (i + 1) / use;
+  const int64_t size = total < INT32_MAX ? int32_t(total) / int32_t(use) : total / use, more = total - size * use;
+  s.begin = size * i + min(int64_t(i), more);
+  s.end = s.begin + size + (i < more ? 1 : 0);
   return s;
+}
+
+// The share that place `at` falls into.
+template <class T>
+__device__ __forceinline__ int share_at(int64_t total, int64_t at, int ctas) {
+  const int64_t use = shares<T>(total, ctas), size = total / use, more = total - size * use;
+  return int(at < more * (size + 1) ? at / (size + 1) : more + (at - more * (size + 1)) / size);
+}
+
+// Key tiles of the unit that a share has.
+struct Tiles {
+  int begin, end;
+};
+
+template <class T>
+__device__ __forceinline__ Tiles tiles_of(const Share& s, const Unit& u) {
+  Tiles t;
+  t.begin = int(max(s.begin - u.begin - T::OVER, int64_t(0)));
+  t.end = int(max(min(s.end - u.begin - T::OVER, int64_t(u.tiles)), int64_t(0)));
+  return t;
 }
 
 // A CTA's record for the join, in the workspace behind the parts [ctas][2][BM][D + 2]: a share that
 // begins inside a unit leaves its part of it in slot 0, one that only ends inside in slot 1.
+template <class T>
 __device__ __forceinline__ void write_meta(int* meta, const Share& share, const Unit& u, int64_t total, int ctas) {
-  // the share of the unit's last tile: the last one that begins at or before it
-  const int64_t use = min(int64_t(ctas), (total + 1) / 2), last = u.begin + u.tiles - 1;
-  int64_t c = last * use / total;
-  while (c + 1 < use && total * (c + 1) / use <= last) ++c;
+  const int64_t before = share.begin - u.begin - T::OVER;  // tiles of the unit in earlier shares
   int4* const to = reinterpret_cast<int4*>(meta);
-  // the unit this share begins in, if it begins inside it (else n = -1), and its tiles in earlier shares
-  to[0] = make_int4(share.begin > u.begin ? u.n : -1, u.h, u.rt, int(share.begin - u.begin));
-  to[1] = make_int4(int(c), int(share.end - share.begin), 0, 0);
+  // the unit this share continues (n = -1: none) and the share of its last tile
+  to[0] = make_int4(before > 0 ? u.n : -1, u.h, u.rt, int(max(before, int64_t(0))));
+  to[1] = make_int4(share_at<T>(total, u.begin + T::OVER + u.tiles - 1, ctas), int(share.end - share.begin), 0, 0);
 }
 
 // What a join's block reads of share i: false where no unit is cut between shares i - 1 and i, or not for the
@@ -203,9 +230,9 @@ struct CutUnit {
 
 __device__ __forceinline__ bool cut_unit(const int* metas, int i, CutUnit& c) {
   const int4 a = *reinterpret_cast<const int4*>(metas + i * AT_META), b = *reinterpret_cast<const int4*>(metas + i * AT_META + 4);
-  const int before = metas[(i - 1) * AT_META + 5];  // tiles of the share before
+  const int before = metas[(i - 1) * AT_META + 5];  // places of the share before
   c.n = a.x, c.h = a.y, c.rt = a.z, c.parts = b.x - i + 2;
-  return a.x >= 0 && before >= a.w;  // else the unit begins before share i - 1
+  return a.x >= 0 && before >= a.w;  // else share i - 1 continues the unit, too
 }
 
 // Row r of a sequence: token q0 + r / G, query head h G + r % G.

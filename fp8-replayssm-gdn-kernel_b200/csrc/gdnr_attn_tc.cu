@@ -36,6 +36,7 @@ struct TcCfg {
   static constexpr int SMEM = NQ * Q_BYTES + RING * KV_BYTES + 1024;
   // tensor memory columns: two buffers of S (P lies over the first half of its S), then O
   static constexpr int S_COLS = BN, O_COL = 256;
+  static constexpr int OVER = D == 256 ? 4 : 2;  // a unit's beginning and end, 4 to 5 us, in tiles of 0.9 or 2.3 us
   static_assert(SMEM + 512 <= 227 * 1024, "one CTA per SM");
 };
 
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                    const __grid_constant__ CUtensorMap qmap, const AtRows of, const int q_tma) {
   using C = TcCfg<D>;
-  using T = AtTile<C::BM, C::BN>;
+  using T = AtTile<C::BM, C::BN, C::OVER>;
   constexpr int NQ = C::NQ, BN = C::BN, BM = C::BM;
   extern __shared__ uint8_t raw[];
   __shared__ TcBars bars;
@@ -181,13 +182,13 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  const Share share = share_of(bars.total, blockIdx.x, gridDim.x);
+  const Share share = share_of<T>(bars.total, blockIdx.x, gridDim.x);
   const WarpWait wait{p.err, &bars.abort};
   Unit u;
   u.n = p.N;
   if (share.begin < share.end) {
     u = find_unit<T>(p, of, share.begin, lane);
-    if (tid == 0) write_meta(meta, share, u, bars.total, gridDim.x);
+    if (tid == 0) write_meta<T>(meta, share, u, bars.total, gridDim.x);
   } else if (tid == 0) {
     meta[0] = -1;
   }
@@ -205,8 +206,10 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     uint32_t slot = 0, nq[2] = {0, 0};  // tiles and query tiles requested so far
     bool ok = true;
     for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-      const int t0 = int(at - u.begin);
-      int t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const Tiles part_of = tiles_of<T>(share, u);
+      const int t0 = part_of.begin;
+      int t1 = part_of.end;
+      if (t1 <= t0) continue;
       int most = seen(0);
       if (NQ > 1) most = max(most, seen(1));
       t1 = min(t1, most);
@@ -272,7 +275,9 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       if (last) tc_commit(&bars.done[q]);
     };
     for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const Tiles part_of = tiles_of<T>(share, u);
+      const int t0 = part_of.begin, t1 = part_of.end;
+      if (t1 <= t0) continue;
       int end[2] = {min(t1, seen(0)), NQ > 1 ? min(t1, seen(1)) : 0};
       const int last = max(end[0], end[1]);
       if (last <= t0) continue;
@@ -366,7 +371,9 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     uint32_t ns[2] = {0, 0}, no = 0, nd = 0;  // phases of s_full, o_full, done
     bool ok = true;
     for (int64_t at = share.begin; ok && at < share.end; next_unit<T>(p, of, u), at = u.begin) {
-      const int t0 = int(at - u.begin), t1 = int(min(share.end - u.begin, int64_t(u.tiles)));
+      const Tiles part_of = tiles_of<T>(share, u);
+      const int t0 = part_of.begin, t1 = part_of.end;
+      if (t1 <= t0) continue;
       const int end = min(t1, seen(q));
       const int row = u.rt * BM + q * 128 + r;  // row of the sequence
       const bool live = row < u.s.m * p.G;
