@@ -166,7 +166,7 @@ __device__ __forceinline__ uint32_t ck_in_block(int row, int half) { return row 
 struct CkImage {
   // diagonal blocks: T = (I + A)^-1 of the block, below them: -A
   uint8_t t_hi[CK_TRI], t_lo[CK_TRI], p_hi[CK_TRI], p_lo[CK_TRI];
-  float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
+  float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, -beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
   float pad[15];
 };
 static_assert(sizeof(CkImage) == CK_IMAGE_BYTES && sizeof(CkImage) % 16 == 0, "copied in bulk");
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
         const float gh = g_hi[gt], gl = g_lo[gt], ch = g_hi[CK_C - 1], cl = g_lo[CK_C - 1];
         const float ex = ex2_approx(gh + gl), be = gbeta[gt];
         img.beta[gt] = be;
-        img.cx[gt] = be * ex * sm.rk[gt];
+        img.cx[gt] = -be * ex * sm.rk[gt];
         img.cq[gt] = ex * sm.rq[gt];
         img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
         if (gt == 0) img.total = ex2_approx(ch + cl);
@@ -433,6 +433,9 @@ template <int NW, int KS>
 struct CsCfg {
   static constexpr int GROUPS = NW / KS, ROWS = GROUPS * 16, PARTS = 128 / ROWS;
   static constexpr int V_BOXES = ROWS > 64 ? 2 : 1;
+  // four warps leave room for one more that requests the chunks; of eight, the first does it beside its work
+  static constexpr bool LOADER = NW == 4;
+  static constexpr int THREADS = (NW + (LOADER ? 1 : 0)) * 32;
 };
 
 template <int NW, int KS>
@@ -452,6 +455,14 @@ struct CsSmem {
   uint64_t full[CS_STAGES], empty[CS_STAGES];
 };
 static_assert(sizeof(CsSmem<8, 1>) + 1024 <= MAX_DYN_SMEM && sizeof(CsSmem<4, 2>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
+
+// Two neighbouring floats of a factor
+__device__ __forceinline__ uint64_t pair_at(const float* p) { return *reinterpret_cast<const uint64_t*>(p); }
+
+__device__ __forceinline__ void plus4(float* x, const float4& y) {
+  const float2 a = unpack2(add2(pack2(x[0], x[1]), pack2(y.x, y.y))), b = unpack2(add2(pack2(x[2], x[3]), pack2(y.z, y.w)));
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
 
 // Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
 __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
@@ -526,7 +537,7 @@ __device__ __forceinline__ void ck_out_column(float (*O)[4], const uint32_t* nh,
 }
 
 template <int NW, int KS>
-__global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
+__global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
                                                                   const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
   using C = CsCfg<NW, KS>;
@@ -568,8 +579,20 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
       ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + (v0 & 64) + b * 64, row, bar);
     bulk_g2s(&st.img, images + int64_t(c) * p.HV * CK_IMAGE_BYTES, CK_IMAGE_BYTES, bar);
   };
-  int issued = 0;  // of thread 0
-  if (tid == 0)
+  if (C::LOADER && warp == NW) {
+    if (lane == 0) {
+      int c = 0;
+      for (; c < chunks; ++c) {
+        if (c >= CS_STAGES && !mbar_wait_bounded(&sm.empty[c % CS_STAGES], (c / CS_STAGES - 1) & 1, p.err)) break;
+        load(c);
+      }
+      if (c < chunks)  // a wait gave up: copies in flight are waited for
+        for (int k = max(c - CS_STAGES, 0); k < c; ++k) mbar_wait_bounded(&sm.full[k % CS_STAGES], (k / CS_STAGES) & 1, p.err);
+    }
+    return;
+  }
+  int issued = 0;  // of thread 0, where there is no loader
+  if (!C::LOADER && tid == 0)
     for (; issued < CS_STAGES - 1 && issued < chunks; ++issued) load(issued);
 
   const int g = lane >> 2, t2 = 2 * (lane & 3);
@@ -603,10 +626,6 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
     }
     float X[8][4], O[8][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) X[j][e] = O[j][e] = 0.f;
-#pragma unroll
     for (int s = 0; s < KT / 2; ++s) {
       uint32_t hi[4], lo[4];
       ck_left(S + 2 * s, hi, lo);
@@ -624,12 +643,17 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            mma_bf16(X[2 * jj + j], half ? lo : hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
-            mma_bf16(O[2 * jj + j], half ? lo : hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            if (s == 0 && half == 0) {
+              mma_bf16_first(X[2 * jj + j], hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
+              mma_bf16_first(O[2 * jj + j], hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            } else {
+              mma_bf16(X[2 * jj + j], half ? lo : hi, bk[j >> 1][2 * (j & 1)], bk[j >> 1][2 * (j & 1) + 1]);
+              mma_bf16(O[2 * jj + j], half ? lo : hi, bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            }
           }
       }
     }
-    if (tid == 0 && issued < chunks) {
+    if (!C::LOADER && tid == 0 && issued < chunks) {
       // the stage of the chunk before this one, which all warps have left by now or soon
       if (c > 0) ok = mbar_wait_bounded(&sm.empty[issued % CS_STAGES], ((c - 1) / CS_STAGES) & 1, p.err);
       if (!ok) break;
@@ -650,16 +674,14 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float4 y = sm.swap[peer][j][lane];
-        X[j][0] += y.x, X[j][1] += y.y, X[j][2] += y.z, X[j][3] += y.w;
+        plus4(X[j], y);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float4 y = sm.swap[peer][8 + j][lane];
-        float* a = O[j < 2 ? j : j + 4];
-        float* b = O[j + 2];
         // kh 0 keeps blocks 0 and 3, kh 1 blocks 1 and 2; the other two are not used again
-        a[0] += y.x, a[1] += y.y, a[2] += y.z, a[3] += y.w;
-        b[0] += y.x, b[1] += y.y, b[2] += y.z, b[3] += y.w;
+        plus4(O[j < 2 ? j : j + 4], y);
+        plus4(O[j + 2], y);
       }
       bar_sync(2 + warp % C::GROUPS, 64);  // read before the next chunk's overwrite it
     }
@@ -672,34 +694,33 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int tok = j * 16 + hf * 8 + t2;
-        const float2 be = *reinterpret_cast<const float2*>(&im.beta[tok]), cx = *reinterpret_cast<const float2*>(&im.cx[tok]),
-                     cq = *reinterpret_cast<const float2*>(&im.cq[tok]);
+        // (im.cx holds -beta e^G rk)
+        const uint64_t be = pair_at(&im.beta[tok]), cx = pair_at(&im.cx[tok]);
         const float2 v0f = bf16x2_to_f2(w[2 * hf]), v1f = bf16x2_to_f2(w[2 * hf + 1]);
         float* x = X[2 * j + hf];
-        float* o = O[2 * j + hf];
-        x[0] = be.x * v0f.x - cx.x * x[0], x[1] = be.y * v0f.y - cx.y * x[1];
-        x[2] = be.x * v1f.x - cx.x * x[2], x[3] = be.y * v1f.y - cx.y * x[3];
+        const float2 r0 = unpack2(fma2(pack2(x[0], x[1]), cx, mul2(be, pack2(v0f.x, v0f.y))));
+        const float2 r1 = unpack2(fma2(pack2(x[2], x[3]), cx, mul2(be, pack2(v1f.x, v1f.y))));
+        x[0] = r0.x, x[1] = r0.y, x[2] = r1.x, x[3] = r1.y;
         top0 = fmaxf(top0, fmaxf(fabsf(x[0]), fabsf(x[1])));
         top1 = fmaxf(top1, fmaxf(fabsf(x[2]), fabsf(x[3])));
-        o[0] *= cq.x, o[1] *= cq.y, o[2] *= cq.x, o[3] *= cq.y;
       }
     }
     // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
     float up0, down0, up1, down1;
     ck_row_scale(top0, up0, down0);
     ck_row_scale(top1, up1, down1);
+    const uint64_t up0_2 = pack2(up0, up0), up1_2 = pack2(up1, up1);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      X[j][0] *= up0, X[j][1] *= up0, X[j][2] *= up1, X[j][3] *= up1;
-      O[j][0] *= up0, O[j][1] *= up0, O[j][2] *= up1, O[j][3] *= up1;
+      scale2(X[j], up0_2);
+      scale2(X[j] + 2, up1_2);
+      const uint64_t cq = pair_at(&im.cq[j * 8 + t2]);
+      scale2(O[j], mul2(cq, up0_2));
+      scale2(O[j] + 2, mul2(cq, up1_2));
     }
     const uint32_t th = smem_addr(im.t_hi), tlo = smem_addr(im.t_lo), ph = smem_addr(im.p_hi), pl = smem_addr(im.p_lo);
     float N[8][4];
     uint32_t nh[4][4], nl[4][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) N[j][e] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // column j of blocks: T_jj, then -A_ij below it
@@ -714,7 +735,10 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
       for (int q = 0; q < 3; ++q)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          mma_f16(N[2 * j + i], q == 1 ? rl : rh, (q == 2 ? bl : b)[j][2 * i], (q == 2 ? bl : b)[j][2 * i + 1]);
+          if (q == 0)
+            mma_f16_first(N[2 * j + i], rh, b[j][2 * i], b[j][2 * i + 1]);
+          else
+            mma_f16(N[2 * j + i], q == 1 ? rl : rh, (q == 2 ? bl : b)[j][2 * i], (q == 2 ? bl : b)[j][2 * i + 1]);
       ck_left_f16(N + 2 * j, nh[j], nl[j]);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
@@ -724,20 +748,23 @@ __global__ void __launch_bounds__(NW * 32, 1) prefill_scan_kernel(const __grid_c
           mma_f16(X[i], q == 1 ? nl[j] : nh[j], w[2 * (i & 1)], w[2 * (i & 1) + 1]);
         }
     }
-    const float total = im.total;
+    const uint64_t total = pack2(im.total, im.total), down0_2 = pack2(down0, down0), down1_2 = pack2(down1, down1);
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[i][e] *= total;
+    for (int i = 0; i < KT; ++i) {
+      scale2(S[i], total);
+      scale2(S[i] + 2, total);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t hi[4], lo[4], rest[4];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const float2 cs = *reinterpret_cast<const float2*>(&im.cs[j * 16 + hf * 8 + t2]);
-        const float* x = N[2 * j + hf];
-        split3_bf16x2(x[0] * (cs.x * down0), x[1] * (cs.y * down0), hi[2 * hf], lo[2 * hf], rest[2 * hf]);
-        split3_bf16x2(x[2] * (cs.x * down1), x[3] * (cs.y * down1), hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
+        const uint64_t cs = pair_at(&im.cs[j * 16 + hf * 8 + t2]);
+        float* x = N[2 * j + hf];
+        scale2(x, mul2(cs, down0_2));
+        scale2(x + 2, mul2(cs, down1_2));
+        split3_bf16x2(x[0], x[1], hi[2 * hf], lo[2 * hf], rest[2 * hf]);
+        split3_bf16x2(x[2], x[3], hi[2 * hf + 1], lo[2 * hf + 1], rest[2 * hf + 1]);
       }
 #pragma unroll
       for (int ii = 0; ii < KT / 2; ii += 4) {
@@ -794,7 +821,7 @@ cudaError_t scan(const PrefillParams& p, const CUtensorMap& map, cudaStream_t st
   auto kern = prefill_scan_kernel<NW, KS>;
   cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), bytes, cache);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(unsigned(int64_t(p.N) * p.HV * CsCfg<NW, KS>::PARTS)), NW * 32, bytes, stream>>>(p, map);
+  kern<<<dim3(unsigned(int64_t(p.N) * p.HV * CsCfg<NW, KS>::PARTS)), CsCfg<NW, KS>::THREADS, bytes, stream>>>(p, map);
   return cudaGetLastError();
 }
 
