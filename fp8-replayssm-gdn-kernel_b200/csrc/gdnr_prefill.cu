@@ -8,6 +8,8 @@
 #include "gdnr_hybrid.h"
 #include "gdnr_tile.cuh"
 
+#include <algorithm>
+
 namespace gdnr {
 
 namespace {
@@ -192,6 +194,9 @@ __device__ __forceinline__ void ck_zero_rows(uint8_t* tile, int boxes, int valid
   }
 }
 
+// Two neighbouring floats of a factor
+__device__ __forceinline__ uint64_t pair_at(const float* p) { return *reinterpret_cast<const uint64_t*>(p); }
+
 // ---------------------------------------------------------------- chunked form, first kernel
 constexpr int CD_THREADS = 256;
 constexpr int CD_LDA = 20;  // floats of a row of a diagonal block
@@ -199,7 +204,7 @@ constexpr int CD_LDA = 20;  // floats of a row of a diagonal block
 struct CdSmem {
   uint8_t k[CK_C * 256], q[CK_C * 256];
   CkImage img[2];
-  float a[CK_C * CD_LDA];  // -A's diagonal blocks: warp w's at rows 16 w
+  float a[2][CK_C * CD_LDA];  // -A's diagonal blocks of two heads: warp w's at rows 16 w
   float g_hi[2][CK_C], g_lo[2][CK_C], gbeta[2][CK_C];  // prefix sums of the gates in units of ln 2, in two parts
   float rk[CK_C], rq[CK_C];
   uint64_t bar;
@@ -332,12 +337,25 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
     (of_q ? sm.rq : sm.rk)[row] = gain * rsqrtf(x0 + L2_EPS);
     (of_q ? sm.rq : sm.rk)[row + 8] = gain * rsqrtf(x1 + L2_EPS);
   }
+  __syncthreads();  // gates and norms
+  // what all heads share: the products times both norms (and the sign of -A)
+  const int rbm = warp == 1 ? warp : rb2;
+  const float gain = of_q ? 1.f : -1.f;
+  const float* rn = of_q ? sm.rq : sm.rk;
+#pragma unroll
+  for (int u = 0; u < 5; ++u) {
+    const int row = (u < 2 ? warp : (u < 4 ? rbm : rb2)) * 16 + (lane >> 2);
+    const uint64_t rk = pair_at(&sm.rk[unit_tile[u] * 8 + 2 * (lane & 3)]);
+    const float f0 = gain * rn[row], f1 = gain * rn[row + 8];
+    scale2(m[u], mul2(rk, pack2(f0, f0)));
+    scale2(m[u] + 2, mul2(rk, pack2(f1, f1)));
+  }
   for (int e0 = 0; e0 < group; e0 += 2) {
     if (e0) {  // the two images have left
       if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       make_gates(e0);
+      __syncthreads();
     }
-    __syncthreads();  // gates, norms
     for (int e = 0; e < 2 && e0 + e < group; ++e) {
       CkImage& img = sm.img[e];
       const float *g_hi = sm.g_hi[e], *g_lo = sm.g_lo[e], *gbeta = sm.gbeta[e];
@@ -351,65 +369,70 @@ __global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __g
         img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
         if (gt == 0) img.total = ex2_approx(ch + cl);
       }
+      // the rows of the three blocks that this thread's units lie in
+      float rh[3][2], rl[3][2], rb[3][2];
 #pragma unroll
-      for (int u = 0; u < 5; ++u) {
-        const int rb = u < 2 ? warp : (u < 4 ? (warp == 1 ? warp : rb2) : rb2);
-        const int row0 = rb * 16 + (lane >> 2), col = unit_tile[u] * 8 + 2 * (lane & 3);
-        const uint32_t block = ck_block(rb, unit_tile[u] >> 1);
-        const float2 gh = *reinterpret_cast<const float2*>(&g_hi[col]), gl = *reinterpret_cast<const float2*>(&g_lo[col]),
-                     rk = *reinterpret_cast<const float2*>(&sm.rk[col]);
+      for (int k = 0; k < 3; ++k)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const int row = row0 + 8 * hf;
-          const float rh = g_hi[row], rl = g_lo[row], f = of_q ? sm.rq[row] : -gbeta[row] * sm.rk[row];
-          float x0 = ex2_approx((rh - gh.x) + (rl - gl.x)) * rk.x * f * m[u][2 * hf];
-          float x1 = ex2_approx((rh - gh.y) + (rl - gl.y)) * rk.y * f * m[u][2 * hf + 1];
+          const int row = (k == 0 ? warp : (k == 1 ? rbm : rb2)) * 16 + (lane >> 2) + 8 * hf;
+          rh[k][hf] = g_hi[row], rl[k][hf] = g_lo[row], rb[k][hf] = of_q ? 1.f : gbeta[row];
+        }
+      const uint64_t minus = pack2(-1.f, -1.f);
+#pragma unroll
+      for (int u = 0; u < 5; ++u) {
+        const int k = u < 2 ? 0 : (u < 4 ? 1 : 2), block_row = k == 0 ? warp : (k == 1 ? rbm : rb2);
+        const int col = unit_tile[u] * 8 + 2 * (lane & 3);
+        const uint64_t gh = pair_at(&g_hi[col]), gl = pair_at(&g_lo[col]);
+        // (rows r and r + 8 have their halves in the same order)
+        const uint32_t at = ck_block(block_row, unit_tile[u] >> 1) + ck_in_block(lane >> 2, unit_tile[u] & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float2 d = unpack2(add2(fma2(gh, minus, pack2(rh[k][hf], rh[k][hf])), fma2(gl, minus, pack2(rl[k][hf], rl[k][hf]))));
+          const uint64_t f = of_q ? pack2(m[u][2 * hf], m[u][2 * hf + 1]) : mul2(pack2(m[u][2 * hf], m[u][2 * hf + 1]), pack2(rb[k][hf], rb[k][hf]));
+          float2 x = unpack2(mul2(pack2(ex2_approx(d.x), ex2_approx(d.y)), f));
           if (u < 2) {  // diagonal block: above the diagonal the exponentials may be anything
-            const int last = of_q ? row : row - 1;
-            x0 = col <= last ? x0 : 0.f;
-            x1 = col < last ? x1 : 0.f;
+            const int row = (lane >> 2) + 8 * hf, c = (unit_tile[u] & 1) * 8 + 2 * (lane & 3), last = of_q ? row : row - 1;
+            x.x = c <= last ? x.x : 0.f;
+            x.y = c < last ? x.y : 0.f;
+            if (!of_q) *reinterpret_cast<float2*>(&sm.a[e][(warp * 16 + row) * CD_LDA + c]) = x;
           }
-          if (u < 2 && !of_q) {
-            *reinterpret_cast<float2*>(&sm.a[row * CD_LDA + (col & 15)]) = make_float2(x0, x1);
-          } else {
+          if (u >= 2 || of_q) {
             uint32_t wh, wl;
-            split_f16x2(x0, x1, wh, wl);
-            const uint32_t at = block + ck_in_block(row & 15, unit_tile[u] & 1) + 4 * (lane & 3);
-            *reinterpret_cast<uint32_t*>((of_q ? img.p_hi : img.t_hi) + at) = wh;
-            *reinterpret_cast<uint32_t*>((of_q ? img.p_lo : img.t_lo) + at) = wl;
+            split_f16x2(x.x, x.y, wh, wl);
+            *reinterpret_cast<uint32_t*>((of_q ? img.p_hi : img.t_hi) + at + hf * 256) = wh;
+            *reinterpret_cast<uint32_t*>((of_q ? img.p_lo : img.t_lo) + at + hf * 256) = wl;
           }
         }
       }
-      if (!of_q) {
-        __syncwarp();
-        // the warp's diagonal block of I + A (sm.a holds -A) inverted by substitution, lane = column (both
-        // halves of the warp alike)
-        const float* ad = sm.a + warp * 16 * CD_LDA;
-        const int cl = lane & 15;
-        float x[16];
+    }
+    if (!of_q) {
+      __syncwarp();
+      // the warp's diagonal blocks of I + A (sm.a holds -A) inverted by substitution: half a warp a head, lane = column
+      const int e = lane >> 4, cl = lane & 15;
+      const float* ad = sm.a[e] + warp * 16 * CD_LDA;
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float s[4] = {i == cl ? 1.f : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < i; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(&ad[i * CD_LDA + j]);
+          s[0] += v.x * x[j];
+          if (j + 1 < i) s[1] += v.y * x[j + 1];
+          if (j + 2 < i) s[2] += v.z * x[j + 2];
+          if (j + 3 < i) s[3] += v.w * x[j + 3];
+        }
+        x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+      }
+      if (e0 + e < group)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float s0 = i == cl ? 1.f : 0.f, s1 = 0.f;
-#pragma unroll
-          for (int j = 0; j < i; ++j) {
-            if (j & 1)
-              s1 += ad[i * CD_LDA + j] * x[j];
-            else
-              s0 += ad[i * CD_LDA + j] * x[j];
-          }
-          x[i] = s0 + s1;
+          const __half vh = __float2half_rn(x[i]);
+          const uint32_t at = ck_block(warp, warp) + ck_in_block(i, cl >> 3) + 2 * (cl & 7);
+          *reinterpret_cast<__half*>(sm.img[e].t_hi + at) = vh;
+          *reinterpret_cast<__half*>(sm.img[e].t_lo + at) = __float2half_rn(x[i] - __half2float(vh));
         }
-        // rows of the first half by lanes 0..15, of the second by the others
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = lane < 16 ? x[i] : x[8 + i];
-          const __half vh = __float2half_rn(v);
-          const uint32_t at = ck_block(warp, warp) + ck_in_block(i + (lane < 16 ? 0 : 8), cl >> 3) + 2 * (cl & 7);
-          *reinterpret_cast<__half*>(img.t_hi + at) = vh;
-          *reinterpret_cast<__half*>(img.t_lo + at) = __float2half_rn(v - __half2float(vh));
-        }
-      }
-      __syncwarp();  // sm.a is the warp's own
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
@@ -455,9 +478,6 @@ struct CsSmem {
   uint64_t full[CS_STAGES], empty[CS_STAGES];
 };
 static_assert(sizeof(CsSmem<8, 1>) + 1024 <= MAX_DYN_SMEM && sizeof(CsSmem<4, 2>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
-
-// Two neighbouring floats of a factor
-__device__ __forceinline__ uint64_t pair_at(const float* p) { return *reinterpret_cast<const uint64_t*>(p); }
 
 __device__ __forceinline__ void plus4(float* x, const float4& y) {
   const float2 a = unpack2(add2(pack2(x[0], x[1]), pack2(y.x, y.y))), b = unpack2(add2(pack2(x[2], x[3]), pack2(y.z, y.w)));
@@ -827,7 +847,7 @@ cudaError_t scan(const PrefillParams& p, const CUtensorMap& map, cudaStream_t st
 
 }  // namespace
 
-cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream) {
+cudaError_t launch_prefill_chunk(const PrefillParams& p, int64_t longest, cudaStream_t stream) {
   CUtensorMap map;
   // boxes of 64 columns x 64 tokens of mixed_qkv
   const uint64_t dims[2] = {uint64_t(2 * p.H + p.HV) * 128, uint64_t(p.T)};
@@ -843,16 +863,24 @@ cudaError_t launch_prefill_chunk(const PrefillParams& p, cudaStream_t stream) {
   prefill_derive_kernel<<<dim3(unsigned(ids * p.H)), CD_THREADS, bytes, stream>>>(p, map);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (p.N * int64_t(p.HV) * 4 <= multiprocessor_count()) return scan<4, 2>(p, map, stream);
-  if (p.N * int64_t(p.HV) * 2 <= multiprocessor_count()) return scan<4, 1>(p, map, stream);
-  return scan<8, 1>(p, map, stream);
+  // Three ways to put a head's value rows on multiprocessors: all 128 on one (7 us a chunk), 64 (3 to 4 us), or
+  // 32 with their key columns halved (2.8 us, 12 us of multiprocessor time a head's chunk).  What takes longest is the
+  // chunks of all sequences, spread over the machine, or those of the longest one after another: one
+  // prompt of 8192 tokens 0.85 ms / 0.51 ms / 0.42 ms, eight of 2048 tokens 0.55 ms / 0.59 ms / 0.77 ms.
+  const int64_t chain = (longest + CK_C - 1) / CK_C, all = ids * p.HV / multiprocessor_count();
+  const int64_t t8 = std::max(all * 72, chain * 66), t4 = std::max(all * 80, chain * 31), t2 = std::max(all * 120, chain * 28);
+  if (t2 < t4 && t2 < t8) return scan<4, 2>(p, map, stream);
+  return t4 < t8 ? scan<4, 1>(p, map, stream) : scan<8, 1>(p, map, stream);
 }
 
 // The longest sequence as the host knows it, or the mean length
-static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) {
-  const int64_t longest = max_seqlen > 0 ? max_seqlen : (tokens + sequences - 1) / sequences;
-  return longest > 8;
+static int64_t longest_of(int64_t tokens, int64_t sequences, int max_seqlen) {
+  return max_seqlen > 0 ? std::min<int64_t>(max_seqlen, tokens) : (tokens + sequences - 1) / sequences;
 }
+
+// A token takes the token-by-token kernel 1.5 us where all CTAs run at once and 20 us at 64 sequences of 32 heads; a chunk
+// takes the other two kernels 27 us and 250 us: equal at some twelve tokens.
+static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 12; }
 
 int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen) {
   if (sequences <= 0 || tokens <= 0 || !prefill_chunked(tokens, sequences, max_seqlen)) return 0;
@@ -861,7 +889,7 @@ int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value
 
 cudaError_t launch_prefill(const PrefillParams& p, int max_seqlen, cudaStream_t stream) {
   if (p.T == 0 || !prefill_chunked(p.T, p.N, max_seqlen)) return launch_prefill_recurrent(p, stream);
-  return launch_prefill_chunk(p, stream);
+  return launch_prefill_chunk(p, longest_of(p.T, p.N, max_seqlen), stream);
 }
 
 cudaError_t launch_prefill_recurrent(const PrefillParams& p, cudaStream_t stream) {
