@@ -202,8 +202,12 @@ constexpr int CD_THREADS = 256;
 constexpr int CD_LDA = 20;  // floats of a row of a diagonal block
 
 struct CdSmem {
-  uint8_t k[CK_C * 256], q[CK_C * 256];
-  CkImage img[2];
+  union {
+    struct {
+      uint8_t k[CK_C * 256], q[CK_C * 256];
+    };
+    CkImage img[2];  // once the products are in registers
+  };
   float a[2][CK_C * CD_LDA];  // -A's diagonal blocks of two heads: warp w's at rows 16 w
   float g_hi[2][CK_C], g_lo[2][CK_C], gbeta[2][CK_C];  // prefix sums of the gates in units of ln 2, in two parts
   float rk[CK_C], rq[CK_C];
@@ -213,7 +217,7 @@ struct CdSmem {
 // One CTA a chunk and key head; its value heads share the products of the raw rows.  The first
 // four warps make A (rows of K against K) and invert its diagonal blocks, the others make P
 // (rows of Q against K) and the factors.
-__global__ void __launch_bounds__(CD_THREADS, 2) prefill_derive_kernel(const __grid_constant__ PrefillParams p,
+__global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __grid_constant__ PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
   CdSmem& sm = *reinterpret_cast<CdSmem*>(raw + (-smem_addr(raw) & 1023u));
