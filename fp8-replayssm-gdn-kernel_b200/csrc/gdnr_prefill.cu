@@ -22,12 +22,15 @@ __device__ __forceinline__ float sigmoid_f(float x) { return 1.0f / (1.0f + expf
 // ---------------------------------------------------------------- recurrent form
 // One warp owns 8 value rows of S in registers (lane: 4 key columns of each), a CTA 32
 // rows, so a head is four CTAs and a batch of single tokens reads and writes each state
-// once, in 512-byte row pieces.  S k and S q are both taken from the state before the
-// update (o = e^g S q + d (k.q)), so a token has one chain of shuffles.  The sums of 8 rows
-// over 32 lanes are folded together: 4 + 2 + 1 exchanges halve the rows a lane holds,
-// 2 more finish the sum, 9 shuffles instead of 40.
+// once, in 512-byte row pieces.  What does not depend on the state (inverse norms, q.k, gates) is
+// made for up to 16 tokens at a time, the tokens shared by the warps, so that a token
+// costs its own chain only: S k and S q, both from the state before the update
+// (o = e^g S q + d (k.q)), one chain of shuffles, the update.  The sums of 8 rows over 32 lanes are
+// folded together: 4 + 2 + 1 exchanges halve the rows a lane holds, 2 more finish the
+// sum, 9 shuffles instead of 40.
 constexpr int RC_ROWS = 8;
 constexpr int RC_WARPS = 4;
+constexpr int RC_BLOCK = 16;
 
 // Sum over the warp of x[r], r = 0..7; lane l gets row (l >> 2).
 __device__ __forceinline__ float fold8(const float* x, int lane) {
@@ -50,29 +53,19 @@ __device__ __forceinline__ float fold8(const float* x, int lane) {
   return s;
 }
 
-struct RcToken {
-  uint2 q, k;
-  uint16_t v;
-  float a, b;
+struct RcSmem {
+  uint2 q[RC_BLOCK][32], k[RC_BLOCK][32];  // raw rows, a lane's four elements
+  uint16_t v[RC_BLOCK][RC_ROWS * RC_WARPS];
+  float alpha[RC_BLOCK], beta[RC_BLOCK], rk[RC_BLOCK], rq[RC_BLOCK], qk[RC_BLOCK];
 };
 
-__device__ __forceinline__ RcToken rc_load(const PrefillParams& p, int t, int h, int hv, int row, int lane) {
-  RcToken x;
-  const uint16_t* m = p.mixed + int64_t(t) * p.mx_s;
-  x.q = *reinterpret_cast<const uint2*>(m + h * 128 + lane * 4);
-  x.k = *reinterpret_cast<const uint2*>(m + (p.H + h) * 128 + lane * 4);
-  x.v = m[(2 * p.H + hv) * 128 + row];
-  x.a = load_scalar(p.a, int64_t(t) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt);
-  x.b = load_scalar(p.b, int64_t(t) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt);
-  return x;
-}
-
 __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const __grid_constant__ PrefillParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ RcSmem sm;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int PARTS = 128 / (RC_ROWS * RC_WARPS);
   const int part = blockIdx.x % PARTS, nh = blockIdx.x / PARTS;
   const int n = nh / p.HV, hv = nh - n * p.HV, h = hv / (p.HV / p.H);
-  const int row0 = part * (RC_ROWS * RC_WARPS) + warp * RC_ROWS;
+  const int part0 = part * (RC_ROWS * RC_WARPS), row0 = part0 + warp * RC_ROWS;
   const int my_row = row0 + (lane >> 2);
   const SeqRange r = prefill_seq(p, n);
   if (r.slot < 0) {
@@ -87,42 +80,62 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 #pragma unroll
   for (int i = 0; i < RC_ROWS; ++i)
     S[i] = fresh ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(st + i * 128);
-  const float neg_a = -expf(p.a_log[hv * p.al_s]), dtb = p.dt_bias[hv * p.db_s];
-  RcToken nx = {};
-  if (r.begin < r.end) nx = rc_load(p, r.begin, h, hv, my_row, lane);
-  for (int t = r.begin; t < r.end; ++t) {
-    const RcToken x = nx;
-    if (t + 1 < r.end) nx = rc_load(p, t + 1, h, hv, my_row, lane);
-    const float2 q01 = bf16x2_to_f2(x.q.x), q23 = bf16x2_to_f2(x.q.y), k01 = bf16x2_to_f2(x.k.x), k23 = bf16x2_to_f2(x.k.y);
-    float qq = q01.x * q01.x + q01.y * q01.y + q23.x * q23.x + q23.y * q23.y;
-    float kk = k01.x * k01.x + k01.y * k01.y + k23.x * k23.x + k23.y * k23.y;
-    float qk = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
-    float sk[RC_ROWS], sq[RC_ROWS];
-#pragma unroll
-    for (int i = 0; i < RC_ROWS; ++i) {
-      sk[i] = S[i].x * k01.x + S[i].y * k01.y + S[i].z * k23.x + S[i].w * k23.y;
-      sq[i] = S[i].x * q01.x + S[i].y * q01.y + S[i].z * q23.x + S[i].w * q23.y;
+  for (int t0 = r.begin; t0 < r.end; t0 += RC_BLOCK) {
+    const int count = min(RC_BLOCK, r.end - t0);
+    if (t0 > r.begin) __syncthreads();  // the block before has been used
+    if (tid >= 64 && tid < 64 + count) {  // gates: a thread a token
+      const int i = tid - 64, t = t0 + i;
+      const float a = load_scalar(p.a, int64_t(t) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt) + p.dt_bias[hv * p.db_s];
+      const float b = load_scalar(p.b, int64_t(t) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt);
+      sm.alpha[i] = expf(-expf(p.a_log[hv * p.al_s]) * softplus_gate(a));
+      sm.beta[i] = sigmoid_f(b);
     }
-    const float g = neg_a * softplus_gate(x.a + dtb), alpha = expf(g), beta = sigmoid_f(x.b);
+    for (int i = warp; i < count; i += RC_WARPS) {
+      const uint16_t* m = p.mixed + int64_t(t0 + i) * p.mx_s;
+      const uint2 q = *reinterpret_cast<const uint2*>(m + h * 128 + lane * 4), k = *reinterpret_cast<const uint2*>(m + (p.H + h) * 128 + lane * 4);
+      sm.v[i][lane] = m[(2 * p.H + hv) * 128 + part0 + lane];
+      sm.q[i][lane] = q;
+      sm.k[i][lane] = k;
+      const float2 q01 = bf16x2_to_f2(q.x), q23 = bf16x2_to_f2(q.y), k01 = bf16x2_to_f2(k.x), k23 = bf16x2_to_f2(k.y);
+      float qq = q01.x * q01.x + q01.y * q01.y + q23.x * q23.x + q23.y * q23.y;
+      float kk = k01.x * k01.x + k01.y * k01.y + k23.x * k23.x + k23.y * k23.y;
+      float qk = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      qq += __shfl_xor_sync(0xffffffffu, qq, o);
-      kk += __shfl_xor_sync(0xffffffffu, kk, o);
-      qk += __shfl_xor_sync(0xffffffffu, qk, o);
+      for (int o = 16; o > 0; o >>= 1) {
+        qq += __shfl_xor_sync(0xffffffffu, qq, o);
+        kk += __shfl_xor_sync(0xffffffffu, kk, o);
+        qk += __shfl_xor_sync(0xffffffffu, qk, o);
+      }
+      if (lane == 0) {
+        const float rk = rsqrtf(kk + L2_EPS), rq = 0.08838834764831845f * rsqrtf(qq + L2_EPS);
+        sm.rk[i] = rk, sm.rq[i] = rq, sm.qk[i] = qk * rk * rq;
+      }
     }
-    const float rk = 1.0f / sqrtf(kk + L2_EPS), rq = 0.08838834764831845f / sqrtf(qq + L2_EPS);
-    const float my_sk = fold8(sk, lane) * rk, my_sq = fold8(sq, lane) * rq;
-    const float d = beta * (bf16_to_f(x.v) - alpha * my_sk);
-    if ((lane & 3) == 0)
-      p.out[int64_t(t) * p.o_st + int64_t(hv) * p.o_sh + my_row] = f_to_bf16(alpha * my_sq + d * (qk * rk * rq));
-    const float dk = d * rk;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      const uint2 q = sm.q[i][lane], k = sm.k[i][lane];
+      const float2 q01 = bf16x2_to_f2(q.x), q23 = bf16x2_to_f2(q.y), k01 = bf16x2_to_f2(k.x), k23 = bf16x2_to_f2(k.y);
+      float sk[RC_ROWS], sq[RC_ROWS];
 #pragma unroll
-    for (int i = 0; i < RC_ROWS; ++i) {
-      const float di = __shfl_sync(0xffffffffu, dk, i * 4);
-      S[i].x = alpha * S[i].x + di * k01.x;
-      S[i].y = alpha * S[i].y + di * k01.y;
-      S[i].z = alpha * S[i].z + di * k23.x;
-      S[i].w = alpha * S[i].w + di * k23.y;
+      for (int j = 0; j < RC_ROWS; ++j) {
+        sk[j] = S[j].x * k01.x + S[j].y * k01.y + S[j].z * k23.x + S[j].w * k23.y;
+        sq[j] = S[j].x * q01.x + S[j].y * q01.y + S[j].z * q23.x + S[j].w * q23.y;
+      }
+      const float alpha = sm.alpha[i], rk = sm.rk[i];
+      const float my_sk = fold8(sk, lane), my_sq = fold8(sq, lane);
+      const float d = sm.beta[i] * (bf16_to_f(sm.v[i][warp * RC_ROWS + (lane >> 2)]) - alpha * rk * my_sk);
+      if ((lane & 3) == 0)
+        p.out[int64_t(t0 + i) * p.o_st + int64_t(hv) * p.o_sh + my_row] = f_to_bf16(alpha * sm.rq[i] * my_sq + d * sm.qk[i]);
+      const float dk = d * rk;
+#pragma unroll
+      for (int j = 0; j < RC_ROWS; ++j) {
+        const float dj = __shfl_sync(0xffffffffu, dk, j * 4);
+        S[j].x = alpha * S[j].x + dj * k01.x;
+        S[j].y = alpha * S[j].y + dj * k01.y;
+        S[j].z = alpha * S[j].z + dj * k23.x;
+        S[j].w = alpha * S[j].w + dj * k23.y;
+      }
     }
   }
 #pragma unroll
@@ -882,9 +895,9 @@ static int64_t longest_of(int64_t tokens, int64_t sequences, int max_seqlen) {
   return max_seqlen > 0 ? std::min<int64_t>(max_seqlen, tokens) : (tokens + sequences - 1) / sequences;
 }
 
-// A token takes the token-by-token kernel 1.5 us where all CTAs run at once and 20 us at 64 sequences of 32 heads; a chunk
-// takes the other two kernels 27 us and 250 us: equal at some twelve tokens.
-static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 12; }
+// At 64 sequences of 32 heads a token takes the token-by-token kernel 9 us (135 us at twelve), a chunk the other two
+// 235 us; at one sequence 0.3 us and 18 us a call: equal at some two dozen tokens.
+static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 24; }
 
 int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen) {
   if (sequences <= 0 || tokens <= 0 || !prefill_chunked(tokens, sequences, max_seqlen)) return 0;
