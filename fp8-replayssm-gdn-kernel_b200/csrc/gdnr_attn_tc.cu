@@ -40,16 +40,19 @@ struct TcCfg {
   static_assert(SMEM + 512 <= 227 * 1024, "one CTA per SM");
 };
 
-__device__ __forceinline__ uint64_t tc_desc_k(uint32_t addr) {  // rows of 128 bytes, 128-byte swizzle, K contiguous
-  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
-}
+// Matrix descriptors, the low words (the start address is added, in units of 16 bytes): 128-byte swizzle, groups of eight rows
+// 1024 bytes apart.  Rows of 128 bytes with K along them: the other distance is not used.  Rows of 128 bytes (64
+// elements of N) with K across them: column blocks `lbo` bytes apart.
+__host__ __device__ constexpr uint32_t tc_low_k() { return 1u << 16; }
+__host__ __device__ constexpr uint32_t tc_low_mn(uint32_t lbo) { return (lbo >> 4) << 16; }
+constexpr uint32_t TC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
 
-// K in rows of 128 bytes (64 elements of N), 128-byte swizzle: groups of eight rows 1024 bytes apart, column blocks
-// `lbo` bytes apart
-__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr, uint32_t lbo) {
-  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// One lane of a whole warp.  (With a branch on the lane number instead, the compiler moves every operand of an
+// instruction that wants uniform registers there one by one: 58 ns a product against 36.)
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // f32 accumulator, bf16 operands, M = 128; B with N contiguous where `bn`
@@ -57,19 +60,20 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool bn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (bn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// acc 0: d = a b, else d += a b
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .b64 da, db;\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(TC_HIGH)
       : "memory");
 }
 
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .b64 db;\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(TC_HIGH)
       : "memory");
 }
 
@@ -259,18 +263,18 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
     auto kv_wait = [&](uint32_t k) { return wait(&bars.kv_full[k % C::RING], (k / C::RING) & 1); };
     auto kv_addr = [&](uint32_t k) { return kv_base + (k % C::RING) * C::KV_BYTES; };
     auto score = [&](int q, int buf, uint32_t k, bool last) {  // S[buf] = Q_q K^T
+      const uint32_t lq = tc_low_k() + ((base + q * C::Q_BYTES) >> 4), lk = tc_low_k() + (kv_addr(k) >> 4), to = tmem + buf * C::S_COLS;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
-        tc_mma_ss(tmem + buf * C::S_COLS, tc_desc_k(base + q * C::Q_BYTES + (i >> 2) * 16384 + (i & 3) * 32),
-                  tc_desc_k(kv_addr(k) + (i >> 2) * (BN * 128) + (i & 3) * 32), QK, i > 0);
+        tc_mma_ss(to, lq + (i >> 2) * 1024 + (i & 3) * 2, lk + (i >> 2) * (BN * 8) + (i & 3) * 2, QK, i > 0);
       tc_commit(&bars.s_full[buf]);
       if (last) tc_commit(&bars.q_free[q]);
     };
     auto weigh = [&](int q, int buf, uint32_t k, bool first, bool last) {  // O_q += P[buf] V
+      const uint32_t lv = tc_low_mn(BN * 128) + (kv_addr(k) >> 4), from = tmem + buf * C::S_COLS;
 #pragma unroll
       for (int i = 0; i < BN / 16; ++i)
-        tc_mma_ts(tmem + C::O_COL + q * D, tmem + buf * C::S_COLS + i * 8, tc_desc_mn(kv_addr(k) + i * 2048, BN * 128), PV,
-                  !first || i > 0);
+        tc_mma_ts(tmem + C::O_COL + q * D, from + i * 8, lv + i * 128, PV, !first || i > 0);
       if (NQ == 1) tc_commit(&bars.o_full);
       if (last) tc_commit(&bars.done[q]);
     };
@@ -298,12 +302,12 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         __syncwarp();
       };
       auto free_slot = [&](uint32_t k) {
-        if (lane == 0) tc_commit(&bars.kv_empty[k % C::RING]);
+        if (tc_elect()) tc_commit(&bars.kv_empty[k % C::RING]);
       };
       if constexpr (NQ == 2) {
         // S0(t), S1(t); then for each stream P(t) V(t) and S(t + 1)
         if (ok) ok = kv_wait(k0);
-        if (ok && lane == 0)
+        if (ok && tc_elect())
           for (int q = 0; q < 2; ++q)
             if (end[q] > t0) score(q, q, k0, t0 + 1 == end[q]);
         free_slot(k0);
@@ -318,11 +322,11 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
             ok = wait(&bars.p_full[q], np[q]++ & 1);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) weigh(q, q, kv, t == t0, t + 1 == end[q]);
+            if (tc_elect()) weigh(q, q, kv, t == t0, t + 1 == end[q]);
             if (t + 1 < end[q]) {
               if (!have_k) ok = kv_wait(kk), have_k = true;
               if (!ok) break;
-              if (lane == 0) score(q, q, kk, t + 2 == end[q]);
+              if (tc_elect()) score(q, q, kk, t + 2 == end[q]);
             }
             __syncwarp();
           }
@@ -332,15 +336,16 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       } else {
         // S(t + 1) is issued before P(t) V(t), into the other buffer
         if (ok) ok = kv_wait(k0);
-        if (ok && lane == 0) score(0, t0 & 1, k0, t0 + 1 == last);
+        if (ok && tc_elect()) score(0, t0 & 1, k0, t0 + 1 == last);
         free_slot(k0);
         for (int t = t0; t < last && ok; ++t) {
           const uint32_t kk = k0 + 2 * (t + 1 - t0), kv = k0 + 2 * (t - t0) + 1;
           if (t + 1 < last) {
             ok = kv_wait(kk);
             if (!ok) break;
-            if (lane == 0) score(0, (t + 1) & 1, kk, t + 2 == last);
+            if (tc_elect()) score(0, (t + 1) & 1, kk, t + 2 == last);
             __syncwarp();
+            free_slot(kk);
           }
           ok = kv_wait(kv);
           if (!ok) break;
@@ -348,10 +353,9 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
           ok = wait(&bars.p_full[t & 1], np[t & 1]++ & 1);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) weigh(0, t & 1, kv, t == t0, t + 1 == last);
+          if (tc_elect()) weigh(0, t & 1, kv, t == t0, t + 1 == last);
           __syncwarp();
           free_slot(kv);
-          if (t + 1 < last) free_slot(kk);
         }
       }
       slot = k0 + 2 * (last - t0);
