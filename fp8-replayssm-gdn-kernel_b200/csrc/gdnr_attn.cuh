@@ -64,7 +64,7 @@ __device__ __forceinline__ int unit_tiles(const AttnParams& p, const SeqLen& s, 
 // keep a single lane busy.
 __device__ __forceinline__ int lanes_per_seq(int n) { return n >= 32 ? 1 : (n > 16 ? 1 : (n > 8 ? 2 : (n > 4 ? 4 : (n > 2 ? 8 : (n > 1 ? 16 : 32))))); }
 
-// Places of sequence n (0 past the last), in each of its `per` lanes.
+// Places of one head of sequence n (0 past the last), in each of its `per` lanes.
 template <class T>
 __device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const AtRows& r, int n, int per, int lane) {
   int64_t sum = 0;
@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const AtRows& 
     for (int rt = lane & (per - 1); rt < rts; rt += per) sum += T::OVER + unit_tiles<T>(p, s, rt);
   }
   for (int o = per >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * p.Hk;
+  return sum;
 }
 
 // Places of the batch (one whole warp).
@@ -84,7 +84,7 @@ __device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& 
   int64_t w = 0;
   for (int n0 = 0; n0 < p.N; n0 += step) {
     const int64_t x = seq_tiles<T>(p, r, n0 + lane / per, per, lane);
-    if ((lane & (per - 1)) == 0) w += x;
+    if ((lane & (per - 1)) == 0) w += x * p.Hk;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
@@ -107,7 +107,7 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
   u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
   u.s.q0 = u.s.m = u.s.kv = 0;
   for (int n0 = 0; n0 < p.N; n0 += step) {
-    const int64_t w = seq_tiles<T>(p, r, n0 + lane / per, per, lane);
+    const int64_t head = seq_tiles<T>(p, r, n0 + lane / per, per, lane), w = head * p.Hk;
     int64_t pre = w;
     for (int o = per; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
@@ -119,10 +119,15 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
       int64_t start = base + __shfl_sync(0xffffffffu, pre - w, src);
       u.n = n0 + src / per;
       u.s = seq_len(p, u.n, r);
-      const int64_t per_head = __shfl_sync(0xffffffffu, w, src) / p.Hk;
-      u.h = int((at - start) / per_head);
+      const int64_t per_head = __shfl_sync(0xffffffffu, head, src);
+      u.h = at - start < INT32_MAX ? int(uint32_t(at - start) / uint32_t(min(per_head, int64_t(INT32_MAX)))) : int((at - start) / per_head);
       start += u.h * per_head;
       const int rts = (u.s.m * p.G + T::BM - 1) / T::BM;
+      if (rts == 1) {
+        u.tiles = int(per_head) - T::OVER;
+        u.begin = start;
+        return u;
+      }
       for (int rt0 = 0; rt0 < rts; rt0 += 32) {
         const int mine = rt0 + lane < rts ? T::OVER + unit_tiles<T>(p, u.s, rt0 + lane) : 0;
         int sum = mine;
