@@ -37,25 +37,26 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
   using T = AtTile<C::BM, AT_BN, 1>;
   constexpr int BM = C::BM, ROWB = C::ROWB, CH = ROWB / 16, NT = AT_BN / WN / 8;  // NT: 8-key tiles of a warp
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sh_total;
+  constexpr int WARPS = WM * WN;
+  __shared__ int64_t sh_places[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wm = warp / WN, wn = warp % WN;
   const uint32_t q_s = smem_addr(smem), kv_s = q_s + C::Q_BYTES;
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
-  if (warp == 0) {
-    const int64_t w = all_tiles<T>(p, of, lane);
-    if (lane == 0) sh_total = w;
-  }
+  const int64_t places = warp_places<T>(p, of, warp, WARPS, lane);
+  if (lane == 0) sh_places[warp] = places;
   __syncthreads();
-  const int64_t total = sh_total;
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) total += sh_places[w];
   const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   if (share.begin >= share.end) {
     if (tid == 0) meta[0] = -1;
     return;
   }
-  Unit u = find_unit<T>(p, of, share.begin, lane);
+  Unit u = find_unit<T>(p, of, share.begin, sh_places, WARPS, lane);
   if (tid == 0) write_meta<T>(meta, share, u, total, gridDim.x);
   const float sl2 = p.scale * LOG2E;
   for (int64_t at = share.begin; at < share.end; next_unit<T>(p, of, u), at = u.begin) {
@@ -282,7 +283,7 @@ struct AsCfg {
 
 struct AsShared {
   uint64_t full[8], empty[8];
-  int64_t total;
+  int64_t places[5];
   int abort;
   float ml[4][16][2];  // maximum and sum of the rows of each warp's keys
 };
@@ -307,10 +308,11 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
-  if (warp == 0) {
-    const int64_t w = all_tiles<T>(p, of, lane);
-    if (lane == 0) sh.total = w;
-  } else if (tid == 32) {
+  constexpr int WARPS = WM * WN + 1;
+  static_assert(WARPS == 5, "AsShared::places");
+  const int64_t places = warp_places<T>(p, of, warp, WARPS, lane);
+  if (lane == 0) sh.places[warp] = places;
+  if (tid == 32) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], WM * WN);
@@ -319,14 +321,16 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
     fence_mbar_init();
   }
   __syncthreads();
-  const int64_t total = sh.total;
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) total += sh.places[w];
   const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   if (share.begin >= share.end) {
     if (tid == 0) meta[0] = -1;
     return;
   }
   const WarpWait wait{p.err, &sh.abort};
-  Unit u = find_unit<T>(p, of, share.begin, lane);
+  Unit u = find_unit<T>(p, of, share.begin, sh.places, WARPS, lane);
   uint32_t k = 0;  // tiles requested or consumed so far
   bool ok = true;
 

@@ -77,13 +77,19 @@ __device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const AtRows& 
   return sum;
 }
 
-// Places of the batch (one whole warp).
+// The warps of a CTA count the batch's places together: warp w the sequences [w per, (w + 1) per), all of a short batch
+// by the first.
+__device__ __forceinline__ int seqs_per_warp(const AttnParams& p, int warps) { return p.N <= 32 ? p.N : (p.N + warps - 1) / warps; }
+
+// Places of a warp's sequences.
 template <class T>
-__device__ __forceinline__ int64_t all_tiles(const AttnParams& p, const AtRows& r, int lane) {
-  const int per = lanes_per_seq(p.N), step = 32 / per;
+__device__ __forceinline__ int64_t warp_places(const AttnParams& p, const AtRows& r, int warp, int warps, int lane) {
+  const int first = warp * seqs_per_warp(p, warps), last = min(first + seqs_per_warp(p, warps), p.N);
+  const int per = lanes_per_seq(last - first), step = 32 / per;
   int64_t w = 0;
-  for (int n0 = 0; n0 < p.N; n0 += step) {
-    const int64_t x = seq_tiles<T>(p, r, n0 + lane / per, per, lane);
+  for (int n0 = first; n0 < last; n0 += step) {
+    const int n = n0 + lane / per;
+    const int64_t x = seq_tiles<T>(p, r, n < last ? n : p.N, per, lane);
     if ((lane & (per - 1)) == 0) w += x * p.Hk;
   }
 #pragma unroll
@@ -98,16 +104,20 @@ struct Unit {
   int tiles;
 };
 
-// The unit that place `at` of the batch falls into (one whole warp).
+// The unit that place `at` of the batch falls into (one whole warp); places: every warp's, as warp_places counts them.
 template <class T>
-__device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, int64_t at, int lane) {
-  const int per = lanes_per_seq(p.N), step = 32 / per;
+__device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, int64_t at, const int64_t* places, int warps, int lane) {
   int64_t base = 0;
+  int first = 0;
+  const int mine = seqs_per_warp(p, warps);
+  for (int w = 0; w + 1 < warps && base + places[w] <= at; ++w) base += places[w], first += mine;
+  const int last = min(first + mine, p.N), per = lanes_per_seq(last - first), step = 32 / per;
   Unit u;
   u.n = 0, u.h = 0, u.rt = 0, u.begin = 0, u.tiles = 0;
   u.s.q0 = u.s.m = u.s.kv = 0;
-  for (int n0 = 0; n0 < p.N; n0 += step) {
-    const int64_t head = seq_tiles<T>(p, r, n0 + lane / per, per, lane), w = head * p.Hk;
+  for (int n0 = first; n0 < last; n0 += step) {
+    const int n = n0 + lane / per;
+    const int64_t head = seq_tiles<T>(p, r, n < last ? n : p.N, per, lane), w = head * p.Hk;
     int64_t pre = w;
     for (int o = per; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
@@ -129,8 +139,8 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
         return u;
       }
       for (int rt0 = 0; rt0 < rts; rt0 += 32) {
-        const int mine = rt0 + lane < rts ? T::OVER + unit_tiles<T>(p, u.s, rt0 + lane) : 0;
-        int sum = mine;
+        const int own = rt0 + lane < rts ? T::OVER + unit_tiles<T>(p, u.s, rt0 + lane) : 0;
+        int sum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -140,8 +150,8 @@ __device__ __forceinline__ Unit find_unit(const AttnParams& p, const AtRows& r, 
         if (in) {
           const int l = __ffs(in) - 1;
           u.rt = rt0 + l;
-          u.tiles = __shfl_sync(0xffffffffu, mine, l) - T::OVER;
-          u.begin = start + __shfl_sync(0xffffffffu, sum - mine, l);
+          u.tiles = __shfl_sync(0xffffffffu, own, l) - T::OVER;
+          u.begin = start + __shfl_sync(0xffffffffu, sum - own, l);
           return u;
         }
         start += __shfl_sync(0xffffffffu, sum, 31);

@@ -143,7 +143,7 @@ struct TcBars {
   uint64_t done[2];     // matrix warp -> softmax warps: the stream's last PV of a unit is complete
   int abort;
   uint32_t tmem;
-  int64_t total;
+  int64_t places[12];
 };
 
 template <int D>
@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
-  if (warp == 0) {
-    const int64_t w = all_tiles<T>(p, of, lane);
-    if (lane == 0) bars.total = w;
-  } else if (warp == 1) {
+  constexpr int WARPS = C::THREADS / 32;
+  const int64_t places = warp_places<T>(p, of, warp, WARPS, lane);
+  if (lane == 0) bars.places[warp] = places;
+  if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bars.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (tid == 64) {
@@ -186,13 +186,16 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  const Share share = share_of<T>(bars.total, blockIdx.x, gridDim.x);
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) total += bars.places[w];
+  const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   const WarpWait wait{p.err, &bars.abort};
   Unit u;
   u.n = p.N;
   if (share.begin < share.end) {
-    u = find_unit<T>(p, of, share.begin, lane);
-    if (tid == 0) write_meta<T>(meta, share, u, bars.total, gridDim.x);
+    u = find_unit<T>(p, of, share.begin, bars.places, WARPS, lane);
+    if (tid == 0) write_meta<T>(meta, share, u, total, gridDim.x);
   } else if (tid == 0) {
     meta[0] = -1;
   }

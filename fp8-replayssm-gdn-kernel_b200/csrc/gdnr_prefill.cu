@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
       float g = 0.f, be = 0.f;
       if (t < valid) {
         g = neg_a * softplus_gate(load_scalar(p.a, int64_t(t0 + t) * p.a_st + int64_t(hv) * p.a_sh, p.a_dt) + dtb);
+        g = g < -1e4f ? -1e4f : g;  // e^g is 0 below; a sum with an infinity would have no differences
         be = sigmoid_f(load_scalar(p.b, int64_t(t0 + t) * p.b_st + int64_t(hv) * p.b_sh, p.b_dt));
       }
       x[i] = double(g);
@@ -532,25 +533,16 @@ __device__ __forceinline__ void ck_right(uint32_t tri, int i, int j, int lane, u
 }
 
 // The n-th sequence from the longest down, so that no long one starts last.  One
-// warp; batches above 256 sequences keep their order (the count grows with N^2).
-__device__ int ck_by_length(const PrefillParams& p, int want, int lane) {
-  if (p.N > 256) return want;
-  int found = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 32) {
-    const int n = n0 + lane;
-    int rank = -1;
-    if (n < p.N) {
-      const int len = p.cu[n + 1] - p.cu[n];
-      rank = 0;
-      for (int m = 0; m < p.N; ++m) {
-        const int other = p.cu[m + 1] - p.cu[m];
-        rank += other > len || (other == len && m < n);
-      }
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, rank == want);
-    if (hit) found = n0 + __ffs(hit) - 1;
+// warp, a lane a sequence; larger batches keep their order.
+__device__ __forceinline__ int ck_by_length(const PrefillParams& p, int want, int lane) {
+  if (p.N == 1 || p.N > 32) return want;
+  const int len = lane < p.N ? p.cu[lane + 1] - p.cu[lane] : -1;
+  int rank = 0;
+  for (int m = 0; m < p.N; ++m) {
+    const int other = __shfl_sync(0xffffffffu, len, m);
+    rank += other > len || (other == len && m < lane);
   }
-  return found;
+  return __ffs(__ballot_sync(0xffffffffu, lane < p.N && rank == want)) - 1;
 }
 
 // Column j of blocks of O += N P^T: rows of blocks 0 and 3 where `outer`, of 1 and 2 where `inner`
@@ -895,9 +887,9 @@ static int64_t longest_of(int64_t tokens, int64_t sequences, int max_seqlen) {
   return max_seqlen > 0 ? std::min<int64_t>(max_seqlen, tokens) : (tokens + sequences - 1) / sequences;
 }
 
-// At 64 sequences of 32 heads a token takes the token-by-token kernel 9 us (135 us at twelve), a chunk the other two
-// 235 us; at one sequence 0.3 us and 18 us a call: equal at some two dozen tokens.
-static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 24; }
+// At 64 sequences of 32 heads a token takes the token-by-token kernel 9 us (135 us at twelve), at 128 20 us; a chunk the other two
+// 235 us and 387 us: equal at about twenty tokens.  (One sequence: 0.3 us a token and 18 us a call.)
+static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 20; }
 
 int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen) {
   if (sequences <= 0 || tokens <= 0 || !prefill_chunked(tokens, sequences, max_seqlen)) return 0;

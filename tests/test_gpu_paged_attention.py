@@ -205,3 +205,12 @@ def test_lse_joins_two_halves_of_a_context(cuda_device):
     joined = o1.float() * (l1 - l).exp()[..., None] + o2.float() * (l2 - l).exp()[..., None]
     assert R.rel(joined, whole) < 2 * TOL_OUT
     assert math.isfinite(float(l.sum()))
+
+
+@pytest.mark.parametrize("n", [33, 200])
+def test_many_sequences(cuda_device, n):
+    """More sequences than a warp has lanes, single tokens and a few chunks."""
+    q_lens = [1] * n
+    check(make(n, q_lens, [(37 * i) % 150 for i in range(n)], 8, 2, 64, 16))
+    q_lens[5], q_lens[n - 1] = 70, 30
+    check(make(n, q_lens, [70 + (37 * i) % 150 for i in range(n)], 8, 2, 128, 16))

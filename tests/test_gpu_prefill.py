@@ -202,3 +202,18 @@ def test_decode_continues_from_a_prefilled_state(cuda_device):
     got = st.step(d["mixed"][m:], d["a"][m:], d["b"][m:], d["a_log"], d["dt_bias"])
     want, _ = R.gdn(d["mixed"], d["a"], d["b"], d["a_log"], d["dt_bias"], d["state"], [m + 1], [False])
     assert R.rel(got, want[m:]) < TOL_OUT  # the step's ring rounds q, k to bf16
+
+
+@pytest.mark.parametrize("lens", [[70], [3]])
+def test_gates_of_minus_infinity(cuda_device, lens):
+    """A decay so strong that its logarithm overflows float32 clears the state; nothing turns into NaN."""
+    d = inputs(15, lens, 2, 4)
+    d["a_log"] = torch.full((4,), 80.0, device="cuda")  # exp(80) softplus(20) = 1e36, times 3e38 / 20 below: infinite
+    d["a"][::2] = 3.0e38
+    d["a"][1::2] = -200.0  # softplus underflows: no decay
+    check(d, lens)
+
+
+def test_many_sequences(cuda_device):
+    lens = [1 + (7 * i) % 90 for i in range(60)]
+    check(inputs(16, lens, 1, 2), lens, fresh=[i % 3 == 0 for i in range(60)])
