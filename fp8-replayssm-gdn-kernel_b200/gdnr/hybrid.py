@@ -10,9 +10,9 @@ have built from the prompt, and a hybrid model's other layers attend a paged cac
 * :func:`paged_attention` -- causal attention of the new tokens over that cache.
 
 A ragged batch is packed: the tokens of sequence ``n`` are rows ``cu_seqlens[n]``
-to ``cu_seqlens[n + 1] - 1``.  ``max_seqlen`` is the longest sequence as far as the
-host knows it (it picks kernels and grids; a longer one is reported in the device error
-word as ``GDNR_DEVERR_BAD_HINT``).  All work runs on the current stream of the
+to ``cu_seqlens[n + 1] - 1``; rows that belong to no sequence are not written.  ``max_seqlen`` is
+the longest sequence as far as the host knows it (it picks kernels and grids; ``paged_attention``
+reports a longer one in the device error word as ``GDNR_DEVERR_BAD_HINT``).  All work runs on the current stream of the
 tensors' device; nothing synchronises.
 """
 

@@ -246,8 +246,9 @@ int gdnr_bf16_step(const gdnr_bf16_step_args* args, void* stream);
  * A ragged batch of N sequences is packed: the tokens of sequence n are rows
  * cu_seqlens[n] .. cu_seqlens[n+1]-1 of the token tensors (cu_seqlens [N+1] I32,
  * ascending from 0; a sequence may be empty).  max_seqlen is the longest of them as far
- * as the host knows it (0: unknown); it picks kernels and grids.  A longer sequence is
- * reported as GDNR_DEVERR_BAD_HINT and its rows may be incomplete. */
+ * as the host knows it (0: unknown); it picks kernels and grids.  gdnr_paged_attention
+ * reports a longer one as GDNR_DEVERR_BAD_HINT, and its rows may be incomplete.  Token
+ * rows that belong to no sequence are not written. */
 
 /* ---- gdnr_gdn_prefill: the gated delta rule over whole sequences ----------
  * Per value head, token by token, with k = k_raw / sqrt(|k_raw|^2 + 1e-6), q likewise
