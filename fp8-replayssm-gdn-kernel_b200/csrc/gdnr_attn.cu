@@ -704,26 +704,11 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const 
   if (warp == 0) write_lse(p, s, cut.h, rr, m, l);
 }
 
-// The join may be set up while the kernel before it still runs; it waits for that one's results (griddep_wait).
-template <class K>
-void launch_join(K kern, dim3 grid, const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(AJ_WARPS * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, p, of, ctas);
-}
-
 template <int D, int BM, int ROWS>
 void join(const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
   // rows a unit can have, by the longest sequence the host knows of
   const int rows = int(std::min<int64_t>(BM, int64_t(p.max_q) * p.G));
-  launch_join(attn_join_kernel<D, BM, ROWS>, dim3(ctas - 1, (rows + ROWS - 1) / ROWS), p, ctas, of, stream);
+  launch_behind(attn_join_kernel<D, BM, ROWS>, dim3(ctas - 1, (rows + ROWS - 1) / ROWS), AJ_WARPS * 32, 0, stream, p, of, ctas);
 }
 
 template <int D>
@@ -733,7 +718,7 @@ void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream
   else if (bm == 64)
     join<D, 64, 2>(p, ctas, of, stream);
   else
-    launch_join(attn_join_columns_kernel<D, D == 256 ? 128 : 256>, dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), p, ctas, of, stream);
+    launch_behind(attn_join_columns_kernel<D, D == 256 ? 128 : 256>, dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), AJ_WARPS * 32, 0, stream, p, of, ctas);
 }
 
 template <int D, int WM, int WN, int STAGES, int PER_SM>

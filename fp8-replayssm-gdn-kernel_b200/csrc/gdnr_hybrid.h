@@ -123,4 +123,21 @@ int multiprocessor_count();
 cudaError_t encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                             const uint32_t* box);
 
+// Launches a kernel that may be set up while the one before it in the stream still runs; it waits for that one's
+// results itself (griddep_wait).
+template <class K, class... A>
+cudaError_t launch_behind(K kern, dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 }  // namespace gdnr
