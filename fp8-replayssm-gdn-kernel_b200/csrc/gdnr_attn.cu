@@ -278,7 +278,7 @@ struct AsCfg {
   // the first kilobyte: AsShared; the stages begin at the second, a multiple of 1024 bytes (two CTAs of 115,712 bytes
   // are what a multiprocessor holds: there is no room to align by hand)
   static constexpr int SMEM = 1024 + STAGES * 2 * TILE + Q_BYTES;
-  static_assert(WN == 1 || WN * 16 * D * 4 <= 2 * TILE, "the join uses the last tile's stage");
+  static_assert(WN == 1 || WM * WN * 16 * D * 4 <= 2 * TILE, "the join uses the last tile's stage");
 };
 
 struct AsShared {
@@ -522,29 +522,29 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
         }
       }
     } else {
-      // join the WN warps' parts of the 16 rows in the last tile's stage, [WN][16][D] floats, columns changed by row
-      static_assert(WM == 1 || WN == 1, "one of the two");
+      // join the WN warps' parts of each 16 rows in the last tile's stage, [WM][WN][16][D] floats, columns changed by row
       const uint32_t st = (k - 1) % STAGES;
       float* js = reinterpret_cast<float*>(raw + 1024 + st * 2 * C::TILE);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int r = (lane >> 2) + 8 * j;
-        float* dst = js + (wn * 16 + r) * D;
+        float* dst = js + (warp * 16 + r) * D;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
           *reinterpret_cast<float2*>(dst + ((c * 8 + 2 * (lane & 3)) ^ ((r & 7) * 8))) = make_float2(o[c][2 * j], o[c][2 * j + 1]);
-        if ((lane & 3) == 0) sh.ml[wn][r][0] = mx[j], sh.ml[wn][r][1] = sum[j];
+        if ((lane & 3) == 0) sh.ml[warp][r][0] = mx[j], sh.ml[warp][r][1] = sum[j];
       }
       bar_sync(1, C::CONSUMERS);
-      for (int r = warp; r < 16 && r < rows; r += WM * WN) {
+      for (int r = warp; r < BM && r < rows; r += WM * WN) {
+        const int w0 = (r >> 4) * WN, r16 = r & 15;  // its warps, its row there
         float m = -INFINITY, f[WN], l = 0.f;
 #pragma unroll
-        for (int w = 0; w < WN; ++w) m = fmaxf(m, sh.ml[w][r][0]);
+        for (int w = 0; w < WN; ++w) m = fmaxf(m, sh.ml[w0 + w][r16][0]);
         const float b = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int w = 0; w < WN; ++w) {
-          f[w] = ex2_approx(sh.ml[w][r][0] - b);
-          l += f[w] * sh.ml[w][r][1];
+          f[w] = ex2_approx(sh.ml[w0 + w][r16][0] - b);
+          l += f[w] * sh.ml[w0 + w][r16][1];
         }
         const int64_t to = out_at(p, u, row_base + r);
         const float inv = l > 0.f ? 1.0f / l : 0.f;
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
           float2 x = make_float2(0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < WN; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(js + (w * 16 + r) * D + (c ^ ((r & 7) * 8)));
+            const float2 y = *reinterpret_cast<const float2*>(js + ((w0 + w) * 16 + r16) * D + (c ^ ((r & 7) * 8)));
             x.x += f[w] * y.x;
             x.y += f[w] * y.y;
           }
@@ -715,6 +715,8 @@ template <int D>
 void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream_t stream) {
   if (bm == 16)
     join<D, 16, 1>(p, ctas, of, stream);
+  else if (bm == 32)
+    join<D, 32, 2>(p, ctas, of, stream);
   else if (bm == 64)
     join<D, 64, 2>(p, ctas, of, stream);
   else
@@ -754,7 +756,11 @@ cudaError_t run_stream(const AttnParams& p, const AtRows& of, cudaStream_t strea
 
 template <int D, int STAGES, int PER_SM>
 cudaError_t pick(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
-  if (kv_tma_takes(p)) return most <= 16 ? run_stream<D, 1, 4, STAGES, PER_SM>(p, of, stream) : run_stream<D, 4, 1, STAGES, PER_SM>(p, of, stream);
+  if (kv_tma_takes(p)) {
+    if (most <= 16) return run_stream<D, 1, 4, STAGES, PER_SM>(p, of, stream);
+    if (most <= 32) return run_stream<D, 2, 2, STAGES, PER_SM>(p, of, stream);
+    return run_stream<D, 4, 1, STAGES, PER_SM>(p, of, stream);
+  }
   constexpr int S = D == 256 ? 2 : 3;  // pages of any size
   return most <= 16 ? run<D, 1, 4, S, PER_SM>(p, of, stream) : run<D, 4, 1, S, PER_SM>(p, of, stream);
 }
@@ -767,7 +773,7 @@ cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, cudaStre
 
 // Sequences of at most so many rows (tokens times query heads of a key head) are bound by reading their keys
 // and stay on warp-level tiles.
-constexpr int AT_FEW_ROWS = 64;
+constexpr int few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
 }  // namespace
 
@@ -809,12 +815,13 @@ int64_t attn_workspace_bytes(int head_dim) {
 
 cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream) {
   const int64_t most = std::min<int64_t>(int64_t(p.max_q) * p.G, INT32_MAX);
-  if (most <= AT_FEW_ROWS || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, stream);
-  // sequences of many rows on the tensor-memory tiles, the others, if there can be any, as above
+  if (most <= few_rows(p.D) || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, stream);
   if (int64_t(p.T) == int64_t(p.N) * p.max_q) return launch_attn_tc(p, 0, stream);  // all of the same length
-  cudaError_t e = launch_attn_tc(p, AT_FEW_ROWS, stream);
+  // sequences of many rows on the tensor-memory tiles, the others, mostly of one token, on tiles of few rows
+  const int lo = p.G <= 16 ? 16 : few_rows(p.D);
+  cudaError_t e = launch_attn_tc(p, lo, stream);
   if (e != cudaSuccess) return e;
-  return small_rows(p, AT_FEW_ROWS, AtRows{0, AT_FEW_ROWS}, stream);
+  return small_rows(p, lo, AtRows{0, lo}, stream);
 }
 
 }  // namespace gdnr
