@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   const uint32_t kv_s = smem_addr(raw) + 1024, q_s = kv_s + STAGES * 2 * C::TILE;
   if (kv_s & 1023u) {  // the swizzled tiles would not be where the products look for them
     if (tid == 0) atomicOr(p.err, GDNR_DEVERR_LAYOUT);
+    griddep_wait();
     return;
   }
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   const Share share = share_of<T>(total, blockIdx.x, gridDim.x);
   if (share.begin >= share.end) {
     if (tid == 0) meta[0] = -1;
+    griddep_wait();
     return;
   }
   const WarpWait wait{p.err, &sh.abort};
@@ -359,6 +361,8 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
         while (!mbar_try_wait(smem_addr(&full[j % STAGES]), (j / STAGES) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
         }
       }
+    // a CTA does not end before the kernel that this one may run beside has: what comes next waits for this one only
+    griddep_wait();
     return;
   }
 
@@ -576,24 +580,29 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   }
 }
 
-// Joins the parts of the units that are cut between shares.  Block (i - 1, y) looks at
+// Joins the parts of the units that are cut between shares.  Block (i, y) looks at
 // the cut between shares i - 1 and i: where it is the first cut of its unit, the
 // block joins ROWS rows of all parts in the order of the shares (a fixed order: the
 // result does not depend on which CTA ran when).  The eight warps have a row each, or share one
 // row's parts: a unit of few rows may be cut into as many parts as there are shares.
 constexpr int AJ_WARPS = 8;
 
+// A kernel's parts, and how many blocks look at a cut.
+struct Cuts {
+  const float* ws;
+  AtRows rows;
+  int ctas, ys;
+};
+
 template <int D, int BM, int ROWS>
-__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_constant__ AttnParams p, const AtRows of, int ctas) {
+__device__ __forceinline__ void join_rows(const AttnParams& p, const Cuts& of, int i, int y0) {
   constexpr int PER_ROW = AJ_WARPS / ROWS;
   __shared__ float sm[AJ_WARPS][D + 2];
-  const int i = blockIdx.x + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
   CutUnit cut;
-  if (!cut_unit(reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2)), i, cut)) return;
-  const SeqLen s = seq_len(p, cut.n, of);
-  const int r = blockIdx.y * ROWS + warp / PER_ROW, rr = cut.rt * BM + r;
+  if (!cut_unit(reinterpret_cast<const int*>(of.ws + int64_t(of.ctas) * 2 * BM * (D + 2)), i, cut)) return;
+  const SeqLen s = seq_len(p, cut.n, of.rows);
+  const int r = y0 * ROWS + warp / PER_ROW, rr = cut.rt * BM + r;
   const bool live = r < BM && rr < s.m * p.G;
   if (__syncthreads_or(live) == 0) return;
   constexpr int E = D / 32;
@@ -609,7 +618,7 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
       for (int a = 0; a < AHEAD; ++a) {
         const int c = c0 + a * PER_ROW;
         pm[a] = -INFINITY, pl[a] = 0.f;
-        const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
+        const float* src = of.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + int64_t(r) * (D + 2);
         if (c < parts) pm[a] = src[D], pl[a] = src[D + 1];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[a][e] = c < parts ? src[e * 32 + lane] : 0.f;
@@ -657,17 +666,15 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
 }
 
 // The same for parts that lie in columns of BM rows (the tcgen05 kernel's: its threads have a row each).  Block
-// (i - 1, y) has 32 rows, a lane each; its warps share the D columns.
+// (i, y) has 32 rows, a lane each; its warps share the D columns.
 template <int D, int BM>
-__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const __grid_constant__ AttnParams p, const AtRows of, int ctas) {
+__device__ __forceinline__ void join_columns(const AttnParams& p, const Cuts& of, int i, int y0) {
   constexpr int COLS = D / AJ_WARPS;
-  const int i = blockIdx.x + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
   CutUnit cut;
-  if (!cut_unit(reinterpret_cast<const int*>(p.ws + int64_t(ctas) * 2 * BM * (D + 2)), i, cut)) return;
-  const SeqLen s = seq_len(p, cut.n, of);
-  const int r = blockIdx.y * 32 + lane, rr = cut.rt * BM + r;
+  if (!cut_unit(reinterpret_cast<const int*>(of.ws + int64_t(of.ctas) * 2 * BM * (D + 2)), i, cut)) return;
+  const SeqLen s = seq_len(p, cut.n, of.rows);
+  const int r = y0 * 32 + lane, rr = cut.rt * BM + r;
   if (rr >= s.m * p.G) return;
   float m = -INFINITY, l = 0.f, x[COLS];
 #pragma unroll
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const 
   // the next part is on its way while one is added
   float next[COLS], nm, nl;
   auto request = [&](int c) {
-    const float* src = p.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
+    const float* src = of.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
     nm = src[D * BM], nl = src[(D + 1) * BM];
 #pragma unroll
     for (int e = 0; e < COLS; ++e) next[e] = src[(warp * COLS + e) * BM];
@@ -705,22 +712,36 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const 
 }
 
 template <int D, int BM, int ROWS>
-void join(const AttnParams& p, int ctas, const AtRows& of, cudaStream_t stream) {
-  // rows a unit can have, by the longest sequence the host knows of
-  const int rows = int(std::min<int64_t>(BM, int64_t(p.max_q) * p.G));
-  launch_behind(attn_join_kernel<D, BM, ROWS>, dim3(ctas - 1, (rows + ROWS - 1) / ROWS), AJ_WARPS * 32, 0, stream, p, of, ctas);
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_constant__ AttnParams p, const Cuts of) {
+  griddep_wait();
+  join_rows<D, BM, ROWS>(p, of, blockIdx.x + 1, blockIdx.y);
 }
 
 template <int D>
-void join_of(const AttnParams& p, int ctas, int bm, const AtRows& of, cudaStream_t stream) {
-  if (bm == 16)
-    join<D, 16, 1>(p, ctas, of, stream);
-  else if (bm == 32)
-    join<D, 32, 2>(p, ctas, of, stream);
-  else if (bm == 64)
-    join<D, 64, 2>(p, ctas, of, stream);
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const __grid_constant__ AttnParams p, const Cuts of) {
+  griddep_wait();
+  join_columns<D, attn_tc_rows(D)>(p, of, blockIdx.x + 1, blockIdx.y);
+}
+
+// Both kernels' units of a mixed batch in one launch.
+template <int D, int BM, int ROWS>
+__global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_both_kernel(const __grid_constant__ AttnParams p, const Cuts many, const Cuts few) {
+  griddep_wait();
+  const int of_many = (many.ctas - 1) * many.ys, b = blockIdx.x;
+  if (b < of_many)
+    join_columns<D, attn_tc_rows(D)>(p, many, b / many.ys + 1, b % many.ys);
   else
-    launch_behind(attn_join_columns_kernel<D, D == 256 ? 128 : 256>, dim3(ctas - 1, (D == 256 ? 128 : 256) / 32), AJ_WARPS * 32, 0, stream, p, of, ctas);
+    join_rows<D, BM, ROWS>(p, few, (b - of_many) / few.ys + 1, (b - of_many) % few.ys);
+}
+
+// The few-row kernel's cuts and, where there are any, the tcgen05 kernel's.
+template <int D, int BM, int ROWS>
+cudaError_t join(const AttnParams& p, Cuts few, const Cuts& many, cudaStream_t stream) {
+  // rows a unit can have, by the longest sequence the host knows of
+  few.ys = (int(std::min<int64_t>(BM, int64_t(p.max_q) * p.G)) + ROWS - 1) / ROWS;
+  if (!many.ctas) return launch_behind(attn_join_kernel<D, BM, ROWS>, dim3(few.ctas - 1, few.ys), AJ_WARPS * 32, 0, stream, p, few);
+  return launch_behind(attn_join_both_kernel<D, BM, ROWS>, dim3((many.ctas - 1) * many.ys + (few.ctas - 1) * few.ys), AJ_WARPS * 32, 0, stream, p,
+                       many, few);
 }
 
 template <int D, int WM, int WN, int STAGES, int PER_SM>
@@ -734,11 +755,13 @@ cudaError_t run(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
   kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, of);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_attn_join(p, ctas, C::BM, of, stream);
+  return ctas < 2 ? cudaSuccess : join<D, C::BM, C::BM == 16 ? 1 : 2>(p, Cuts{p.ws, of, ctas, 0}, Cuts{}, stream);
 }
 
+// `many`: the tcgen05 kernel's cuts, if that has just been launched for the batch's other sequences.  Its parts stay where
+// they are, this kernel begins on the multiprocessors that are done with the other, and one join follows.
 template <int D, int WM, int WN, int STAGES, int PER_SM>
-cudaError_t run_stream(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
+cudaError_t run_stream(AttnParams p, const AtRows& of, const Cuts& many, cudaStream_t stream) {
   using C = AsCfg<D, WM, WN, STAGES>;
   CUtensorMap maps[2];
   cudaError_t e = encode_kv_maps(p, AT_BN, maps);
@@ -748,32 +771,48 @@ cudaError_t run_stream(const AttnParams& p, const AtRows& of, cudaStream_t strea
   e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), C::SMEM, cache);
   if (e != cudaSuccess) return e;
   const int ctas = multiprocessor_count() * PER_SM;
-  kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], of);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return launch_attn_join(p, ctas, C::BM, of, stream);
+  if (many.ctas) {
+    p.ws += attn_tc_floats(D);
+    e = launch_behind(kern, dim3(ctas), C::THREADS, C::SMEM, stream, p, maps[0], maps[1], of);
+  } else {
+    kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], of);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess || ctas < 2) return e;
+  return join<D, C::BM, C::BM == 16 ? 1 : 2>(p, Cuts{p.ws, of, ctas, 0}, many, stream);
 }
 
 template <int D, int STAGES, int PER_SM>
-cudaError_t pick(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
+cudaError_t pick(const AttnParams& p, int most, const AtRows& of, const Cuts& many, cudaStream_t stream) {
   if (kv_tma_takes(p)) {
-    if (most <= 16) return run_stream<D, 1, 4, STAGES, PER_SM>(p, of, stream);
-    if (most <= 32) return run_stream<D, 2, 2, STAGES, PER_SM>(p, of, stream);
-    return run_stream<D, 4, 1, STAGES, PER_SM>(p, of, stream);
+    if (most <= 16) return run_stream<D, 1, 4, STAGES, PER_SM>(p, of, many, stream);
+    if (most <= 32) return run_stream<D, 2, 2, STAGES, PER_SM>(p, of, many, stream);
+    return run_stream<D, 4, 1, STAGES, PER_SM>(p, of, many, stream);
   }
   constexpr int S = D == 256 ? 2 : 3;  // pages of any size
   return most <= 16 ? run<D, 1, 4, S, PER_SM>(p, of, stream) : run<D, 4, 1, S, PER_SM>(p, of, stream);
 }
 
-cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, cudaStream_t stream) {
-  if (p.D == 64) return pick<64, 6, 2>(p, most, of, stream);
-  if (p.D == 128) return pick<128, 3, 2>(p, most, of, stream);
-  return pick<256, 3, 1>(p, most, of, stream);
+cudaError_t small_rows(const AttnParams& p, int most, const AtRows& of, const Cuts& many, cudaStream_t stream) {
+  if (p.D == 64) return pick<64, 6, 2>(p, most, of, many, stream);
+  if (p.D == 128) return pick<128, 3, 2>(p, most, of, many, stream);
+  return pick<256, 3, 1>(p, most, of, many, stream);
 }
 
 // Sequences of at most so many rows (tokens times query heads of a key head) are bound by reading their keys
 // and stay on warp-level tiles.
 constexpr int few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
+
+Cuts tc_cuts(const AttnParams& p, int lo) { return Cuts{p.ws, AtRows{lo, INT32_MAX}, multiprocessor_count(), attn_tc_rows(p.D) / 32}; }
+
+cudaError_t launch_attn_tc_join(const AttnParams& p, int lo, cudaStream_t stream) {
+  const Cuts of = tc_cuts(p, lo);
+  if (of.ctas < 2) return cudaSuccess;
+  const dim3 grid(of.ctas - 1, of.ys);
+  if (p.D == 64) return launch_behind(attn_join_columns_kernel<64>, grid, AJ_WARPS * 32, 0, stream, p, of);
+  if (p.D == 128) return launch_behind(attn_join_columns_kernel<128>, grid, AJ_WARPS * 32, 0, stream, p, of);
+  return launch_behind(attn_join_columns_kernel<256>, grid, AJ_WARPS * 32, 0, stream, p, of);
+}
 
 }  // namespace
 
@@ -796,32 +835,20 @@ cudaError_t encode_kv_maps(const AttnParams& p, int bn, CUtensorMap* maps) {
   return cudaSuccess;
 }
 
-cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream) {
-  if (ctas < 2) return cudaSuccess;
-  if (p.D == 64)
-    join_of<64>(p, ctas, bm, rows, stream);
-  else if (p.D == 128)
-    join_of<128>(p, ctas, bm, rows, stream);
-  else
-    join_of<256>(p, ctas, bm, rows, stream);
-  return cudaGetLastError();
-}
-
 int64_t attn_workspace_bytes(int head_dim) {
-  const int64_t sms = multiprocessor_count(), ctas = sms * AT_MAX_CTAS_PER_SM;
-  const int64_t rows = std::max<int64_t>(ctas * 2 * 64, sms * 2 * attn_tc_rows(head_dim));
-  return (rows * (head_dim + 2) + ctas * AT_META) * 4;
+  const int64_t ctas = int64_t(multiprocessor_count()) * AT_MAX_CTAS_PER_SM;
+  return (attn_tc_floats(head_dim) + ctas * (2 * 64 * (head_dim + 2) + AT_META)) * 4;
 }
 
 cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream) {
   const int64_t most = std::min<int64_t>(int64_t(p.max_q) * p.G, INT32_MAX);
-  if (most <= few_rows(p.D) || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, stream);
-  if (int64_t(p.T) == int64_t(p.N) * p.max_q) return launch_attn_tc(p, 0, stream);  // all of the same length
+  if (most <= few_rows(p.D) || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, Cuts{}, stream);
+  const bool alike = int64_t(p.T) == int64_t(p.N) * p.max_q;  // all of the same length
   // sequences of many rows on the tensor-memory tiles, the others, mostly of one token, on tiles of few rows
-  const int lo = p.G <= 16 ? 16 : few_rows(p.D);
+  const int lo = alike ? 0 : (p.G <= 16 ? 16 : few_rows(p.D));
   cudaError_t e = launch_attn_tc(p, lo, stream);
   if (e != cudaSuccess) return e;
-  return small_rows(p, lo, AtRows{0, lo}, stream);
+  return alike ? launch_attn_tc_join(p, lo, stream) : small_rows(p, lo, AtRows{0, lo}, tc_cuts(p, lo), stream);
 }
 
 }  // namespace gdnr

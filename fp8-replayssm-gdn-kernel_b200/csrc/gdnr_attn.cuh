@@ -332,12 +332,11 @@ __device__ __forceinline__ KvBox kv_box(const AttnParams& p, const Unit& u, cons
   return b;
 }
 
-// Joins the parts of the units of BM rows that were cut between `ctas` shares (gdnr_attn.cu).
-cudaError_t launch_attn_join(const AttnParams& p, int ctas, int bm, const AtRows& rows, cudaStream_t stream);
-
-// Tiles on the fifth-generation tensor cores (gdnr_attn_tc.cu): sequences of more than `lo` rows.
+// Tiles on the fifth-generation tensor cores (gdnr_attn_tc.cu): sequences of more than `lo` rows, in tiles of attn_tc_rows.
+// Its parts and records are the first attn_tc_floats of the workspace; the join (gdnr_attn.cu) has to follow.
+constexpr int attn_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 bool attn_tc_takes(const AttnParams& p);
+int64_t attn_tc_floats(int head_dim);
 cudaError_t launch_attn_tc(const AttnParams& p, int lo, cudaStream_t stream);
-int attn_tc_rows(int head_dim);
 
 }  // namespace gdnr

@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
+  griddep_launch();  // what is launched behind takes over a multiprocessor when this CTA ends
   constexpr int WARPS = C::THREADS / 32;
   const int64_t places = warp_places<T>(p, of, warp, WARPS, lane);
   if (lane == 0) bars.places[warp] = places;
@@ -565,14 +566,14 @@ cudaError_t run_tc(const AttnParams& p, const AtRows& of, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
   }
   kern<<<ctas, C::THREADS, C::SMEM, stream>>>(p, maps[0], maps[1], qmap, of, q_tma);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return launch_attn_join(p, ctas, C::BM, of, stream);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-int attn_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
+int64_t attn_tc_floats(int head_dim) {
+  return int64_t(multiprocessor_count()) * (2 * attn_tc_rows(head_dim) * (head_dim + 2) + AT_META);
+}
 
 // Scores that grow with the dot product: the maximum is taken before the scale
 bool attn_tc_takes(const AttnParams& p) { return p.scale > 0.f && kv_tma_takes(p); }
