@@ -666,49 +666,61 @@ __device__ __forceinline__ void join_rows(const AttnParams& p, const Cuts& of, i
 }
 
 // The same for parts that lie in columns of BM rows (the tcgen05 kernel's: its threads have a row each).  Block
-// (i, y) has 32 rows, a lane each; its warps share the D columns.
-template <int D, int BM>
+// (i, y) has 32 rows, a lane each, and AJ_WARPS * COLS columns, COLS a warp.
+template <int D, int BM, int COLS, int AHEAD>
 __device__ __forceinline__ void join_columns(const AttnParams& p, const Cuts& of, int i, int y0) {
-  constexpr int COLS = D / AJ_WARPS;
+  constexpr int BLOCKS = D / (AJ_WARPS * COLS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   CutUnit cut;
   if (!cut_unit(reinterpret_cast<const int*>(of.ws + int64_t(of.ctas) * 2 * BM * (D + 2)), i, cut)) return;
   const SeqLen s = seq_len(p, cut.n, of.rows);
-  const int r = y0 * 32 + lane, rr = cut.rt * BM + r;
+  const int col = (y0 % BLOCKS * AJ_WARPS + warp) * COLS, r = y0 / BLOCKS * 32 + lane, rr = cut.rt * BM + r;
   if (rr >= s.m * p.G) return;
   float m = -INFINITY, l = 0.f, x[COLS];
 #pragma unroll
   for (int e = 0; e < COLS; ++e) x[e] = 0.f;
-  // the next part is on its way while one is added
-  float next[COLS], nm, nl;
-  auto request = [&](int c) {
-    const float* src = of.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
-    nm = src[D * BM], nl = src[(D + 1) * BM];
+  // the next parts are on their way while some are added
+  float next[AHEAD][COLS], nm[AHEAD], nl[AHEAD];
+  auto request = [&](int c0) {
 #pragma unroll
-    for (int e = 0; e < COLS; ++e) next[e] = src[(warp * COLS + e) * BM];
+    for (int a = 0; a < AHEAD; ++a) {
+      const int c = c0 + a;
+      if (AHEAD > 1 && c >= cut.parts) break;
+      const float* src = of.ws + (int64_t(i - 1 + c) * 2 + (c == 0 ? 1 : 0)) * BM * (D + 2) + r;
+      nm[a] = src[D * BM], nl[a] = src[(D + 1) * BM];
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) next[a][e] = src[(col + e) * BM];
+    }
   };
   request(0);
-  for (int c = 0; c < cut.parts; ++c) {
-    float y[COLS];
-    const float pm = nm, pl = nl;
+  for (int c0 = 0; c0 < cut.parts; c0 += AHEAD) {
+    float y[AHEAD][COLS], pm[AHEAD], pl[AHEAD];
 #pragma unroll
-    for (int e = 0; e < COLS; ++e) y[e] = next[e];
-    if (c + 1 < cut.parts) request(c + 1);
-    const float top = fmaxf(m, pm), b = top == -INFINITY ? 0.f : top;
-    const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm - b);
-    m = top;
-    l = l * f0 + pl * f1;
+    for (int a = 0; a < AHEAD; ++a) {
+      pm[a] = nm[a], pl[a] = nl[a];
 #pragma unroll
-    for (int e = 0; e < COLS; ++e) x[e] = x[e] * f0 + y[e] * f1;
+      for (int e = 0; e < COLS; ++e) y[a][e] = next[a][e];
+    }
+    if (c0 + AHEAD < cut.parts) request(c0 + AHEAD);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (AHEAD > 1 && c0 + a >= cut.parts) break;
+      const float top = fmaxf(m, pm[a]), b = top == -INFINITY ? 0.f : top;
+      const float f0 = ex2_approx(m - b), f1 = ex2_approx(pm[a] - b);
+      m = top;
+      l = l * f0 + pl[a] * f1;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) x[e] = x[e] * f0 + y[a][e] * f1;
+    }
   }
   const float inv = l > 0.f ? 1.0f / l : 0.f;
   const int tk = token_of(p, rr);
-  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(cut.h * p.G + rr - tk * p.G) * p.o_sh + warp * COLS;
+  uint16_t* dst = p.out + int64_t(s.q0 + tk) * p.o_st + int64_t(cut.h * p.G + rr - tk * p.G) * p.o_sh + col;
 #pragma unroll
   for (int e = 0; e < COLS; e += 8)
     *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16x2(x[e] * inv, x[e + 1] * inv), pack_bf16x2(x[e + 2] * inv, x[e + 3] * inv),
                                                     pack_bf16x2(x[e + 4] * inv, x[e + 5] * inv), pack_bf16x2(x[e + 6] * inv, x[e + 7] * inv));
-  if (warp == 0) write_lse(p, s, cut.h, rr, m, l);
+  if (col == 0) write_lse(p, s, cut.h, rr, m, l);
 }
 
 template <int D, int BM, int ROWS>
@@ -717,10 +729,10 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_kernel(const __grid_c
   join_rows<D, BM, ROWS>(p, of, blockIdx.x + 1, blockIdx.y);
 }
 
-template <int D>
+template <int D, int COLS, int AHEAD>
 __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_columns_kernel(const __grid_constant__ AttnParams p, const Cuts of) {
   griddep_wait();
-  join_columns<D, attn_tc_rows(D)>(p, of, blockIdx.x + 1, blockIdx.y);
+  join_columns<D, attn_tc_rows(D), COLS, AHEAD>(p, of, blockIdx.x + 1, blockIdx.y);
 }
 
 // Both kernels' units of a mixed batch in one launch.
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) attn_join_both_kernel(const __g
   griddep_wait();
   const int of_many = (many.ctas - 1) * many.ys, b = blockIdx.x;
   if (b < of_many)
-    join_columns<D, attn_tc_rows(D)>(p, many, b / many.ys + 1, b % many.ys);
+    join_columns<D, attn_tc_rows(D), D / AJ_WARPS, 1>(p, many, b / many.ys + 1, b % many.ys);
   else
     join_rows<D, BM, ROWS>(p, few, (b - of_many) / few.ys + 1, (b - of_many) % few.ys);
 }
@@ -805,13 +817,23 @@ constexpr int few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
 Cuts tc_cuts(const AttnParams& p, int lo) { return Cuts{p.ws, AtRows{lo, INT32_MAX}, multiprocessor_count(), attn_tc_rows(p.D) / 32}; }
 
-cudaError_t launch_attn_tc_join(const AttnParams& p, int lo, cudaStream_t stream) {
-  const Cuts of = tc_cuts(p, lo);
+// The tcgen05 kernel's cuts.  A block has all D columns of 32 rows, unless units are few and cut into many parts: then 64
+// columns, eight a warp and four parts ahead (40 tokens over 16000 keys, heads of 64 / 128 / 256: 28 / 34 / 36 us a call, not
+// 35 / 42 / 42; 2048 tokens over themselves, 2 parts a unit: 36 / 49 / 79 us this way, else 33 / 45 / 75).
+template <int D>
+cudaError_t tc_join(const AttnParams& p, int lo, cudaStream_t stream) {
+  Cuts of = tc_cuts(p, lo);
   if (of.ctas < 2) return cudaSuccess;
-  const dim3 grid(of.ctas - 1, of.ys);
-  if (p.D == 64) return launch_behind(attn_join_columns_kernel<64>, grid, AJ_WARPS * 32, 0, stream, p, of);
-  if (p.D == 128) return launch_behind(attn_join_columns_kernel<128>, grid, AJ_WARPS * 32, 0, stream, p, of);
-  return launch_behind(attn_join_columns_kernel<256>, grid, AJ_WARPS * 32, 0, stream, p, of);
+  const int64_t units = (int64_t(p.T) * p.G / attn_tc_rows(D) + p.N) * p.Hk;  // or fewer
+  if (units * 8 > of.ctas)
+    return launch_behind(attn_join_columns_kernel<D, D / AJ_WARPS, 1>, dim3(of.ctas - 1, of.ys), AJ_WARPS * 32, 0, stream, p, of);
+  return launch_behind(attn_join_columns_kernel<D, 8, 4>, dim3(of.ctas - 1, of.ys * (D / 64)), AJ_WARPS * 32, 0, stream, p, of);
+}
+
+cudaError_t launch_attn_tc_join(const AttnParams& p, int lo, cudaStream_t stream) {
+  if (p.D == 64) return tc_join<64>(p, lo, stream);
+  if (p.D == 128) return tc_join<128>(p, lo, stream);
+  return tc_join<256>(p, lo, stream);
 }
 
 }  // namespace

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
   float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
   int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
-  griddep_launch();  // what is launched behind takes over a multiprocessor when this CTA ends
+  if (of.lo > 0) griddep_launch();  // the few-row kernel takes over a multiprocessor when this CTA ends
   constexpr int WARPS = C::THREADS / 32;
   const int64_t places = warp_places<T>(p, of, warp, WARPS, lane);
   if (lane == 0) bars.places[warp] = places;
