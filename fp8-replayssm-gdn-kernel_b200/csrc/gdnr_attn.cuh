@@ -275,35 +275,6 @@ __device__ __forceinline__ void kv_tma(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// Waits of a whole warp; they give up after a second, or when another warp has: then every role leaves its loop.
-struct WarpWait {
-  uint32_t* err;
-  volatile int* abort;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    bool ok = mbar_try_wait(smem_addr(bar), parity);
-    if (!ok) ok = slow(bar, parity);
-    return __all_sync(0xffffffffu, ok);
-  }
-  __device__ __forceinline__ bool slow(uint64_t* bar, uint32_t parity) const {
-    const uint32_t a = smem_addr(bar);
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t it = 1; it < WAIT_LIMIT_ITERS; ++it) {
-      if (mbar_try_wait(a, parity)) return true;
-      if ((it & 63u) == 0) {
-        if (*abort) return false;
-        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
-      }
-    }
-    *abort = 1;
-    atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
-    return false;
-  }
-};
-
 // The box of tile t that a lane requests: a page past the sequence's end, or outside the cache, reads as zeros
 // (its coordinate lies past the map).
 struct KvBox {

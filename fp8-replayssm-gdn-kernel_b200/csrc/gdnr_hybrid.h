@@ -36,6 +36,7 @@ struct PrefillParams {
   int64_t o_st, o_sh;
   int32_t N, H, HV, S, T;
   uint8_t* images;  // chunked form: workspace, CK_IMAGE_BYTES a chunk and value head
+  bool whole;       // set by the launcher: the images hold T whole
   uint32_t* err;
 };
 
@@ -65,7 +66,7 @@ __device__ __forceinline__ SeqRange prefill_seq(const PrefillParams& p, int n) {
 }
 
 cudaError_t launch_prefill_recurrent(const PrefillParams& p, cudaStream_t stream);
-cudaError_t launch_prefill_chunk(const PrefillParams& p, int64_t longest, cudaStream_t stream);
+cudaError_t launch_prefill_chunk(PrefillParams p, int64_t longest, cudaStream_t stream);
 // max_seqlen: 0 where the host does not know it
 int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen);
 cudaError_t launch_prefill(const PrefillParams& p, int max_seqlen, cudaStream_t stream);

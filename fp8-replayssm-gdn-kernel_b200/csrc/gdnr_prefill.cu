@@ -6,7 +6,7 @@
 // K^-1/2, g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b).
 #include "gdnr_device.cuh"
 #include "gdnr_hybrid.h"
-#include "gdnr_tile.cuh"
+#include "gdnr_tc.cuh"
 
 #include <algorithm>
 
@@ -183,14 +183,15 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 // strong decay.
 constexpr int CK_C = 64;
 
-// Lower triangular [C, C] of f16 as its ten blocks of 16 x 16, rows of 32 bytes whose two
-// 16-byte halves change places every four rows (eight rows' equal halves cover all banks).
+// Lower triangular [C, C] of f16 as its ten blocks of 16 x 16, column by column: rows of 32 bytes whose two
+// 16-byte halves change places every four rows (the 32-byte swizzle: eight rows' equal halves cover all banks, and
+// a column's blocks are one right operand of the tensor cores).
 constexpr int CK_TRI = 10 * 512;
-__host__ __device__ constexpr int ck_block(int i, int j) { return (i * (i + 1) / 2 + j) * 512; }
+__host__ __device__ constexpr int ck_block(int i, int j) { return (4 * j - j * (j - 1) / 2 + i - j) * 512; }
 __device__ __forceinline__ uint32_t ck_in_block(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
 
 struct CkImage {
-  // diagonal blocks: T = (I + A)^-1 of the block, below them: -A
+  // t: diagonal blocks: (I + A)^-1 of the block, below them: -A; or (whole) T = (I + A)^-1
   uint8_t t_hi[CK_TRI], t_lo[CK_TRI], p_hi[CK_TRI], p_lo[CK_TRI];
   float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, -beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
   float pad[15];
@@ -216,6 +217,14 @@ __device__ __forceinline__ void ck_zero_rows(uint8_t* tile, int boxes, int valid
     const int box = i / ((CK_C - valid) * 8), j = i % ((CK_C - valid) * 8);
     *reinterpret_cast<uint4*>(tile + box * 8192 + (valid + j / 8) * 128 + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
+__device__ __forceinline__ void ck_left_f16(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
+  split_f16x2(x[0][0], x[0][1], hi[0], lo[0]);
+  split_f16x2(x[0][2], x[0][3], hi[1], lo[1]);
+  split_f16x2(x[1][0], x[1][1], hi[2], lo[2]);
+  split_f16x2(x[1][2], x[1][3], hi[3], lo[3]);
 }
 
 // Two neighbouring floats of a factor
@@ -314,6 +323,70 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
       const float hi = float(y);
       sm.g_hi[e][2 * lane + i] = hi;
       sm.g_lo[e][2 * lane + i] = float(y - hi);
+    }
+  };
+  // What lies below the diagonal blocks T_ii of T = (I + A)^-1, in the image, by halves of 32, then of 64 tokens: the
+  // block below two inverses is T_low (-A) T_top.  Two warps a head.  (In float32 on the other units it took 18 us of
+  // the kernel's 67, as products of f16 pairs 6.)
+  auto invert_below = [&](int e0) {
+    const int e = warp >> 1, w = warp & 1;
+    const bool mine = e0 + e < group;
+    CkImage& img = sm.img[e];
+    const uint32_t hi = smem_addr(img.t_hi), lo = smem_addr(img.t_lo), in = ck_in_block(lane & 15, lane >> 4);
+    // acc += L R, R block (i, j) of the image
+    auto times = [&](float* acc, const uint32_t* lh, const uint32_t* ll, int i, int j) {
+      uint32_t rh[4], rl[4];
+      ldsm_x4_t(hi + ck_block(i, j) + in, rh);
+      ldsm_x4_t(lo + ck_block(i, j) + in, rl);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) mma_f16(acc + 4 * t, q == 1 ? ll : lh, (q == 2 ? rl : rh)[2 * t], (q == 2 ? rl : rh)[2 * t + 1]);
+    };
+    auto times_block = [&](float* acc, int li, int lj, int i, int j) {
+      uint32_t lh[4], ll[4];
+      ldsm_x4(hi + ck_block(li, lj) + in, lh);
+      ldsm_x4(lo + ck_block(li, lj) + in, ll);
+      times(acc, lh, ll, i, j);
+    };
+    auto emit = [&](const float* acc, int i, int j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // tile k / 2, rows + 8 (k % 2)
+        uint32_t wh, wl;
+        split_f16x2(acc[2 * k], acc[2 * k + 1], wh, wl);
+        const uint32_t at = ck_block(i, j) + ck_in_block(lane >> 2, k >> 1) + 4 * (lane & 3) + (k & 1) * 256;
+        *reinterpret_cast<uint32_t*>(img.t_hi + at) = wh;
+        *reinterpret_cast<uint32_t*>(img.t_lo + at) = wl;
+      }
+    };
+    float x[2][8] = {}, y[2][8] = {};
+    uint32_t wh[4], wl[4];
+    bar_sync(1, 128);
+    if (mine) {
+      times_block(x[0], 2 * w + 1, 2 * w + 1, 2 * w + 1, 2 * w);  // T_low (-A)
+      ck_left_f16(reinterpret_cast<const float(*)[4]>(x[0]), wh, wl);
+      times(y[0], wh, wl, 2 * w, 2 * w);
+      __syncwarp();
+      emit(y[0], 2 * w + 1, 2 * w);
+    }
+    bar_sync(1, 128);
+    // row 2 + w
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[0][k] = x[1][k] = y[0][k] = 0.f;
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        times_block(x[j], 2 + w, 2, 2, j);
+        if (w) times_block(x[j], 3, 3, 3, j);
+        ck_left_f16(reinterpret_cast<const float(*)[4]>(x[j]), wh, wl);
+        times(y[0], wh, wl, j, 0);
+        if (j) times(y[1], wh, wl, 1, 1);
+      }
+    }
+    bar_sync(1, 128);
+    if (mine) {
+      emit(y[0], 2 + w, 0);
+      emit(y[1], 2 + w, 1);
     }
   };
   make_gates(0);  // while the rows are on their way
@@ -472,6 +545,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
           *reinterpret_cast<__half*>(sm.img[e].t_hi + at) = vh;
           *reinterpret_cast<__half*>(sm.img[e].t_lo + at) = __float2half_rn(x[i] - __half2float(vh));
         }
+      if (p.whole) invert_below(e0);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
@@ -487,57 +561,39 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
   if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// ---------------------------------------------------------------- chunked form, second kernel
-// Bound by the chain of chunks and the instructions of the one warp (two with NW = 8) on each scheduler: 8192 tokens
+// ---------------------------------------------------------------- chunked form, second kernel, few heads
+// Bound by the chain of chunks and the instructions of the one warp on each scheduler: 8192 tokens
 // of 32 heads 0.36 ms, 2.8 us a chunk, tensor cores 47 % busy.  (Four warps to 16 rows: 0.52 ms.)
-// NW warps; the key columns of 16 value rows are shared by KS of them (1 or 2).  With two, each
-// warp has half of S: X and S Q^T are added up through shared memory, both solve for N, and each
-// updates its half of S and makes the output of half the tokens.
-template <int NW, int KS>
-struct CsCfg {
-  static constexpr int GROUPS = NW / KS, ROWS = GROUPS * 16, PARTS = 128 / ROWS;
-  static constexpr int V_BOXES = ROWS > 64 ? 2 : 1;
-  // four warps leave room for one more that requests the chunks; of eight, the first does it beside its work
-  static constexpr bool LOADER = NW == 4;
-  static constexpr int THREADS = (NW + (LOADER ? 1 : 0)) * 32;
-};
+// Four CTAs a head with 32 value rows each; two warps share 16 rows: each
+// has half of S's key columns, X and S Q^T are added up through shared memory, both solve for N, and each
+// updates its half of S and makes the output of half the tokens.  A fifth warp requests the chunks.
+constexpr int CS_WARPS = 4, CS_GROUPS = 2, CS_ROWS = CS_GROUPS * 16, CS_PARTS = 128 / CS_ROWS, CS_THREADS = CS_WARPS * 32 + 32;
+constexpr int CS_STAGES = 3;
 
-template <int NW, int KS>
 struct CsStage {  // one chunk
   alignas(1024) uint8_t k[CK_C * 256];
-  uint8_t q[CK_C * 256], v[CsCfg<NW, KS>::V_BOXES * CK_C * 128];
+  uint8_t q[CK_C * 256], v[CK_C * 128];
   CkImage img;
 };
 
-constexpr int CS_STAGES = 3;
-
-template <int NW, int KS>
 struct CsSmem {
-  CsStage<NW, KS> stage[CS_STAGES];
-  uint8_t out[NW][16 * 48];
-  float4 swap[KS > 1 ? NW : 1][KS > 1 ? 12 : 1][32];  // a warp's X, and S Q^T of the other's tokens
+  CsStage stage[CS_STAGES];
+  uint8_t out[CS_WARPS][16 * 48];
+  float4 swap[CS_WARPS][12][32];  // a warp's X, and S Q^T of the other's tokens
   uint64_t full[CS_STAGES], empty[CS_STAGES];
 };
-static_assert(sizeof(CsSmem<8, 1>) + 1024 <= MAX_DYN_SMEM && sizeof(CsSmem<4, 2>) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
+static_assert(sizeof(CsSmem) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
 
 __device__ __forceinline__ void plus4(float* x, const float4& y) {
   const float2 a = unpack2(add2(pack2(x[0], x[1]), pack2(y.x, y.y))), b = unpack2(add2(pack2(x[2], x[3]), pack2(y.z, y.w)));
   x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 
-// Two accumulator tiles [16, 8] as a left operand [16, 16], in two parts
 __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
   split_bf16x2(x[0][0], x[0][1], hi[0], lo[0]);
   split_bf16x2(x[0][2], x[0][3], hi[1], lo[1]);
   split_bf16x2(x[1][0], x[1][1], hi[2], lo[2]);
   split_bf16x2(x[1][2], x[1][3], hi[3], lo[3]);
-}
-
-__device__ __forceinline__ void ck_left_f16(const float (*x)[4], uint32_t* hi, uint32_t* lo) {
-  split_f16x2(x[0][0], x[0][1], hi[0], lo[0]);
-  split_f16x2(x[0][2], x[0][3], hi[1], lo[1]);
-  split_f16x2(x[1][0], x[1][1], hi[2], lo[2]);
-  split_f16x2(x[1][2], x[1][3], hi[3], lo[3]);
 }
 
 // A power of two that brings a row's largest value (over the four lanes that hold the row) into
@@ -588,20 +644,18 @@ __device__ __forceinline__ void ck_out_column(float (*O)[4], const uint32_t* nh,
       }
 }
 
-template <int NW, int KS>
-__global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
+__global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __grid_constant__ PrefillParams p,
                                                                   const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw[];
-  using C = CsCfg<NW, KS>;
-  CsSmem<NW, KS>& sm = *reinterpret_cast<CsSmem<NW, KS>*>(raw + (-smem_addr(raw) & 1023u));
-  constexpr int PARTS = C::PARTS, ROWS = C::ROWS, KT = 16 / KS;  // KT: tiles of S of a warp
+  CsSmem& sm = *reinterpret_cast<CsSmem*>(raw + (-smem_addr(raw) & 1023u));
+  constexpr int PARTS = CS_PARTS, ROWS = CS_ROWS, KT = 8;  // KT: tiles of S of a warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int heads = p.HV * PARTS;
   const int n = ck_by_length(p, blockIdx.x / heads, lane);
   const int part = blockIdx.x % heads, hv = part / PARTS, v0 = (part % PARTS) * ROWS;
   const SeqRange r = prefill_seq(p, n);
   if (r.slot < 0) {  // null slot: zero rows
-    for (int i = tid; i < (r.end - r.begin) * ROWS; i += NW * 32)
+    for (int i = tid; i < (r.end - r.begin) * ROWS; i += CS_THREADS)
       p.out[int64_t(r.begin + i / ROWS) * p.o_st + int64_t(hv) * p.o_sh + v0 + i % ROWS] = 0;
     griddep_wait();  // no CTA ends before the first kernel has
     return;
@@ -617,25 +671,24 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
   if (tid == 0) {
     for (int i = 0; i < CS_STAGES; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], NW);
+      mbar_init(&sm.empty[i], CS_WARPS);
     }
     fence_mbar_init();
   }
   __syncthreads();
   auto load = [&](int c) {  // one thread
-    CsStage<NW, KS>& st = sm.stage[c % CS_STAGES];
+    CsStage& st = sm.stage[c % CS_STAGES];
     uint64_t* bar = &sm.full[c % CS_STAGES];
     const int row = r.begin + c * CK_C;
-    mbar_arrive_expect_tx(bar, 2 * CK_C * 256 + C::V_BOXES * CK_C * 128 + CK_IMAGE_BYTES);
+    mbar_arrive_expect_tx(bar, 2 * CK_C * 256 + CK_C * 128 + CK_IMAGE_BYTES);
     for (int b = 0; b < 2; ++b) {
       ck_tma(smem_addr(st.k) + b * 8192, &map, (p.H + h) * 128 + b * 64, row, bar);
       ck_tma(smem_addr(st.q) + b * 8192, &map, h * 128 + b * 64, row, bar);
     }
-    for (int b = 0; b < C::V_BOXES; ++b)
-      ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + (v0 & 64) + b * 64, row, bar);
+    ck_tma(smem_addr(st.v), &map, (2 * p.H + hv) * 128 + (v0 & 64), row, bar);
     bulk_g2s(&st.img, images + int64_t(c) * p.HV * CK_IMAGE_BYTES, CK_IMAGE_BYTES, bar);
   };
-  if (C::LOADER && warp == NW) {
+  if (warp == CS_WARPS) {
     griddep_wait();  // the images
     if (lane == 0) {
       int c = 0;
@@ -648,13 +701,8 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
     }
     return;
   }
-  int issued = 0;  // of thread 0, where there is no loader
-  if (!C::LOADER) griddep_wait();
-  if (!C::LOADER && tid == 0)
-    for (; issued < CS_STAGES - 1 && issued < chunks; ++issued) load(issued);
-
   const int g = lane >> 2, t2 = 2 * (lane & 3);
-  const int vr = v0 + (warp % C::GROUPS) * 16, kh = KS > 1 ? warp / C::GROUPS : 0;  // the warp's value rows, its half of the keys
+  const int vr = v0 + (warp % CS_GROUPS) * 16, kh = warp / CS_GROUPS;  // the warp's value rows, its half of the keys
   // S as accumulators: tile n has rows g, g + 8 of the warp's 16 and key columns 8n + t2, + 1
   float* st = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(vr + g) * 128 + kh * KT * 8 + t2;
   float S[KT][4];
@@ -671,16 +719,16 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
   int c = 0;
   bool ok = true;
   for (; c < chunks; ++c) {
-    CsStage<NW, KS>& tl = sm.stage[c % CS_STAGES];
+    CsStage& tl = sm.stage[c % CS_STAGES];
     const CkImage& im = tl.img;
-    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v) + (C::V_BOXES > 1 ? (vr >> 6) * 8192 : 0);
+    const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v);
     ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
     if (!ok) break;
     const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
     if (valid < CK_C) {  // the last chunk
-      ck_zero_rows(tl.k, 2, valid, tid, NW * 32);
-      ck_zero_rows(tl.v, C::V_BOXES, valid, tid, NW * 32);
-      bar_sync(1, NW * 32);
+      ck_zero_rows(tl.k, 2, valid, tid, CS_WARPS * 32);
+      ck_zero_rows(tl.v, 1, valid, tid, CS_WARPS * 32);
+      bar_sync(1, CS_WARPS * 32);
     }
     float X[8][4], O[8][4];
 #pragma unroll
@@ -711,13 +759,7 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
           }
       }
     }
-    if (!C::LOADER && tid == 0 && issued < chunks) {
-      // the stage of the chunk before this one, which all warps have left by now or soon
-      if (c > 0) ok = mbar_wait_bounded(&sm.empty[issued % CS_STAGES], ((c - 1) / CS_STAGES) & 1, p.err);
-      if (!ok) break;
-      load(issued++);
-    }
-    if constexpr (KS > 1) {
+    {
       // the other half's X of all tokens and S Q^T of the tokens this warp writes out: blocks 0 and 3, or 1 and 2
 #pragma unroll
       for (int j = 0; j < 8; ++j) sm.swap[warp][j][lane] = make_float4(X[j][0], X[j][1], X[j][2], X[j][3]);
@@ -727,8 +769,8 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
         sm.swap[warp][8 + j][lane] = kh ? make_float4(O[mine][0], O[mine][1], O[mine][2], O[mine][3])
                                         : make_float4(O[other][0], O[other][1], O[other][2], O[other][3]);
       }
-      const int peer = warp ^ C::GROUPS;
-      bar_sync(2 + warp % C::GROUPS, 64);
+      const int peer = warp ^ CS_GROUPS;
+      bar_sync(2 + warp % CS_GROUPS, 64);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float4 y = sm.swap[peer][j][lane];
@@ -741,7 +783,7 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
         plus4(O[j < 2 ? j : j + 4], y);
         plus4(O[j + 2], y);
       }
-      bar_sync(2 + warp % C::GROUPS, 64);  // read before the next chunk's overwrite it
+      bar_sync(2 + warp % CS_GROUPS, 64);  // read before the next chunk's overwrite it
     }
     // R = beta V^T - (beta e^G rk) X
     float top0 = 0.f, top1 = 0.f;
@@ -837,19 +879,14 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
       }
     }
     // O += N P^T
-    if constexpr (KS == 1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, true, true);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, kh == 0, kh == 1);
-    }
+    for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, kh == 0, kh == 1);
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.empty[c % CS_STAGES])) : "memory");
     // O^T to token rows, 16 tokens at a time through the warp's own rows (48 bytes apart: no bank twice)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (KS > 1 && kh != (j == 1 || j == 2)) continue;
+      if (kh != (j == 1 || j == 2)) continue;
       __syncwarp();
       stsm_x4_t(os + (((lane >> 4) << 3) + (lane & 7)) * 48 + ((lane >> 3) & 1) * 16, cvt_bf16x2(O[2 * j][0] * down0, O[2 * j][1] * down0),
                 cvt_bf16x2(O[2 * j][2] * down1, O[2 * j][3] * down1), cvt_bf16x2(O[2 * j + 1][0] * down0, O[2 * j + 1][1] * down0),
@@ -861,10 +898,7 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
             *reinterpret_cast<const uint4*>(sm.out[warp] + (lane >> 1) * 48 + (lane & 1) * 16);
     }
   }
-  if (!ok) {  // a wait gave up (the error word says so): the state stays, copies in flight are waited for
-    for (; c < issued; ++c) mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
-    return;
-  }
+  if (!ok) return;  // a wait gave up (the error word says so): the state stays, the load warp waits for the copies in flight
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
     *reinterpret_cast<float2*>(st + i * 8) = make_float2(S[i][0], S[i][1]);
@@ -872,20 +906,365 @@ __global__ void __launch_bounds__(CsCfg<NW, KS>::THREADS, 1) prefill_scan_kernel
   }
 }
 
-template <int NW, int KS>
-cudaError_t scan(const PrefillParams& p, const CUtensorMap& map, cudaStream_t stream) {
-  static DynSmemCache cache;
-  constexpr int bytes = sizeof(CsSmem<NW, KS>) + 1024;
-  auto kern = prefill_scan_kernel<NW, KS>;
-  cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), bytes, cache);
-  if (e != cudaSuccess) return e;
-  // may be set up while the first kernel's last CTAs run: it waits for the images (griddep_wait)
-  return launch_behind(kern, dim3(unsigned(int64_t(p.N) * p.HV * CsCfg<NW, KS>::PARTS)), CsCfg<NW, KS>::THREADS, bytes, stream, p, map);
+// ---------------------------------------------------------------- chunked form, second kernel on tcgen05
+// One CTA a sequence and value head: the 128 value rows are the lanes of tensor memory.  Eight warps, two to a
+// quarter of the lanes, have half of the columns of a thread's row each (of S's keys, of the chunk's tokens).
+struct CtStage {  // one chunk
+  alignas(1024) uint8_t kq[2 * 16384];  // 64 columns of K and of Q, then the other 64: one right operand of 128 rows
+  uint8_t v[CK_C * 256];                // V, then the output
+  CkImage img;
+};
+
+struct CtSmem {
+  CtStage stage[CS_STAGES];
+  float top[2][128];
+  uint64_t full[CS_STAGES], empty[CS_STAGES];
+  uint64_t s_ready, x_done, r_ready, n_done, w_ready, u_done, f_ready, o_done;
+  uint64_t top_ready[4], out_ready[2], tail_ready;  // (waits that give up: a barrier would wait for a warp that has given up)
+  int abort;
+  uint32_t tmem;
+};
+static_assert(sizeof(CtSmem) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
+constexpr int CT_WARPS = 8, CT_THREADS = (CT_WARPS + 2) * 32;
+// tensor memory columns: S; its two bf16 parts, later the three of the weighted N; X = S K^T, later the two f16 parts of R;
+// S Q^T; N, later N P^T; the two f16 parts of N
+constexpr int CT_S = 0, CT_PARTS = 128, CT_X = 256, CT_Q = 320, CT_N = 384, CT_NF = 448;
+
+__global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __grid_constant__ PrefillParams p,
+                                                                        const __grid_constant__ CUtensorMap map) {
+  extern __shared__ uint8_t raw[];
+  CtSmem& sm = *reinterpret_cast<CtSmem*>(raw + (-smem_addr(raw) & 1023u));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = ck_by_length(p, blockIdx.x / p.HV, lane), hv = blockIdx.x % p.HV, h = hv / (p.HV / p.H);
+  const SeqRange r = prefill_seq(p, n);
+  if (r.slot < 0) {  // null slot: zero rows
+    for (int i = tid; i < (r.end - r.begin) * 128; i += CT_THREADS)
+      p.out[int64_t(r.begin + i / 128) * p.o_st + int64_t(hv) * p.o_sh + i % 128] = 0;
+    griddep_wait();  // no CTA ends before the first kernel has
+    return;
+  }
+  const bool fresh = p.has_init && !p.has_init[n * p.hi_s];
+  if (r.begin == r.end && !fresh) {
+    griddep_wait();
+    return;
+  }
+  const int chunks = (r.end - r.begin + CK_C - 1) / CK_C;
+  if (warp == CT_WARPS) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid == 0) {
+    for (int i = 0; i < CS_STAGES; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], CT_WARPS + 1);
+    }
+    mbar_init(&sm.s_ready, CT_WARPS);
+    mbar_init(&sm.r_ready, CT_WARPS);
+    mbar_init(&sm.w_ready, CT_WARPS);
+    mbar_init(&sm.f_ready, CT_WARPS);
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.out_ready[i], CT_WARPS / 2);
+    mbar_init(&sm.x_done, 1);
+    mbar_init(&sm.n_done, 1);
+    mbar_init(&sm.o_done, 1);
+    mbar_init(&sm.u_done, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&sm.top_ready[i], 2);
+    mbar_init(&sm.tail_ready, CT_WARPS);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const WarpWait wait{p.err, &sm.abort};
+  auto full = [&](int c) { return wait(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1); };
+  bool ok = true;
+
+  if (warp == CT_WARPS + 1) {
+    // ------------------------------------------------------------ load warp
+    griddep_wait();  // the images
+    const uint8_t* images = p.images + (int64_t(ck_first(r.begin, n)) * p.HV + hv) * CK_IMAGE_BYTES;
+    int c = 0;
+    for (; c < chunks; ++c) {
+      if (c >= CS_STAGES) ok = wait(&sm.empty[c % CS_STAGES], (c / CS_STAGES - 1) & 1);
+      if (!ok) break;
+      if (lane == 0) {
+        CtStage& st = sm.stage[c % CS_STAGES];
+        uint64_t* bar = &sm.full[c % CS_STAGES];
+        const int row = r.begin + c * CK_C;
+        mbar_arrive_expect_tx(bar, 3 * CK_C * 256 + CK_IMAGE_BYTES);
+        for (int b = 0; b < 2; ++b) {
+          ck_tma(smem_addr(st.kq) + b * 16384, &map, (p.H + h) * 128 + b * 64, row, bar);
+          ck_tma(smem_addr(st.kq) + b * 16384 + 8192, &map, h * 128 + b * 64, row, bar);
+          ck_tma(smem_addr(st.v) + b * 8192, &map, (2 * p.H + hv) * 128 + b * 64, row, bar);
+        }
+        bulk_g2s(&st.img, images + int64_t(c) * p.HV * CK_IMAGE_BYTES, CK_IMAGE_BYTES, bar);
+      }
+      __syncwarp();
+    }
+    if (!ok)  // copies in flight end before the CTA does
+      for (int k = max(c - CS_STAGES, 0); k < c; ++k) {
+        const uint64_t t = globaltimer_ns();
+        while (!mbar_try_wait(smem_addr(&sm.full[k % CS_STAGES]), (k / CS_STAGES) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
+        }
+      }
+  } else if (warp == CT_WARPS) {
+    // ------------------------------------------------------------ matrix warp
+    for (int c = 0; ok && c < chunks; ++c) {
+      CtStage& st = sm.stage[c % CS_STAGES];
+      const uint32_t lk = smem_addr(st.kq) >> 4;
+      ok = full(c) && wait(&sm.s_ready, c & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {  // S [K^T Q^T]
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          tc_mma_ts(tmem + CT_X, tmem + CT_PARTS + i * 8, tc_low_k() + lk + ((i >> 2) & 1) * 1024 + (i & 3) * 2, tc_idesc(2 * CK_C, false), i > 0);
+        tc_commit(&sm.x_done);
+      }
+      __syncwarp();
+      // [.., 64] += left [.., 64] in two parts times a triangular matrix in two parts, transposed
+      auto triangle = [&](int to, int left, const uint8_t* hi, const uint8_t* lo) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          const uint32_t right = tc_low_k() + (smem_addr(q == 2 ? lo : hi) >> 4), from = tmem + left + (q == 1 ? 32 : 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma_ts<TC_HIGH_32>(tmem + to + 16 * j, from + 8 * j, right + ck_block(j, j) / 16, tc_idesc_f16(CK_C - 16 * j), q + j > 0);
+        }
+      };
+      ok = wait(&sm.r_ready, c & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+        triangle(CT_N, CT_X, st.img.t_hi, st.img.t_lo);
+        tc_commit(&sm.n_done);
+      }
+      __syncwarp();
+      ok = wait(&sm.w_ready, c & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+#pragma unroll
+        for (int i = 0; i < 12; ++i)  // S += weighted N K
+          tc_mma_ts(tmem + CT_S, tmem + CT_PARTS + i * 8, tc_low_mn(16384) + lk + (i & 3) * 128, tc_idesc(128, true), 1);
+        tc_commit(&sm.u_done);
+      }
+      __syncwarp();
+      ok = wait(&sm.f_ready, c & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+        triangle(CT_N, CT_NF, st.img.p_hi, st.img.p_lo);
+        tc_commit(&sm.o_done);
+        tc_commit(&sm.empty[c % CS_STAGES]);
+      }
+      __syncwarp();
+    }
+    if (!ok) {  // tensor-core work in flight ends before its memory is given back
+      const uint64_t t = globaltimer_ns();
+      while (globaltimer_ns() - t < 1000000) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ a thread a value row
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t mem = tmem + (uint32_t(quarter) << 21);
+    float* state = p.state + int64_t(r.slot) * p.st_ss + int64_t(hv) * p.st_sh + int64_t(row) * 128 + half * 64;
+#pragma unroll 1
+    for (int i = 0; i < 64; i += 16) {
+      uint32_t w[16];
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const uint4 x = fresh ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(state + i + k);
+        w[k] = x.x, w[k + 1] = x.y, w[k + 2] = x.z, w[k + 3] = x.w;
+      }
+      tc_st16(mem + CT_S + half * 64 + i, w);
+    }
+    tc_wait_st();
+    auto announce = [&](uint64_t* bar) {
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    const int tok = half * 32;  // the thread's tokens of a chunk
+    float down = 0.f, sq[32];   // the row's scale, S q of its tokens: kept until the chunk's output is written
+    // The output of chunk c over V, then to memory in whole rows.  Called after the next chunk's products have begun.
+    auto finish = [&](int c) {
+      CtStage& st = sm.stage[c % CS_STAGES];
+      const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
+      if (!wait(&sm.o_done, c & 1)) return false;
+      tc_fence_after();
+      float y[32];
+      tc_ld32(mem + CT_N + tok, y);
+      tc_wait_ld();
+      uint8_t* v = st.v + (row >> 6) * 8192 + (row & 7) * 2;
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) {
+        const uint32_t w = cvt_bf16x2(fmaf(y[k], down, sq[k]), fmaf(y[k + 1], down, sq[k + 1]));
+        *reinterpret_cast<uint16_t*>(v + swz<128>(tok + k, (row & 63) >> 3)) = uint16_t(w);
+        *reinterpret_cast<uint16_t*>(v + swz<128>(tok + k + 1, (row & 63) >> 3)) = uint16_t(w >> 16);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.out_ready[half]);
+      if (!wait(&sm.out_ready[half], c & 1)) return false;
+      uint16_t* to = p.out + int64_t(t0) * p.o_st + int64_t(hv) * p.o_sh;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = tok + i * 8 + (tid & 127) / 16, j = tid & 15;
+        if (t < valid) *reinterpret_cast<uint4*>(to + t * p.o_st + j * 8) = *reinterpret_cast<const uint4*>(st.v + ck_at(t, j));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[c % CS_STAGES]);
+      return true;
+    };
+    for (int c = 0; c < chunks; ++c) {
+      CtStage& st = sm.stage[c % CS_STAGES];
+      const CkImage& im = st.img;
+      const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
+      ok = full(c);
+      if (ok && c) ok = wait(&sm.u_done, (c - 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (valid < CK_C) {  // the last chunk
+        ck_zero_rows(st.kq, 1, valid, tid, CT_WARPS * 32);
+        ck_zero_rows(st.kq + 16384, 1, valid, tid, CT_WARPS * 32);
+        ck_zero_rows(st.v, 2, valid, tid, CT_WARPS * 32);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.tail_ready);
+        ok = wait(&sm.tail_ready, 0);
+        if (!ok) break;
+      }
+      // S as two parts for the products, and decayed for what is added to it
+      {
+        const uint64_t total = pack2(im.total, im.total);
+#pragma unroll
+        for (int i = 0; i < 64; i += 32) {
+          float s[32];
+          tc_ld32(mem + CT_S + half * 64 + i, s);
+          tc_wait_ld();
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            split_bf16x2(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
+            scale2(s + 2 * k, total);
+          }
+          tc_st16(mem + CT_PARTS + half * 32 + i / 2, hi);
+          tc_st16(mem + CT_PARTS + 64 + half * 32 + i / 2, lo);
+          tc_st16(mem + CT_S + half * 64 + i, reinterpret_cast<uint32_t*>(s));
+          tc_st16(mem + CT_S + half * 64 + i + 16, reinterpret_cast<uint32_t*>(s) + 16);
+        }
+      }
+      announce(&sm.s_ready);
+      if (c) {
+        ok = finish(c - 1);
+        if (!ok) break;
+      }
+      // R = beta V^T - (beta e^G rk) X
+      {
+        float x[32];
+        uint64_t bv[16];
+        const uint8_t* v = st.v + (row >> 6) * 8192 + (row & 7) * 2;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float v0 = bf16_to_f(*reinterpret_cast<const uint16_t*>(v + swz<128>(tok + 2 * k, (row & 63) >> 3)));
+          const float v1 = bf16_to_f(*reinterpret_cast<const uint16_t*>(v + swz<128>(tok + 2 * k + 1, (row & 63) >> 3)));
+          bv[k] = mul2(pair_at(&im.beta[tok + 2 * k]), pack2(v0, v1));
+        }
+        ok = wait(&sm.x_done, c & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tc_ld32(mem + CT_X + tok, x);
+        tc_wait_ld();
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float2 y = unpack2(fma2(pack2(x[k], x[k + 1]), pair_at(&im.cx[tok + k]), bv[k / 2]));
+          x[k] = y.x, x[k + 1] = y.y;
+          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
+        // the row near one for f16, by the largest of all 64 tokens
+        sm.top[half][row] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.top_ready[quarter]);  // both warps have read X then, too
+        ok = wait(&sm.top_ready[quarter], c & 1);
+        if (!ok) break;
+        top = fmaxf(top, sm.top[half ^ 1][row]);
+        const int e = min(max(int(__float_as_uint(top) >> 23), 8), 250);
+        const float up = __uint_as_float(uint32_t(258 - e) << 23);
+        down = __uint_as_float(uint32_t(e - 4) << 23);
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) split_f16x2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
+        tc_st16(mem + CT_X + half * 16, hi);
+        tc_st16(mem + CT_X + 32 + half * 16, lo);
+      }
+      announce(&sm.r_ready);
+      // what is added to S first: the next chunk waits for it
+      tc_ld32(mem + CT_Q + tok, sq);
+      tc_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) scale2(sq + k, pair_at(&im.cq[tok + k]));
+      {
+        const uint64_t down2 = pack2(down, down);
+        ok = wait(&sm.n_done, c & 1);
+        if (!ok) break;
+        tc_fence_after();
+        float x[32];
+        tc_ld32(mem + CT_N + tok, x);
+        tc_wait_ld();
+        uint32_t hi[16], lo[16], rest[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float w[2] = {x[2 * k], x[2 * k + 1]};
+          scale2(w, mul2(pair_at(&im.cs[tok + 2 * k]), down2));
+          split3_bf16x2(w[0], w[1], hi[k], lo[k], rest[k]);
+        }
+        tc_st16(mem + CT_PARTS + half * 16, hi);
+        tc_st16(mem + CT_PARTS + 32 + half * 16, lo);
+        tc_st16(mem + CT_PARTS + 64 + half * 16, rest);
+        announce(&sm.w_ready);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) split_f16x2(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
+        tc_st16(mem + CT_NF + half * 16, hi);
+        tc_st16(mem + CT_NF + 32 + half * 16, lo);
+        announce(&sm.f_ready);
+      }
+    }
+    if (ok && chunks) ok = finish(chunks - 1);
+    if (ok && chunks) ok = wait(&sm.u_done, (chunks - 1) & 1);
+    if (ok) {  // (a wait that gave up leaves the state as it was)
+      tc_fence_after();
+#pragma unroll 1
+      for (int i = 0; i < 64; i += 32) {
+        float s[32];
+        tc_ld32(mem + CT_S + half * 64 + i, s);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(state + i + k) = make_float4(s[k], s[k + 1], s[k + 2], s[k + 3]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == CT_WARPS) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// May be set up while the first kernel's last CTAs run: they wait for the images (griddep_wait).
+template <class K>
+cudaError_t launch_scan(K kern, DynSmemCache& cache, int ctas, int threads, int smem, const PrefillParams& p, const CUtensorMap& map,
+                        cudaStream_t stream) {
+  const cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), smem + 1024, cache);
+  return e != cudaSuccess ? e : launch_behind(kern, dim3(unsigned(int64_t(p.N) * p.HV * ctas)), threads, smem + 1024, stream, p, map);
 }
 
 }  // namespace
 
-cudaError_t launch_prefill_chunk(const PrefillParams& p, int64_t longest, cudaStream_t stream) {
+cudaError_t launch_prefill_chunk(PrefillParams p, int64_t longest, cudaStream_t stream) {
   CUtensorMap map;
   // boxes of 64 columns x 64 tokens of mixed_qkv
   const uint64_t dims[2] = {uint64_t(2 * p.H + p.HV) * 128, uint64_t(p.T)};
@@ -898,17 +1277,16 @@ cudaError_t launch_prefill_chunk(const PrefillParams& p, int64_t longest, cudaSt
   e = ensure_dyn_smem(reinterpret_cast<const void*>(prefill_derive_kernel), bytes, cache);
   if (e != cudaSuccess) return e;
   const int64_t ids = int64_t(p.T) / CK_C + p.N;
+  // A head's 128 value rows on one multiprocessor (3.4 us a chunk), or on four, 32 each with their key columns halved
+  // (2.8 us, 12 us of multiprocessor time a head's chunk).
+  const int64_t chain = (longest + CK_C - 1) / CK_C, all = ids * p.HV / multiprocessor_count();
+  p.whole = std::max(all * 120, chain * 28) > std::max(all, chain) * 34;
   prefill_derive_kernel<<<dim3(unsigned(ids * p.H)), CD_THREADS, bytes, stream>>>(p, map);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // Three ways to put a head's value rows on multiprocessors: all 128 on one (7 us a chunk), 64 (3 to 4 us), or
-  // 32 with their key columns halved (2.8 us, 12 us of multiprocessor time a head's chunk).  What takes longest is the
-  // chunks of all sequences, spread over the machine, or those of the longest one after another: one
-  // prompt of 8192 tokens 0.85 ms / 0.51 ms / 0.42 ms, eight of 2048 tokens 0.55 ms / 0.59 ms / 0.77 ms.
-  const int64_t chain = (longest + CK_C - 1) / CK_C, all = ids * p.HV / multiprocessor_count();
-  const int64_t t8 = std::max(all * 72, chain * 66), t4 = std::max(all * 80, chain * 31), t2 = std::max(all * 120, chain * 28);
-  if (t2 < t4 && t2 < t8) return scan<4, 2>(p, map, stream);
-  return t4 < t8 ? scan<4, 1>(p, map, stream) : scan<8, 1>(p, map, stream);
+  static DynSmemCache tc_cache, scan_cache;
+  return p.whole ? launch_scan(prefill_scan_tc_kernel, tc_cache, 1, CT_THREADS, sizeof(CtSmem), p, map, stream)
+                 : launch_scan(prefill_scan_kernel, scan_cache, CS_PARTS, CS_THREADS, sizeof(CsSmem), p, map, stream);
 }
 
 // The longest sequence as the host knows it, or the mean length
