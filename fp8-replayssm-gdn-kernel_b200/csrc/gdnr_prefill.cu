@@ -162,14 +162,15 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 //   S = e^{G_C} S + N diag(e^{G_C - G_j} rk_j) K
 // (N [V, C] holds the tokens' new values).
 //
-// Two kernels.  The first makes what does not depend on the state, for all chunks at once: A with
-// its diagonal blocks of 16 tokens inverted, P, and the factors of each token, an image of
+// Two kernels.  The first makes what does not depend on the state, for all chunks at once: T = (I + A)^-1
+// or A with its diagonal blocks of 16 tokens inverted, P, and the factors of each token, an image of
 // 21 KB a chunk and head in the layout the second one's shared memory has.  The second
-// walks the chunks of a sequence.  It has value rows as the rows of the matrix products: a
-// warp that owns 16 value rows of S keeps S, X, R and N in registers, the accumulators of one
-// product are the left operand of the next, and nothing of the chain from one state to
-// the next passes through shared memory or waits for another warp.  N is solved for by blocks
-// (N_b = R_b T_bb^T, then R_i -= N_b A_ib^T for the blocks below).
+// walks the chunks of a sequence, with value rows as the rows of the matrix products, in one of two forms:
+//   tcgen05: a head's 128 value rows are the lanes of tensor memory, where S stays; N = R T^T.
+//   warp-level, where few heads leave multiprocessors over: a head on four of them.  Two warps share 16 value rows
+//   and keep S, X, R and N in registers; the accumulators of one product are the left operand of the
+//   next.  N is solved for by blocks (N_b = R_b T_bb^T, then R_i -= N_b A_ib^T for the blocks below): the whole
+//   T gained nothing here (0.353 ms a 8192-token prompt, not 0.361, for 8 us more in the first kernel).
 //
 // Rounding: K, Q, V are bf16 as they come.  A float32 matrix meets the tensor cores as a sum
 // of narrower ones, so that the float32 state stays within 1e-5 also where keys are alike and
@@ -248,8 +249,8 @@ struct CdSmem {
 };
 
 // One CTA a chunk and key head; its value heads share the products of the raw rows.  Bound by
-// instructions and barriers (three CTAs a multiprocessor; a 8192-token prompt of 16 / 32 heads: 56 us, 88 MB of
-// images).  The first four warps make A (rows of K against K) and invert its diagonal blocks, the others make P
+// instructions and barriers (three CTAs a multiprocessor; a 8192-token prompt of 16 / 32 heads: 50 us, 88 MB of
+// images; with the gates' loads one after another 56 us).  The first four warps make A (rows of K against K) and invert its diagonal blocks, the others make P
 // (rows of Q against K) and the factors.
 __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __grid_constant__ PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map) {
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
     }
   };
   // What lies below the diagonal blocks T_ii of T = (I + A)^-1, in the image, by halves of 32, then of 64 tokens: the
-  // block below two inverses is T_low (-A) T_top.  Two warps a head.  (In float32 on the other units it took 18 us of
-  // the kernel's 67, as products of f16 pairs 6.)
+  // block below two inverses is T_low (-A) T_top.  Two warps a head.  (12 ragged prompts of 32 heads: the kernel takes
+  // 41 us without it, 49 us with it, and 58 us with the products in float32 on the other units.)
   auto invert_below = [&](int e0) {
     const int e = warp >> 1, w = warp & 1;
     const bool mine = e0 + e < group;
@@ -580,7 +581,7 @@ struct CsSmem {
   CsStage stage[CS_STAGES];
   uint8_t out[CS_WARPS][16 * 48];
   float4 swap[CS_WARPS][12][32];  // a warp's X, and S Q^T of the other's tokens
-  uint64_t full[CS_STAGES], empty[CS_STAGES];
+  uint64_t full[CS_STAGES], empty[CS_STAGES], tail;
 };
 static_assert(sizeof(CsSmem) + 1024 <= MAX_DYN_SMEM, "one CTA per SM");
 
@@ -673,6 +674,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], CS_WARPS);
     }
+    mbar_init(&sm.tail, CS_WARPS);
     fence_mbar_init();
   }
   __syncthreads();
@@ -722,13 +724,14 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
     CsStage& tl = sm.stage[c % CS_STAGES];
     const CkImage& im = tl.img;
     const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v);
-    ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);
-    if (!ok) break;
+    ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);  // (the pair agrees on it below)
     const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
     if (valid < CK_C) {  // the last chunk
       ck_zero_rows(tl.k, 2, valid, tid, CS_WARPS * 32);
       ck_zero_rows(tl.v, 1, valid, tid, CS_WARPS * 32);
-      bar_sync(1, CS_WARPS * 32);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.tail);
+      ok = mbar_wait_bounded(&sm.tail, 0, p.err) && ok;
     }
     float X[8][4], O[8][4];
 #pragma unroll
@@ -770,7 +773,9 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
                                         : make_float4(O[other][0], O[other][1], O[other][2], O[other][3]);
       }
       const int peer = warp ^ CS_GROUPS;
-      bar_sync(2 + warp % CS_GROUPS, 64);
+      // the first of a pair's barriers also tells whether either's wait gave up: none is left waiting for the other
+      ok = !bar_or(2 + warp % CS_GROUPS, 64, !ok);
+      if (!ok) break;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float4 y = sm.swap[peer][j][lane];
@@ -908,7 +913,17 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
 
 // ---------------------------------------------------------------- chunked form, second kernel on tcgen05
 // One CTA a sequence and value head: the 128 value rows are the lanes of tensor memory.  Eight warps, two to a
-// quarter of the lanes, have half of the columns of a thread's row each (of S's keys, of the chunk's tokens).
+// quarter of the lanes, have half of the columns of a thread's row each (of S's keys, of the chunk's tokens); a ninth
+// issues the products, a tenth requests the chunks.  A chunk, as a chain:
+//   warps: S -> its two parts          | products: X = S K^T and S Q^T
+//   warps: R, near one, as two parts   | N = R T^T
+//   warps: weighted N as three parts   | S += it times K
+// and beside it N as two parts, N P^T, and the output of the chunk before.
+// 3.4 us a chunk (all 128 rows on warp-level tiles: 7.2 us); 12 prompts of up to 2047 tokens, 32 heads: 0.12 ms of
+// 0.17.  Bound by the 56 products of a chunk, 90 to 150 cycles each (64 at the full rate: the warps' loads and stores
+// of tensor memory run beside them), and the conversions between.  Slower were: sixteen warps; the output
+// taken out before X or after R; P T from the first kernel, which saves the N P^T products, was even (3.3 us a chunk,
+// 13 us more for the images).
 struct CtStage {  // one chunk
   alignas(1024) uint8_t kq[2 * 16384];  // 64 columns of K and of Q, then the other 64: one right operand of 128 rows
   uint8_t v[CK_C * 256];                // V, then the output
@@ -1278,7 +1293,9 @@ cudaError_t launch_prefill_chunk(PrefillParams p, int64_t longest, cudaStream_t 
   if (e != cudaSuccess) return e;
   const int64_t ids = int64_t(p.T) / CK_C + p.N;
   // A head's 128 value rows on one multiprocessor (3.4 us a chunk), or on four, 32 each with their key columns halved
-  // (2.8 us, 12 us of multiprocessor time a head's chunk).
+  // (2.8 us, 12 us of multiprocessor time a head's chunk).  What takes longest is the chunks of all sequences, spread
+  // over the machine, or those of the longest one after another.  32 heads: 8 prompts of 2048 tokens 0.34 / 0.72 ms,
+  // 64 of 64 tokens 0.18 / 0.31 ms, 2 of 2048 tokens 0.15 / 0.21 ms; 1 of 8192 tokens 0.50 / 0.40 ms.
   const int64_t chain = (longest + CK_C - 1) / CK_C, all = ids * p.HV / multiprocessor_count();
   p.whole = std::max(all * 120, chain * 28) > std::max(all, chain) * 34;
   prefill_derive_kernel<<<dim3(unsigned(ids * p.H)), CD_THREADS, bytes, stream>>>(p, map);
@@ -1294,8 +1311,8 @@ static int64_t longest_of(int64_t tokens, int64_t sequences, int max_seqlen) {
   return max_seqlen > 0 ? std::min<int64_t>(max_seqlen, tokens) : (tokens + sequences - 1) / sequences;
 }
 
-// At 64 sequences of 32 heads a token takes the token-by-token kernel 9 us (135 us at twelve), at 128 20 us; a chunk the other two
-// 235 us and 387 us: equal at about twenty tokens.  (One sequence: 0.3 us a token and 18 us a call.)
+// Twenty tokens a sequence token by token / as a chunk, 32 heads: 1 sequence 15 / 15 us, 12 sequences 50 / 50 us, 64 sequences
+// 216 / 215 us, 128 sequences 415 / 419 us.
 static bool prefill_chunked(int64_t tokens, int64_t sequences, int max_seqlen) { return longest_of(tokens, sequences, max_seqlen) > 20; }
 
 int64_t prefill_workspace_bytes(int64_t tokens, int64_t sequences, int64_t value_heads, int max_seqlen) {

@@ -54,6 +54,15 @@ __device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r
 
 // Named barriers: wait for `count` threads / arrive without waiting.
 __device__ __forceinline__ void bar_sync(int id, int count) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory"); }
+// ... and whether any of them has `x`
+__device__ __forceinline__ bool bar_or(int id, int count, bool x) {
+  int r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+               : "=r"(r)
+               : "r"(id), "r"(count), "r"(int(x))
+               : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void bar_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
