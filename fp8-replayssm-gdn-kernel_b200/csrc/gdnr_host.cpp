@@ -80,7 +80,13 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       return nullptr;
     }
     d.data = t.data_ptr();
-    if (!d.data) d.data = reinterpret_cast<void*>(16);  // an empty tensor is present
+    if (!d.data) {
+      if (t.numel() > 0) {  // a fake tensor, a wrapper subclass, a storage resized to nothing
+        PyErr_Format(PyExc_ValueError, "argument %zd has elements but no memory", i);
+        return nullptr;
+      }
+      d.data = reinterpret_cast<void*>(16);  // an empty tensor is present
+    }
     d.ndim = int32_t(t.dim());
     for (int64_t k = 0; k < t.dim(); ++k) {
       d.shape[k] = t.size(k);
