@@ -7,6 +7,7 @@
 //     address   of an entry point int f(const void* args, void* stream)
 //     tensors   tuple of CUDA tensors or None (absent), the leading gdnr_tensor fields
 //     tail      bytes of the argument structure behind them
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -33,7 +34,10 @@ int dtype_of(c10::ScalarType t) {
 
 constexpr Py_ssize_t MAX_TENSORS = 16, MAX_TAIL = 64;
 
+// Sizes, strides and addresses throw for tensors that have none (transforms' wrappers, sparse ones), as the guard
+// does for a missing device: all of it becomes a Python exception.
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 3 || !PyTuple_Check(args[1]) || !PyBytes_Check(args[2])) {
     PyErr_SetString(PyExc_TypeError, "call(address, tensors, tail)");
     return nullptr;
@@ -99,14 +103,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return nullptr;
   }
   std::memcpy(buf + size_t(n) * sizeof(gdnr_tensor), PyBytes_AS_STRING(args[2]), size_t(tail));
-  try {
-    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
-    void* const stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
-    return PyLong_FromLong(reinterpret_cast<int (*)(const void*, void*)>(address)(buf, stream));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  void* const stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
+  return PyLong_FromLong(reinterpret_cast<int (*)(const void*, void*)>(address)(buf, stream));
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {

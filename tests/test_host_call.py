@@ -2,6 +2,10 @@
 
 Fake tensors say that they are on a CUDA device and have shapes and strides, but no memory."""
 
+import pathlib
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -48,3 +52,33 @@ def test_tensors_on_two_devices_are_refused(fake):
     q, x = bf16(0, 4, 64), append_tensors("cuda:1")
     with pytest.raises(ValueError, match="one device"):
         gdnr.qk_norm_rope_append(q, *x[1:], q_out=q)
+
+
+IN_A_TRANSFORM = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+import gdnr
+from test_host_call import append_tensors, bf16
+
+with FakeTensorMode():
+    x = append_tensors()
+    def call(q):
+        return gdnr.qk_norm_rope_append(q, *x[1:], q_out=q).sum()
+    try:
+        {transform}
+    except RuntimeError as e:
+        print("raised:", str(e).splitlines()[0])
+"""
+
+
+@pytest.mark.parametrize("transform", ["torch.func.grad(call)(x[0])", "torch.func.vmap(call)(bf16(3, 2, 4, 64))"])
+def test_a_transform_raises_and_the_process_goes_on(transform):
+    """A transform's wrapper has no address: torch throws when it is asked for.  In a process of its own."""
+    here = pathlib.Path(__file__).resolve().parent
+    paths = [str(here), str(pathlib.Path(gdnr.__file__).resolve().parent.parent)]
+    run = subprocess.run([sys.executable, "-c", IN_A_TRANSFORM.format(paths=paths, transform=transform)], capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+    assert "raised: Cannot access data pointer" in run.stdout, run.stdout
