@@ -1129,6 +1129,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
         const int t = tok + i * 8 + (tid & 127) / 16, j = tid & 15;
         if (t < valid) *reinterpret_cast<uint4*>(to + t * p.o_st + j * 8) = *reinterpret_cast<const uint4*>(st.v + ck_at(t, j));
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the V of a later chunk there
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[c % CS_STAGES]);
       return true;

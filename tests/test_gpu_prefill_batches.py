@@ -111,3 +111,17 @@ def test_same_result_every_time(cuda_device):
     for _ in range(3):
         again, other = check(d, lens)
         assert torch.equal(first, again) and torch.equal(state, other)
+
+
+def test_stages_are_used_again_many_times(cuda_device):
+    """Twenty chunks a sequence through three stages, each chunk's output laid over its values before the next ones arrive there;
+    values of very different sizes from chunk to chunk, so that one that is not its own shows."""
+    lens = [1280, 1217, 1150, 1030, 1279, 1111, 1283, 1024]
+    d = inputs(119, lens, 16, 32)
+    t = torch.arange(sum(lens), device="cuda") // 64
+    d["mixed"][:, 32 * 128:] *= torch.tensor([1.0, 64.0, 0.25, 8.0, 512.0], device="cuda")[t % 5][:, None].bfloat16()
+    first, state = check(d, lens)
+    for _ in range(10):
+        again = d["state"].clone()
+        got = gdnr.gdn_prefill(d["mixed"], d["a"], d["b"], d["a_log"], d["dt_bias"], again, R.cu(lens), max_seqlen=max(lens))
+        assert torch.equal(first, got) and torch.equal(state, again)

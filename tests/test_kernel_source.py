@@ -1,0 +1,39 @@
+"""Orderings and ways out of the kernels that no run can show reliably, read from their source."""
+
+import pathlib
+import re
+
+CSRC = pathlib.Path(__file__).resolve().parent.parent / "fp8-replayssm-gdn-kernel_b200" / "csrc"
+
+
+def source(name):
+    """A source file without comments."""
+    text = (CSRC / name).read_text()
+    return re.sub(r"/\*.*?\*/", "", re.sub(r"//[^\n]*", "", text), flags=re.S)
+
+
+def block(text, head):
+    """What follows ``head``, to the brace that closes the first one opened behind it."""
+    assert text.count(head) == 1, (head, text.count(head))
+    at = text.index("{", text.index(head) + len(head))
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[at:i + 1]
+    raise AssertionError(head)
+
+
+def body(text, function):
+    """Body of the kernel or function of that name (its definition ends in an opening brace)."""
+    heads = re.findall(r"[^;}]*\b%s\([^;{]*\)\s*(?:const\s*)?(?=\{)" % function, text)
+    assert len(heads) == 1, (function, heads)
+    return block(text, heads[0].strip())
+
+
+def test_output_staged_over_a_tile_is_fenced_before_the_tile_is_given_back():
+    """Ordinary stores into memory that TMA writes next: a proxy fence between them and the arrival that frees it."""
+    finish = block(body(source("gdnr_prefill.cu"), "prefill_scan_tc_kernel"), "auto finish = ")
+    stored = finish.rindex("reinterpret_cast<uint16_t*>(v + swz")
+    freed = finish.index("mbar_arrive(&sm.empty")
+    assert "fence.proxy.async.shared::cta" in finish[stored:freed]
