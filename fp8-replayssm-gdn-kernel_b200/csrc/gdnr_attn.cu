@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
     for (int t = t0; t < t1; ++t, ++k) {
       const uint32_t st = k % STAGES, ks = kv_s + st * 2 * C::TILE, vs = ks + C::TILE;
       ok = wait(&full[st], (k / STAGES) & 1);
-      if (!ok) return;
+      if (!ok) break;  // straight to the unit's next barrier
       // the last page may end inside the tile: what its rows past the end hold (it may be NaN) must not meet a weight of zero
       const int from = u.s.kv - t * AT_BN;
       if (from < AT_BN) {
@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (WN > 1)
           __syncwarp();
-        else
-          bar_sync(1, C::CONSUMERS);
+        else if (bar_or(1, C::CONSUMERS, false))
+          return;
       }
       float s[NT][4];
 #pragma unroll
@@ -502,7 +502,9 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
     }
-    bar_sync(1, C::CONSUMERS);  // every warp is done with the query rows and the last tile
+    // Every warp is done with the query rows and the last tile.  The first barrier that a warp meets after a wait also tells
+    // whether any warp's wait gave up: then all leave, none is left at a barrier that another does not come to.
+    if (bar_or(1, C::CONSUMERS, !ok)) return;
     const bool whole = t0 == 0 && t1 == u.tiles;
     float* part = ws_o + (t0 > 0 ? 0 : 1) * BM * (D + 2);
     if constexpr (WN == 1) {

@@ -37,3 +37,16 @@ def test_output_staged_over_a_tile_is_fenced_before_the_tile_is_given_back():
     stored = finish.rindex("reinterpret_cast<uint16_t*>(v + swz")
     freed = finish.index("mbar_arrive(&sm.empty")
     assert "fence.proxy.async.shared::cta" in finish[stored:freed]
+
+
+def test_consumers_of_attention_leave_together():
+    """A warp whose bounded wait gave up must not leave while others go on to a barrier that counts it: between a wait and the next
+    barrier there is no way out, and that barrier tells all of them."""
+    consumers = block(body(source("gdnr_attn.cu"), "attn_stream_kernel").split("const int wm = warp / WN")[1], "for (int64_t at = share.begin")
+    tiles = block(consumers, "for (int t = t0; t < t1; ++t, ++k)")
+    assert re.search(r"ok = wait\(&full\[st\][^;]*;\s*if \(!ok\) break;", tiles)
+    assert "bar_sync" not in tiles
+    returns = re.findall(r"if \(([^;{}]*)\)\s*return;", consumers)
+    assert len(returns) == consumers.count("return") and all(r.startswith("bar_or(1, C::CONSUMERS, ") for r in returns), returns
+    after = consumers[consumers.index(tiles) + len(tiles):]
+    assert re.match(r"[^;]*\bfor [^{]*\{[^}]*\}\s*if \(bar_or\(1, C::CONSUMERS, !ok\)\) return;", after), after[:300]
