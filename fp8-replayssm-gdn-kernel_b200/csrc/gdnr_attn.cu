@@ -355,12 +355,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
         }
       }
     }
-    if (!ok)  // copies in flight end before the CTA does
-      for (uint32_t j = k > STAGES ? k - STAGES : 0; j < k; ++j) {
-        const uint64_t t = globaltimer_ns();
-        while (!mbar_try_wait(smem_addr(&full[j % STAGES]), (j / STAGES) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
-        }
-      }
+    drain(full, STAGES, k);
     // a CTA does not end before the kernel that this one may run beside has: what comes next waits for this one only
     griddep_wait();
     return;

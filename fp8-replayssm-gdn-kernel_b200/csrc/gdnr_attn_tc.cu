@@ -177,18 +177,8 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
         }
       }
     }
-    if (!ok) {  // copies in flight end before the CTA does
-      for (int q = 0; q < NQ; ++q) {
-        const uint64_t t = globaltimer_ns();
-        while (nq[q] && !mbar_try_wait(smem_addr(&bars.q_full[q]), (nq[q] - 1) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
-        }
-      }
-      for (uint32_t k = slot > C::RING ? slot - C::RING : 0; k < slot; ++k) {
-        const uint64_t t = globaltimer_ns();
-        while (!mbar_try_wait(smem_addr(&bars.kv_full[k % C::RING]), (k / C::RING) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
-        }
-      }
-    }
+    for (int q = 0; q < NQ; ++q) drain(&bars.q_full[q], 1, nq[q]);
+    drain(bars.kv_full, C::RING, slot);
   } else if (warp == C::SOFTMAX_WARPS) {
     // ------------------------------------------------------------ matrix warp
     tc_regs_dec<C::NQ == 2, C::OTHER_REGS>();

@@ -393,7 +393,10 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
   make_gates(0);  // while the rows are on their way
   __syncthreads();  // the barrier is initialised
   const bool ok = mbar_wait_bounded(&sm.bar, 0, p.err);
-  if (__syncthreads_or(!ok)) return;
+  if (__syncthreads_or(!ok)) {
+    if (tid == 0) drain(&sm.bar, 1, 1);
+    return;
+  }
   if (valid < CK_C) {
     ck_zero_rows(sm.k, 2, valid, tid, CD_THREADS);
     ck_zero_rows(sm.q, 2, valid, tid, CD_THREADS);
@@ -698,8 +701,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
         if (c >= CS_STAGES && !mbar_wait_bounded(&sm.empty[c % CS_STAGES], (c / CS_STAGES - 1) & 1, p.err)) break;
         load(c);
       }
-      if (c < chunks)  // a wait gave up: copies in flight are waited for
-        for (int k = max(c - CS_STAGES, 0); k < c; ++k) mbar_wait_bounded(&sm.full[k % CS_STAGES], (k / CS_STAGES) & 1, p.err);
+      drain(sm.full, CS_STAGES, c);
     }
     return;
   }
@@ -1016,12 +1018,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
       }
       __syncwarp();
     }
-    if (!ok)  // copies in flight end before the CTA does
-      for (int k = max(c - CS_STAGES, 0); k < c; ++k) {
-        const uint64_t t = globaltimer_ns();
-        while (!mbar_try_wait(smem_addr(&sm.full[k % CS_STAGES]), (k / CS_STAGES) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
-        }
-      }
+    drain(sm.full, CS_STAGES, c);
   } else if (warp == CT_WARPS) {
     // ------------------------------------------------------------ matrix warp
     for (int c = 0; ok && c < chunks; ++c) {

@@ -155,6 +155,15 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// Copies in flight end before their CTA does: waits until the last tiles of a ring, `tiles` in all, have landed (one limit for
+// all of them).  Whoever requests tiles calls it before leaving, whether its own waits gave up or only those of the others.
+__device__ __forceinline__ void drain(uint64_t* full, uint32_t stages, uint32_t tiles) {
+  const uint64_t t = globaltimer_ns();
+  for (uint32_t k = tiles > stages ? tiles - stages : 0; k < tiles; ++k)
+    while (!mbar_try_wait(smem_addr(&full[k % stages]), (k / stages) & 1) && globaltimer_ns() - t < WAIT_LIMIT_NS) {
+    }
+}
+
 // Waits of a whole warp; they give up after a second, or when another warp has: then every role leaves its loop.
 struct WarpWait {
   uint32_t* err;

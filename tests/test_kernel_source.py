@@ -50,3 +50,18 @@ def test_consumers_of_attention_leave_together():
     assert len(returns) == consumers.count("return") and all(r.startswith("bar_or(1, C::CONSUMERS, ") for r in returns), returns
     after = consumers[consumers.index(tiles) + len(tiles):]
     assert re.match(r"[^;]*\bfor [^{]*\{[^}]*\}\s*if \(bar_or\(1, C::CONSUMERS, !ok\)\) return;", after), after[:300]
+
+
+def test_copies_in_flight_land_whoever_gave_up():
+    """A warp that requests tiles waits for the last of them also where its own waits were all met: no condition before it."""
+    attn, tc, prefill = (source(f) for f in ("gdnr_attn.cu", "gdnr_attn_tc.cu", "gdnr_prefill.cu"))
+    for text, kernel, drains in ((attn, "attn_stream_kernel", ["drain(full, STAGES, k);"]),
+                                 (tc, "attn_tc_kernel", ["drain(&bars.q_full[q], 1, nq[q]);", "drain(bars.kv_full, C::RING, slot);"]),
+                                 (prefill, "prefill_scan_kernel", ["drain(sm.full, CS_STAGES, c);"]),
+                                 (prefill, "prefill_scan_tc_kernel", ["drain(sm.full, CS_STAGES, c);"])):
+        for drain in drains:
+            before = body(text, kernel).split(drain)
+            assert len(before) == 2, (kernel, drain)
+            assert not re.search(r"if \([^)]*\)\s*$", before[0]), (kernel, before[0][-80:])
+    derive = body(prefill, "prefill_derive_kernel")
+    assert "drain(&sm.bar, 1, 1);" in block(derive, "if (__syncthreads_or(!ok)) ")
