@@ -77,6 +77,7 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     if (mbar_try_wait(a, parity)) return true;
     if ((it & 255u) == 0 && globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
   }
+  if (mbar_try_wait(a, parity)) return true;  // the thread itself may have been held up since it last looked
   atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
   return false;
 }

@@ -183,6 +183,7 @@ struct WarpWait {
         if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) break;
       }
     }
+    if (mbar_try_wait(a, parity)) return true;  // the warp itself may have been held up since it last looked
     *abort = 1;
     atomicOr(err, GDNR_DEVERR_WAIT_TIMEOUT);
     return false;

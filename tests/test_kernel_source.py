@@ -65,3 +65,11 @@ def test_copies_in_flight_land_whoever_gave_up():
             assert not re.search(r"if \([^)]*\)\s*$", before[0]), (kernel, before[0][-80:])
     derive = body(prefill, "prefill_derive_kernel")
     assert "drain(&sm.bar, 1, 1);" in block(derive, "if (__syncthreads_or(!ok)) ")
+
+
+def test_a_wait_looks_once_more_before_it_reports_a_timeout():
+    """The clock may have run out because the waiting thread itself was held up, with the barrier complete meanwhile."""
+    for name, wait in (("gdnr_tile.cuh", "slow"), ("gdnr_device.cuh", "mbar_wait_bounded")):
+        text = body(source(name), wait)
+        behind = text[text.index(block(text, "for (")):]
+        assert "if (mbar_try_wait(a, parity)) return true;" in behind[len(block(text, "for (")):behind.index("atomicOr")], name
