@@ -301,13 +301,16 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
   uint64_t *const full = sh.full, *const empty = sh.empty;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t kv_s = smem_addr(raw) + 1024, q_s = kv_s + STAGES * 2 * C::TILE;
+  float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
+  int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
   if (kv_s & 1023u) {  // the swizzled tiles would not be where the products look for them
-    if (tid == 0) atomicOr(p.err, GDNR_DEVERR_LAYOUT);
+    if (tid == 0) {
+      atomicOr(p.err, GDNR_DEVERR_LAYOUT);
+      meta[0] = -1;  // nothing to join
+    }
     griddep_wait();
     return;
   }
-  float* const ws_o = p.ws + int64_t(blockIdx.x) * 2 * BM * (D + 2);
-  int* const meta = reinterpret_cast<int*>(p.ws + int64_t(gridDim.x) * 2 * BM * (D + 2)) + blockIdx.x * AT_META;
 
   constexpr int WARPS = WM * WN + 1;
   static_assert(WARPS == 5, "AsShared::places");

@@ -73,3 +73,14 @@ def test_a_wait_looks_once_more_before_it_reports_a_timeout():
         text = body(source(name), wait)
         behind = text[text.index(block(text, "for (")):]
         assert "if (mbar_try_wait(a, parity)) return true;" in behind[len(block(text, "for (")):behind.index("atomicOr")], name
+
+
+def test_every_share_leaves_a_record_for_the_join():
+    """The join reads a record of each CTA from a workspace that holds anything: no way out before it is written."""
+    for name, kernel in (("gdnr_attn.cu", "attn_kernel"), ("gdnr_attn.cu", "attn_stream_kernel"), ("gdnr_attn_tc.cu", "attn_tc_kernel")):
+        text = body(source(name), kernel)
+        before = re.split(r"write_meta<T>|WarpWait wait\{", text)[0].split("return;")
+        for way_out in before[:-1]:
+            assert "meta[0] = -1" in way_out, (kernel, way_out[-200:])
+    tc = body(source("gdnr_attn_tc.cu"), "attn_tc_kernel")
+    assert re.search(r"write_meta<T>[^}]*\}\s*else if \(tid == 0\) \{\s*meta\[0\] = -1;", tc)
