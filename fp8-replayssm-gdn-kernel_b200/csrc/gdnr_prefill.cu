@@ -195,7 +195,8 @@ struct CkImage {
   // t: diagonal blocks: (I + A)^-1 of the block, below them: -A; or (whole) T = (I + A)^-1
   uint8_t t_hi[CK_TRI], t_lo[CK_TRI], p_hi[CK_TRI], p_lo[CK_TRI];
   float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, -beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
-  float pad[15];
+  uint32_t made;  // 1: all of it is there; 0: the first kernel's wait gave up
+  float pad[14];
 };
 static_assert(sizeof(CkImage) == CK_IMAGE_BYTES && sizeof(CkImage) % 16 == 0, "copied in bulk");
 
@@ -394,6 +395,9 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
   __syncthreads();  // the barrier is initialised
   const bool ok = mbar_wait_bounded(&sm.bar, 0, p.err);
   if (__syncthreads_or(!ok)) {
+    // the second kernel must not take what lies in the workspace for this chunk's images
+    for (int e = tid; e < group; e += CD_THREADS)
+      reinterpret_cast<CkImage*>(p.images + (int64_t(id) * p.HV + h * group + e) * CK_IMAGE_BYTES)->made = 0;
     if (tid == 0) drain(&sm.bar, 1, 1);
     return;
   }
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
         img.cx[gt] = -be * ex * sm.rk[gt];
         img.cq[gt] = ex * sm.rq[gt];
         img.cs[gt] = ex2_approx((ch - gh) + (cl - gl)) * sm.rk[gt];
-        if (gt == 0) img.total = ex2_approx(ch + cl);
+        if (gt == 0) img.total = ex2_approx(ch + cl), img.made = 1;
       }
       // the rows of the three blocks that this thread's units lie in
       float rh[3][2], rl[3][2], rb[3][2];
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
     CsStage& tl = sm.stage[c % CS_STAGES];
     const CkImage& im = tl.img;
     const uint32_t ks = smem_addr(tl.k), qs = smem_addr(tl.q), vs = smem_addr(tl.v);
-    ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err);  // (the pair agrees on it below)
+    ok = mbar_wait_bounded(&sm.full[c % CS_STAGES], (c / CS_STAGES) & 1, p.err) && im.made;  // (the pair agrees on it below)
     const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
     if (valid < CK_C) {  // the last chunk
       ck_zero_rows(tl.k, 2, valid, tid, CS_WARPS * 32);
@@ -905,7 +909,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
             *reinterpret_cast<const uint4*>(sm.out[warp] + (lane >> 1) * 48 + (lane & 1) * 16);
     }
   }
-  if (!ok) return;  // a wait gave up (the error word says so): the state stays, the load warp waits for the copies in flight
+  if (!ok) return;  // a wait gave up, here or in the first kernel (the error word says so): the state stays
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
     *reinterpret_cast<float2*>(st + i * 8) = make_float2(S[i][0], S[i][1]);
@@ -1136,6 +1140,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
       const CkImage& im = st.img;
       const int t0 = r.begin + c * CK_C, valid = min(CK_C, r.end - t0);
       ok = full(c);
+      if (ok && !im.made) ok = false, sm.abort = 1;
       if (ok && c) ok = wait(&sm.u_done, (c - 1) & 1);
       if (!ok) break;
       tc_fence_after();
@@ -1247,7 +1252,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
     }
     if (ok && chunks) ok = finish(chunks - 1);
     if (ok && chunks) ok = wait(&sm.u_done, (chunks - 1) & 1);
-    if (ok) {  // (a wait that gave up leaves the state as it was)
+    if (ok) {  // (a wait that gave up, here or in the first kernel, leaves the state as it was)
       tc_fence_after();
 #pragma unroll 1
       for (int i = 0; i < 64; i += 32) {

@@ -84,3 +84,17 @@ def test_every_share_leaves_a_record_for_the_join():
             assert "meta[0] = -1" in way_out, (kernel, way_out[-200:])
     tc = body(source("gdnr_attn_tc.cu"), "attn_tc_kernel")
     assert re.search(r"write_meta<T>[^}]*\}\s*else if \(tid == 0\) \{\s*meta\[0\] = -1;", tc)
+
+
+def test_a_chunk_without_images_stops_the_scan():
+    """Where the first kernel's wait gave up the workspace holds anything: it says so, and neither scan stores a state made of it."""
+    text = source("gdnr_prefill.cu")
+    assert re.search(r"->made = 0;", block(body(text, "prefill_derive_kernel"), "if (__syncthreads_or(!ok)) "))
+    assert "img.made = 1;" in body(text, "prefill_derive_kernel")
+    for kernel, agreed in (("prefill_scan_kernel", "bar_or("), ("prefill_scan_tc_kernel", "announce(&sm.s_ready)")):
+        scan = body(text, kernel)
+        looked = scan.index("im.made")
+        assert looked < scan.index(agreed), kernel
+        assert re.search(r"if \(!ok\) (break|return);", scan[looked:scan.index(agreed) + 200]), kernel
+    assert re.search(r"if \(!ok\) return;\s*#pragma unroll", body(text, "prefill_scan_kernel"))
+    assert re.search(r"if \(ok\) \{\s*tc_fence_after", body(text, "prefill_scan_tc_kernel"))
