@@ -817,7 +817,20 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
       }
     }
     // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
+    // The row of O is scaled alike.  Where next to nothing is written (beta of zero) and S is not small, that must not
+    // overflow: R then counts as 2^-96 of O at least, far less than what float32 keeps of S beside it.
+    if (__any_sync(0xffffffffu, fminf(top0, top1) < 0x1p-60f)) {
+      float o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 cq = unpack2(pair_at(&im.cq[j * 8 + t2]));
+        o0 = fmaxf(o0, fmaxf(fabsf(O[j][0] * cq.x), fabsf(O[j][1] * cq.y)));
+        o1 = fmaxf(o1, fmaxf(fabsf(O[j][2] * cq.x), fabsf(O[j][3] * cq.y)));
+      }
+      top0 = fmaxf(top0, o0 * 0x1p-96f), top1 = fmaxf(top1, o1 * 0x1p-96f);
+    }
     float up0, down0, up1, down1;
+    ck_row_scale(top0, up0, down0);
     ck_row_scale(top0, up0, down0);
     ck_row_scale(top1, up1, down1);
     const uint64_t up0_2 = pack2(up0, up0), up1_2 = pack2(up1, up1);

@@ -217,3 +217,13 @@ def test_gates_of_minus_infinity(cuda_device, lens):
 def test_many_sequences(cuda_device):
     lens = [1 + (7 * i) % 90 for i in range(60)]
     check(inputs(16, lens, 1, 2), lens, fresh=[i % 3 == 0 for i in range(60)])
+
+
+@pytest.mark.parametrize("lens,h,hv", [([70, 200], 2, 4), ([3, 1], 2, 4), ([64, 70, 130, 64, 90, 64, 65, 64, 100, 64], 16, 32)])
+@pytest.mark.parametrize("b", [-200.0, -85.0])
+def test_nothing_written_beside_a_large_state(cuda_device, lens, h, hv, b):
+    """beta of zero, or next to it, and outputs of hundreds: what is written and what is read differ by 2^100 and more."""
+    d = inputs(17, lens, h, hv, decay="weak")
+    d["b"].fill_(b)
+    d["state"] *= 20000
+    check(d, lens)
