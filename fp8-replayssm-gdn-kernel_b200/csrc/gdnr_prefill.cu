@@ -605,11 +605,11 @@ __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint3
 }
 
 // A power of two that brings a row's largest value (over the four lanes that hold the row) into
-// [2^4, 2^5), and its inverse
+// [2^4, 2^5), and its inverse.  At most 2^115: the factors of O, up to 2^7 (a query of zeros), times it stay finite.
 __device__ __forceinline__ void ck_row_scale(float top, float& up, float& down) {
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int e = min(max(int(__float_as_uint(top) >> 23), 8), 250);
+  const int e = min(max(int(__float_as_uint(top) >> 23), 16), 250);
   up = __uint_as_float(uint32_t(258 - e) << 23);
   down = __uint_as_float(uint32_t(e - 4) << 23);
 }

@@ -227,3 +227,29 @@ def test_nothing_written_beside_a_large_state(cuda_device, lens, h, hv, b):
     d["b"].fill_(b)
     d["state"] *= 20000
     check(d, lens)
+
+
+@pytest.mark.parametrize("lens,h,hv", [([70, 130], 2, 4), ([3, 1], 2, 4), ([64, 70, 130, 64, 90, 64, 65, 64, 100, 64], 16, 32)])
+@pytest.mark.parametrize("part", ["all", "values and some queries", "keys"])
+def test_zeros(cuda_device, lens, h, hv, part):
+    """What a dry run gives: nothing is written and nothing read, but norms of zero have factors of up to 1e3."""
+    d = inputs(18, lens, h, hv)
+    if part == "all":
+        d["mixed"].zero_()
+    elif part == "keys":
+        d["mixed"][:, h * 128:2 * h * 128] = 0
+    else:
+        d["mixed"][:, 2 * h * 128:] = 0
+        d["mixed"][::3, :h * 128] = 0
+    d["state"].zero_()
+    got, state = check(d, lens)
+    assert (got == 0).all() and (state == 0).all()
+
+
+@pytest.mark.parametrize("lens,h,hv", [([70, 130], 2, 4), ([3, 1], 2, 4), ([64, 70, 130, 64, 90, 64, 65, 64, 100, 64], 16, 32)])
+def test_small_state_and_no_values(cuda_device, lens, h, hv):
+    """A state far below one, still far inside float32's range, that the tokens only correct: as exact as any other."""
+    d = inputs(19, lens, h, hv, decay="weak")
+    d["mixed"][:, 2 * h * 128:] = 0
+    d["state"] *= 1e-25
+    check(d, lens)
