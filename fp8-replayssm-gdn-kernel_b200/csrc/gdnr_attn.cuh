@@ -256,10 +256,11 @@ __device__ __forceinline__ int64_t out_at(const AttnParams& p, const Unit& u, in
   return int64_t(u.s.q0 + t) * p.o_st + int64_t(u.h * p.G + row - t * p.G) * p.o_sh;
 }
 
+// -inf marks a row that saw no place (a sum of zero); a sum of NaN, from a NaN in the row or in a key it saw, stays one.
 __device__ __forceinline__ void write_lse(const AttnParams& p, const SeqLen& s, int h, int row, float max2, float sum) {
   if (!p.lse) return;
   const int t = token_of(p, row);
-  p.lse[int64_t(s.q0 + t) * p.l_st + int64_t(h * p.G + row - t * p.G) * p.l_sh] = sum > 0.f ? (max2 + log2f(sum)) * LN2 : -INFINITY;
+  p.lse[int64_t(s.q0 + t) * p.l_st + int64_t(h * p.G + row - t * p.G) * p.l_sh] = sum == 0.f ? -INFINITY : (max2 + log2f(sum)) * LN2;
 }
 
 // ---------------------------------------------------------------- keys and values by TMA
