@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(32 * WM * WN) attn_kernel(const __grid_constan
     const int rows = u.s.m * p.G - u.rt * BM;  // rows of the sequence from this tile on
     const int row_base = u.rt * BM;
     const int32_t* table = p.table + int64_t(u.n) * p.tb_s;
-    if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+    if (tid == 0) report_unit(p, u);
     // query rows of the tile; rows beyond the sequence's are zeros
     for (int i = tid; i < BM * CH; i += C::THREADS) {
       const int r = i / CH, c = i % CH;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
     const int t0 = part_of.begin, t1 = part_of.end;
     if (t1 <= t0) continue;
     const int row_base = u.rt * BM, rows = u.s.m * p.G - row_base;  // rows of the sequence from this tile on
-    if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+    if (tid == 0) report_unit(p, u);
     // query rows of the tile; rows beyond the sequence's are zeros
     for (int i = tid; i < BM * CH; i += C::CONSUMERS) {
       const int r = i / CH, c = i % CH;

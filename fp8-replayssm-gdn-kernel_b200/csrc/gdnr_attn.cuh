@@ -250,6 +250,17 @@ __device__ __forceinline__ bool cut_unit(const int* metas, int i, CutUnit& c) {
   return a.x >= 0 && before >= a.w;  // else share i - 1 continues the unit, too
 }
 
+// What a unit's sequence has that is not in order (one thread).  Only a length that is zero or fills the block table may have
+// been cut by seq_len: only then is it read again.
+__device__ __forceinline__ void report_unit(const AttnParams& p, const Unit& u) {
+  const int64_t most = int64_t(p.width) * p.page_size;
+  if (u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+  if (u.s.kv == 0 || u.s.kv == most) {
+    const int kv = p.kv_lens[u.n * p.kl_s];
+    if (kv < 0 || kv > most) atomicOr(p.err, GDNR_DEVERR_BAD_SLOT);
+  }
+}
+
 // Row r of a sequence: token q0 + r / G, query head h G + r % G.
 __device__ __forceinline__ int64_t out_at(const AttnParams& p, const Unit& u, int row) {
   const int t = token_of(p, row);

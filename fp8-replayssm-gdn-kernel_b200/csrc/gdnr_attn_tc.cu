@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(TcCfg<D>::THREADS, 1)
       const int row = u.rt * BM + q * 128 + r;  // row of the sequence
       const bool live = row < u.s.m * p.G;
       const int lim = live ? min(u.s.kv - 1, u.s.kv - u.s.m + token_of(p, row)) : -1;  // last key the row sees
-      if (tid == 0 && u.s.m > p.max_q) atomicOr(p.err, GDNR_DEVERR_BAD_HINT);  // the join's grid goes by max_q
+      if (tid == 0) report_unit(p, u);
       float mx = -INFINITY, sum = 0.f;
       if (end > t0 && !q_tma) {
         // D / 8 lanes copy a row, eight loads in flight; rows past the sequence's are zeros

@@ -124,7 +124,8 @@ def paged_attention(
     The ``m`` new tokens of sequence ``n`` are the last of its ``kv_lens[n]`` cached ones (append
     them first): row ``i`` attends places ``0 .. kv_lens[n] - m + i``; a row without any
     is zeros.  ``k_cache``/``v_cache`` [pages,page_size,Hk,D] bf16, any page size; ``block_table``
-    [N,width] int32 holds each sequence's pages.  ``scale`` defaults to ``D ** -0.5``.  With
+    [N,width] int32 holds each sequence's pages; a page outside the cache, or a length outside
+    ``[0, width * page_size]``, is reported as ``GDNR_DEVERR_BAD_SLOT``.  ``scale`` defaults to ``D ** -0.5``.  With
     ``return_lse`` also the float32 log of each row's sum of exponentials [T,Hq]
     (-inf for a row without places).
     """

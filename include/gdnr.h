@@ -317,7 +317,9 @@ int gdnr_qk_norm_rope_append(const gdnr_append_args* args, void* stream);
  * What pages hold past a sequence's end is never used; the values of the places
  * before it are expected to be finite.  block_table[n][j] is the page of places
  * j*page_size ..; entries beyond the sequence's pages are not read.  A page outside the
- * cache sets GDNR_DEVERR_BAD_SLOT and reads as zeros. */
+ * cache sets GDNR_DEVERR_BAD_SLOT and reads as zeros.  So does a kv_lens[n] below zero or past
+ * the block table (width*page_size places) where the sequence has rows: they are
+ * computed as if it were zero, or the table's places. */
 typedef struct {
   gdnr_tensor q;           /* [T,Hq,D] BF16, D = 64, 128 or 256 */
   gdnr_tensor k_cache, v_cache; /* [pages,page_size,Hk,D] BF16 */
