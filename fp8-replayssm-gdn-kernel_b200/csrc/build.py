@@ -1,4 +1,4 @@
-"""Build libgdnr.so (all CUDA sources of this directory) for sm_100a, and the host call path (_host).
+"""Build libgdnr.so (all CUDA sources of this directory) for sm_100a, and the host call path (_host) if there is a torch.
 
     python fp8-replayssm-gdn-kernel_b200/csrc/build.py [--verbose-ptxas] [--force]
 
@@ -54,22 +54,35 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> pathlib.Path:
             cmd += ["-Xptxas", "-v"]
         print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-    build_host(force)
     if force or not TARGET.exists() or any(o.stat().st_mtime > TARGET.stat().st_mtime for o in objects):
         cmd = [nvcc(), *ARCH, "-shared", "-o", str(TARGET), *map(str, objects), "-lcuda"]
         print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_host(force)  # last: the C library needs no torch
     return TARGET
 
 
-def build_host(force: bool = False) -> pathlib.Path:
-    """gdnr/_host.so: the CPython module over torch's C++ tensors (g++, no device code)."""
+def torch_root() -> pathlib.Path | None:
+    """The installed torch, if it has its C++ headers."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    root = pathlib.Path(torch.__file__).resolve().parent
+    return root if (root / "include" / "torch").is_dir() else None
+
+
+def build_host(force: bool = False) -> pathlib.Path | None:
+    """gdnr/_host.so: the CPython module over torch's C++ tensors (g++, no device code); None without torch."""
+    root = torch_root()
+    if root is None:
+        print("no torch with C++ headers: gdnr/_host.so (the Python functions of the prompt operators) is not built", flush=True)
+        return None
     newest = max(HOST_SOURCE.stat().st_mtime, (INCLUDE / "gdnr.h").stat().st_mtime)
     if not force and HOST_TARGET.exists() and HOST_TARGET.stat().st_mtime >= newest:
         return HOST_TARGET
     import torch
 
-    root = pathlib.Path(torch.__file__).resolve().parent
     cuda = pathlib.Path(nvcc()).resolve().parent.parent
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
