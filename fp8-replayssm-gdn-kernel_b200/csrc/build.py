@@ -5,7 +5,7 @@
 Objects go to ``csrc/_build/``; the shared library is written next to the
 Python host package (``gdnr/libgdnr.so``) so that it travels with the tree.
 Incremental: a source is recompiled when it or any header is newer than its
-object.
+object, the host call path also when torch or Python are others than it was built for.
 """
 
 from __future__ import annotations
@@ -78,18 +78,24 @@ def build_host(force: bool = False) -> pathlib.Path | None:
     if root is None:
         print("no torch with C++ headers: gdnr/_host.so (the Python functions of the prompt operators) is not built", flush=True)
         return None
-    newest = max(HOST_SOURCE.stat().st_mtime, (INCLUDE / "gdnr.h").stat().st_mtime)
-    if not force and HOST_TARGET.exists() and HOST_TARGET.stat().st_mtime >= newest:
-        return HOST_TARGET
     import torch
 
+    # what the module's import compares (gdnr/_lib.py)
+    built_for = f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+    record = BUILD / "host.txt"
+    newest = max(HOST_SOURCE.stat().st_mtime, (INCLUDE / "gdnr.h").stat().st_mtime)
+    if (not force and HOST_TARGET.exists() and HOST_TARGET.stat().st_mtime >= newest
+            and record.exists() and record.read_text() == built_for):
+        return HOST_TARGET
     cuda = pathlib.Path(nvcc()).resolve().parent.parent
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DGDNR_BUILT_FOR="{built_for}"',
            "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
            "-I", sysconfig.get_paths()["include"], "-I", str(cuda / "include"), str(HOST_SOURCE), "-o", str(HOST_TARGET),
            "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+    record.write_text(built_for)
     return HOST_TARGET
 
 

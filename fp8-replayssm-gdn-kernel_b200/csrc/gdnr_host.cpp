@@ -3,6 +3,7 @@
 // of their device.  In Python the views of eleven tensors take 10 us, more than the kernel of
 // a call on a few tokens; here about 0.5 us.
 //
+//   _host.built_for   the torch and the Python it was compiled against
 //   _host.call(address, tensors, tail) -> status
 //     address   of an entry point int f(const void* args, void* stream)
 //     tensors   tuple of CUDA tensors or None (absent), the leading gdnr_tensor fields
@@ -117,4 +118,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Call path of libgdnr's pr
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* const m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", GDNR_BUILT_FOR) < 0) {  // the torch and the Python: build.py
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import sys
 import threading
 
 import torch
@@ -270,9 +271,12 @@ _host_module = None
 def _host():
     global _host_module
     if _host_module is None:
+        installed = f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
         try:
             from . import _host as module
-        except ImportError as e:
+            if module.built_for != installed:
+                raise ImportError(f"built for {module.built_for}, installed is {installed}")
+        except (ImportError, AttributeError) as e:
             raise RuntimeError(
                 "gdnr/_host.so is missing or does not fit this torch: build it with "
                 f"`python fp8-replayssm-gdn-kernel_b200/csrc/build.py` ({e})") from e

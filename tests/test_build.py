@@ -4,9 +4,12 @@ import importlib.util
 import pathlib
 import subprocess
 import sys
+import types
 
 import pytest
-import torch  # noqa: F401
+import torch
+
+from gdnr import _lib
 
 CSRC = pathlib.Path(__file__).resolve().parent.parent / "fp8-replayssm-gdn-kernel_b200" / "csrc"
 
@@ -49,3 +52,26 @@ def test_c_library_without_torch(builder, monkeypatch, tmp_path, without):
         monkeypatch.setattr(sys.modules["torch"], "__file__", str(tmp_path / "torch" / "__init__.py"))
     assert builder.build() == builder.TARGET
     assert builder.commands[-1] == "libgdnr.so"
+
+
+@pytest.mark.parametrize("changed", ["torch", "python"])
+def test_host_module_again_after_an_upgrade(builder, monkeypatch, changed):
+    builder.build()
+    builder.commands.clear()
+    if changed == "torch":
+        monkeypatch.setattr(torch, "__version__", "99.0")
+    else:
+        monkeypatch.setattr(builder.sys, "version_info", types.SimpleNamespace(major=9, minor=9))
+    builder.build()
+    assert builder.commands == ["_host.so"]
+    builder.build()
+    assert builder.commands == ["_host.so"]
+
+
+def test_host_module_of_another_torch_is_not_used(monkeypatch):
+    """A module that still loads could misread another torch's tensors."""
+    assert _lib._host().built_for.startswith(f"torch {torch.__version__},")
+    monkeypatch.setattr(_lib, "_host_module", None)
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    with pytest.raises(RuntimeError, match="build.py.*installed is torch 99.0"):
+        _lib._host()
