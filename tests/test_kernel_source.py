@@ -106,3 +106,9 @@ def test_null_slot_rows_are_counted_in_64_bits():
     for kernel in ("prefill_scan_kernel", "prefill_scan_tc_kernel"):
         zeros = block(body(text, kernel), "if (r.slot < 0) ")
         assert re.search(r"for \(int64_t i = tid; i < int64_t\(r\.end - r\.begin\) \* ", zeros), kernel
+
+
+def test_error_word_address_is_not_kept():
+    """It belongs to the device's context: an address kept over a reset would be written to by the next call's kernel."""
+    lookup = body(source("gdnr_api.cu"), "default_error_word")
+    assert "cudaGetSymbolAddress" in lookup and "static" not in lookup.replace("static_cast", "")
