@@ -663,8 +663,8 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
   const int part = blockIdx.x % heads, hv = part / PARTS, v0 = (part % PARTS) * ROWS;
   const SeqRange r = prefill_seq(p, n);
   if (r.slot < 0) {  // null slot: zero rows
-    for (int64_t i = tid; i < int64_t(r.end - r.begin) * ROWS; i += CS_THREADS)
-      p.out[(r.begin + i / ROWS) * p.o_st + int64_t(hv) * p.o_sh + v0 + i % ROWS] = 0;
+    static_assert(ROWS == 32, "a lane a value");
+    for (int t = r.begin + warp; t < r.end; t += CS_THREADS / 32) p.out[t * p.o_st + int64_t(hv) * p.o_sh + v0 + lane] = 0;
     griddep_wait();  // no CTA ends before the first kernel has
     return;
   }
@@ -972,8 +972,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
   const int n = ck_by_length(p, blockIdx.x / p.HV, lane), hv = blockIdx.x % p.HV, h = hv / (p.HV / p.H);
   const SeqRange r = prefill_seq(p, n);
   if (r.slot < 0) {  // null slot: zero rows
-    for (int64_t i = tid; i < int64_t(r.end - r.begin) * 128; i += CT_THREADS)
-      p.out[(r.begin + i / 128) * p.o_st + int64_t(hv) * p.o_sh + i % 128] = 0;
+    for (int t = r.begin + warp; t < r.end; t += CT_THREADS / 32)
+      *reinterpret_cast<uint2*>(p.out + t * p.o_st + int64_t(hv) * p.o_sh + lane * 4) = make_uint2(0, 0);
     griddep_wait();  // no CTA ends before the first kernel has
     return;
   }

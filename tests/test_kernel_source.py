@@ -100,12 +100,12 @@ def test_a_chunk_without_images_stops_the_scan():
     assert re.search(r"if \(ok\) \{\s*tc_fence_after", body(text, "prefill_scan_tc_kernel"))
 
 
-def test_null_slot_rows_are_counted_in_64_bits():
-    """Rows times values of a sequence pass 2^31 before its tokens do (up to 2^30 of them are taken)."""
+def test_null_slot_rows_are_counted_in_tokens():
+    """A sequence's values pass 2^31 before its tokens do (up to 2^30 of them are taken): the loop counts tokens."""
     text = source("gdnr_prefill.cu")
     for kernel in ("prefill_scan_kernel", "prefill_scan_tc_kernel"):
         zeros = block(body(text, kernel), "if (r.slot < 0) ")
-        assert re.search(r"for \(int64_t i = tid; i < int64_t\(r\.end - r\.begin\) \* ", zeros), kernel
+        assert re.findall(r"for \([^)]*\)", zeros) == [re.search(r"for \(int t = r\.begin \+ warp; t < r\.end; t \+= [^)]*\)", zeros)[0]], kernel
 
 
 def test_error_word_address_is_not_kept():
