@@ -75,10 +75,6 @@ __device__ __forceinline__ void tc_ld16(uint32_t addr, float* r) {
       : "memory");
 }
 
-__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::TC_W8(0), "r"(addr) : "memory");
-}
-
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TC_W8(0),

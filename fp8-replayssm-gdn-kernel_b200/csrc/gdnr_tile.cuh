@@ -52,7 +52,7 @@ __device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r
                : "memory");
 }
 
-// Named barriers: wait for `count` threads / arrive without waiting.
+// Named barriers: wait for `count` threads
 __device__ __forceinline__ void bar_sync(int id, int count) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory"); }
 // ... and whether any of them has `x`
 __device__ __forceinline__ bool bar_or(int id, int count, bool x) {
@@ -62,9 +62,6 @@ __device__ __forceinline__ bool bar_or(int id, int count, bool x) {
                : "r"(id), "r"(count), "r"(int(x))
                : "memory");
   return r != 0;
-}
-__device__ __forceinline__ void bar_arrive(int id, int count) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
 // Two floats in one register pair: one instruction for both
