@@ -125,3 +125,28 @@ def test_stages_are_used_again_many_times(cuda_device):
         again = d["state"].clone()
         got = gdnr.gdn_prefill(d["mixed"], d["a"], d["b"], d["a_log"], d["dt_bias"], again, R.cu(lens), max_seqlen=max(lens))
         assert torch.equal(first, got) and torch.equal(state, again)
+
+
+@pytest.mark.parametrize("h,hv,lens", [(16, 32, [70, 64, 128, 65, 64, 64, 80, 64, 64, 64]), (2, 4, [70, 64, 150])])
+def test_decay_that_clears_the_state(cuda_device, h, hv, lens):
+    """Gates of minus infinity, several in a row and at the borders of chunks and of their 16-token blocks: what came before such
+    a token is gone, nothing turns into NaN, also for the whole inverse of the chunk's system."""
+    d = inputs(120, lens, h, hv)
+    d["a_log"] = torch.full((hv,), 80.0, device="cuda")  # exp(80) softplus(3e38) is infinite
+    d["a"].fill_(-200.0)  # softplus underflows: no decay
+    for t in (0, 15, 16, 17, 31, 48, 63, 64, 69, 70, 100, 133, 134, 140, 200, sum(lens) - 1):
+        d["a"][t] = 3.0e38
+    got, state = check(d, lens)
+    cleared = d["state"].clone() * 1e6
+    again = gdnr.gdn_prefill(d["mixed"], d["a"], d["b"], d["a_log"], d["dt_bias"], cleared, R.cu(lens), max_seqlen=max(lens))
+    assert torch.equal(again[:70], got[:70]) and torch.equal(cleared[0], state[0])  # its first token clears the state
+
+
+def test_other_sequences_garbage_stays_theirs_with_few_heads(cuda_device):
+    """As above on the scan that spreads a head over multiprocessors."""
+    lens = [70, 64, 33, 100]
+    d = inputs(121, lens, 2, 4)
+    clean, _ = check(d, lens)
+    d["mixed"][70:134] = float("nan")
+    got = gdnr.gdn_prefill(d["mixed"], d["a"], d["b"], d["a_log"], d["dt_bias"], d["state"].clone(), R.cu(lens), max_seqlen=max(lens))
+    assert torch.equal(got[:70], clean[:70]) and torch.equal(got[134:], clean[134:])
