@@ -176,9 +176,11 @@ __global__ void __launch_bounds__(RC_WARPS * 32) prefill_recurrent_kernel(const 
 // of narrower ones, so that the float32 state stays within 1e-5 also where keys are alike and
 // N is what is left of large terms: S as two bf16 (against K and Q); the weighted N as
 // three (its products add up in S, which may be far smaller than their sum of
-// sizes); A, T and P, whose entries are at most about one, as two f16, and with them R and N,
-// each row brought near one by a power of two first (with two bf16 here the state was
-// 1.8e-5 off on such keys).  The output needs it too, although it is bf16: S Q^T and N P^T
+// sizes); A, T and P, whose entries are at most one, as two f16 of 2^14 times them, and with them R and N,
+// each row of R brought to 2^8 by a power of two first (with two bf16 here the state was
+// 1.8e-5 off on such keys).  f16 ends at 2^-24: an entry of T is exact to 2^-39, one of R to 2^-34 of its row's largest
+// in the chunk (2^-25 and 2^-30 without the powers: a state that little was written to, behind large and decayed
+// values, had errors of 1e-4).  The output needs it too, although it is bf16: S Q^T and N P^T
 // nearly cancel there, and operands rounded once left it 8e-3 off instead of 2e-3.
 // Gates are summed in double: differences of float32 prefix sums would cancel under
 // strong decay.
@@ -191,8 +193,10 @@ constexpr int CK_TRI = 10 * 512;
 __host__ __device__ constexpr int ck_block(int i, int j) { return (4 * j - j * (j - 1) / 2 + i - j) * 512; }
 __device__ __forceinline__ uint32_t ck_in_block(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
 
+constexpr float CK_UP = 16384.f, CK_DOWN = 1.f / CK_UP;
+
 struct CkImage {
-  // t: diagonal blocks: (I + A)^-1 of the block, below them: -A; or (whole) T = (I + A)^-1
+  // t: diagonal blocks: (I + A)^-1 of the block, below them: -A; or (whole) T = (I + A)^-1; t and p times CK_UP
   uint8_t t_hi[CK_TRI], t_lo[CK_TRI], p_hi[CK_TRI], p_lo[CK_TRI];
   float beta[CK_C], cx[CK_C], cq[CK_C], cs[CK_C], total;  // beta, -beta e^G rk, e^G rq K^-1/2, e^{G_C - G} rk; e^{G_C}
   uint32_t made;  // 1: all of it is there; 0: the first kernel's wait gave up
@@ -361,13 +365,21 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
         *reinterpret_cast<uint32_t*>(img.t_lo + at) = wl;
       }
     };
+    // T_low (-A) comes as CK_UP^2 times it; 2^10 times it as a left operand (its entries: at most 33, sums of T's)
+    auto scale = [&](float* v, float f) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) scale2(v + k, pack2(f, f));
+    };
+    constexpr float LEFT = 1024.f, TO_LEFT = LEFT / (CK_UP * CK_UP), FROM_LEFT = 1.f / LEFT;
     float x[2][8] = {}, y[2][8] = {};
     uint32_t wh[4], wl[4];
     bar_sync(1, 128);
     if (mine) {
       times_block(x[0], 2 * w + 1, 2 * w + 1, 2 * w + 1, 2 * w);  // T_low (-A)
+      scale(x[0], TO_LEFT);
       ck_left_f16(reinterpret_cast<const float(*)[4]>(x[0]), wh, wl);
       times(y[0], wh, wl, 2 * w, 2 * w);
+      scale(y[0], FROM_LEFT);
       __syncwarp();
       emit(y[0], 2 * w + 1, 2 * w);
     }
@@ -380,6 +392,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
       for (int j = 0; j < 2; ++j) {
         times_block(x[j], 2 + w, 2, 2, j);
         if (w) times_block(x[j], 3, 3, 3, j);
+        scale(x[j], TO_LEFT);
         ck_left_f16(reinterpret_cast<const float(*)[4]>(x[j]), wh, wl);
         times(y[0], wh, wl, j, 0);
         if (j) times(y[1], wh, wl, 1, 1);
@@ -387,6 +400,8 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
     }
     bar_sync(1, 128);
     if (mine) {
+      scale(y[0], FROM_LEFT);
+      scale(y[1], FROM_LEFT);
       emit(y[0], 2 + w, 0);
       emit(y[1], 2 + w, 1);
     }
@@ -460,7 +475,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
   __syncthreads();  // gates and norms
   // what all heads share: the products times both norms (and the sign of -A)
   const int rbm = warp == 1 ? warp : rb2;
-  const float gain = of_q ? 1.f : -1.f;
+  const float gain = of_q ? CK_UP : -CK_UP;
   const float* rn = of_q ? sm.rq : sm.rk;
 #pragma unroll
   for (int u = 0; u < 5; ++u) {
@@ -515,7 +530,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
             const int row = (lane >> 2) + 8 * hf, c = (unit_tile[u] & 1) * 8 + 2 * (lane & 3), last = of_q ? row : row - 1;
             x.x = c <= last ? x.x : 0.f;
             x.y = c < last ? x.y : 0.f;
-            if (!of_q) *reinterpret_cast<float2*>(&sm.a[e][(warp * 16 + row) * CD_LDA + c]) = x;
+            if (!of_q) *reinterpret_cast<float2*>(&sm.a[e][(warp * 16 + row) * CD_LDA + c]) = make_float2(x.x * CK_DOWN, x.y * CK_DOWN);
           }
           if (u >= 2 || of_q) {
             uint32_t wh, wl;
@@ -534,7 +549,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float s[4] = {i == cl ? 1.f : 0.f, 0.f, 0.f, 0.f};
+        float s[4] = {i == cl ? CK_UP : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < i; j += 4) {
           const float4 v = *reinterpret_cast<const float4*>(&ad[i * CD_LDA + j]);
@@ -605,13 +620,14 @@ __device__ __forceinline__ void ck_left(const float (*x)[4], uint32_t* hi, uint3
 }
 
 // A power of two that brings a row's largest value (over the four lanes that hold the row) into
-// [2^4, 2^5), and its inverse.  At most 2^115: the factors of O, up to 2^7 (a query of zeros), times it stay finite.
+// [2^8, 2^9), and its inverse.  N then stays below 2^15: keys are of unit length and beta at most one, so that a token's N is
+// at most the sum of 64 R.  At most 2^103: the factors of O, up to 2^7 (a query of zeros), times it and CK_UP stay finite.
 __device__ __forceinline__ void ck_row_scale(float top, float& up, float& down) {
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int e = min(max(int(__float_as_uint(top) >> 23), 16), 250);
-  up = __uint_as_float(uint32_t(258 - e) << 23);
-  down = __uint_as_float(uint32_t(e - 4) << 23);
+  const int e = min(max(int(__float_as_uint(top) >> 23), 32), 250);
+  up = __uint_as_float(uint32_t(262 - e) << 23);
+  down = __uint_as_float(uint32_t(e - 8) << 23);
 }
 
 // Right operand of block (i, j) of a triangular matrix: both 8-token halves, k of 16
@@ -816,7 +832,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
         top1 = fmaxf(top1, fmaxf(fabsf(x[2]), fabsf(x[3])));
       }
     }
-    // rows to at most 2^5 (N stays far below 2^15 then: keys are of unit length and beta at most one)
+    // rows to at most 2^9, here CK_UP times them: what the blocks of A take off is of that size
     // The row of O is scaled alike.  Where next to nothing is written (beta of zero) and S is not small, that must not
     // overflow: R then counts as 2^-96 of O at least, far less than what float32 keeps of S beside it.
     if (__any_sync(0xffffffffu, fminf(top0, top1) < 0x1p-60f)) {
@@ -833,7 +849,8 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
     ck_row_scale(top0, up0, down0);
     ck_row_scale(top0, up0, down0);
     ck_row_scale(top1, up1, down1);
-    const uint64_t up0_2 = pack2(up0, up0), up1_2 = pack2(up1, up1);
+    up0 *= CK_UP, up1 *= CK_UP;
+    const uint64_t up0_2 = pack2(up0, up0), up1_2 = pack2(up1, up1), back_2 = pack2(CK_DOWN, CK_DOWN);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       scale2(X[j], up0_2);
@@ -854,6 +871,8 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
         ck_right(th, i, j, lane, b[i]);
         ck_right(tlo, i, j, lane, bl[i]);
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) scale2(X[2 * j + i], back_2), scale2(X[2 * j + i] + 2, back_2);
       ck_left_f16(X + 2 * j, rh, rl);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
@@ -863,6 +882,8 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
             mma_f16_first(N[2 * j + i], rh, b[j][2 * i], b[j][2 * i + 1]);
           else
             mma_f16(N[2 * j + i], q == 1 ? rl : rh, (q == 2 ? bl : b)[j][2 * i], (q == 2 ? bl : b)[j][2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) scale2(N[2 * j + i], back_2), scale2(N[2 * j + i] + 2, back_2);
       ck_left_f16(N + 2 * j, nh[j], nl[j]);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
@@ -907,6 +928,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
     for (int j = 0; j < 4; ++j) ck_out_column(O, nh[j], nl[j], ph, pl, j, lane, kh == 0, kh == 1);
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.empty[c % CS_STAGES])) : "memory");
+    down0 *= CK_DOWN, down1 *= CK_DOWN;
     // O^T to token rows, 16 tokens at a time through the warp's own rows (48 bytes apart: no bank twice)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -935,7 +957,7 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
 // quarter of the lanes, have half of the columns of a thread's row each (of S's keys, of the chunk's tokens); a ninth
 // issues the products, a tenth requests the chunks.  A chunk, as a chain:
 //   warps: S -> its two parts          | products: X = S K^T and S Q^T
-//   warps: R, near one, as two parts   | N = R T^T
+//   warps: R, near 2^8, as two parts   | N = R T^T
 //   warps: weighted N as three parts   | S += it times K
 // and beside it N as two parts, N P^T, and the output of the chunk before.
 // 3.4 us a chunk (all 128 rows on warp-level tiles: 7.2 us); 12 prompts of up to 2047 tokens, 32 heads: 0.12 ms of
@@ -1117,7 +1139,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
       if (lane == 0) mbar_arrive(bar);
     };
     const int tok = half * 32;  // the thread's tokens of a chunk
-    float down = 0.f, sq[32];   // the row's scale, S q of its tokens: kept until the chunk's output is written
+    float down = 0.f, sq[32];   // the row's scale (back from N, CK_UP times it), S q of its tokens: kept until the chunk's output is written
     // The output of chunk c over V, then to memory in whole rows.  Called after the next chunk's products have begun.
     auto finish = [&](int c) {
       CtStage& st = sm.stage[c % CS_STAGES];
@@ -1215,16 +1237,17 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
           x[k] = y.x, x[k + 1] = y.y;
           top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
         }
-        // the row near one for f16, by the largest of all 64 tokens
+        // the row near 2^8 for f16, by the largest of all 64 tokens
         sm.top[half][row] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.top_ready[quarter]);  // both warps have read X then, too
         ok = wait(&sm.top_ready[quarter], c & 1);
         if (!ok) break;
         top = fmaxf(top, sm.top[half ^ 1][row]);
-        const int e = min(max(int(__float_as_uint(top) >> 23), 8), 250);
-        const float up = __uint_as_float(uint32_t(258 - e) << 23);
-        down = __uint_as_float(uint32_t(e - 4) << 23);
+        // (as ck_row_scale)
+        const int e = min(max(int(__float_as_uint(top) >> 23), 32), 250);
+        const float up = __uint_as_float(uint32_t(262 - e) << 23);
+        down = __uint_as_float(uint32_t(e - 8) << 23) * CK_DOWN;
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) split_f16x2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
@@ -1257,7 +1280,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1) prefill_scan_tc_kernel(const __
         tc_st16(mem + CT_PARTS + 64 + half * 16, rest);
         announce(&sm.w_ready);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) split_f16x2(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
+        for (int k = 0; k < 16; ++k) {
+          scale2(x + 2 * k, pack2(CK_DOWN, CK_DOWN));
+          split_f16x2(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
+        }
         tc_st16(mem + CT_NF + half * 16, hi);
         tc_st16(mem + CT_NF + 32 + half * 16, lo);
         announce(&sm.f_ready);

@@ -253,3 +253,15 @@ def test_small_state_and_no_values(cuda_device, lens, h, hv):
     d["mixed"][:, 2 * h * 128:] = 0
     d["state"] *= 1e-25
     check(d, lens)
+
+
+@pytest.mark.parametrize("lens,h,hv", [([64, 128, 70], 2, 4), ([19, 7], 2, 4), ([64, 70, 130, 64, 90, 64, 65, 64, 100, 64], 16, 32)])
+def test_little_written_behind_large_values(cuda_device, lens, h, hv):
+    """The last tokens of each sequence write 1e-4 of what the ones before them did, which has decayed: the state is theirs.
+    Entries of the chunk's system count to 2^-39 there and values to 2^-34 of the largest, 1e-6 of such a state."""
+    d = inputs(20, lens, h, hv)
+    end = 0
+    for m in lens:
+        end += m
+        d["mixed"][end - min(m // 2, 40):end, 2 * h * 128:] *= 1e-4
+    check(d, lens)
