@@ -869,8 +869,11 @@ cudaError_t launch_attn(const AttnParams& p, cudaStream_t stream) {
   const int64_t most = std::min<int64_t>(int64_t(p.max_q) * p.G, INT32_MAX);
   if (most <= few_rows(p.D) || !attn_tc_takes(p)) return small_rows(p, int(most), AtRows{0, INT32_MAX}, Cuts{}, stream);
   const bool alike = int64_t(p.T) == int64_t(p.N) * p.max_q;  // all of the same length
-  // sequences of many rows on the tensor-memory tiles, the others, mostly of one token, on tiles of few rows: 12 sequences
-  // of 1 to 701 tokens 73 us (78 us with everything up to 64 rows on tiles of 64)
+  // sequences of many rows on the tensor-memory tiles, the others, mostly of one token, on tiles of few rows.  The limit is 16
+  // rows and not few_rows, although drafts by themselves are better off below that: here the tcgen05 kernel runs anyway, and the
+  // other one keeps its smallest tiles.  With 16 / with few_rows, 16 / 2 heads of 64, 128, 256: 32 drafts of 3 to 8 tokens beside a chunk
+  // of 2048 over 4096 keys 85 / 92, 103 / 122, 159 / 171 us; 8 of 4 beside 512 over 4096 39 / 47, 49 / 63, 69 / 85 us; 12
+  // sequences of 1 to 701 tokens 39 / 43, 49 / 56, 69 / 71 us.
   const int lo = alike ? 0 : (p.G <= 16 ? 16 : few_rows(p.D));
   cudaError_t e = launch_attn_tc(p, lo, stream);
   if (e != cudaSuccess) return e;

@@ -11,7 +11,8 @@
 // stream, on the next tile's S).  The reference maximum of a row only moves when the row's maximum
 // has grown by more than 2^8 (p <= 2^8 keeps bf16's relative precision); only then O is rescaled.
 //
-// 2048 tokens over 32768 keys, 16 / 2 heads of 128: 414 us, 1.29 PFLOP/s (heads of 256 over 16384 keys: 1.11).  A stream's
+// 2048 tokens over 32768 keys, 16 / 2 heads of 128: 416 us, 1.28 PFLOP/s in bursts of a hundred calls, 480 to 490 us, 1.1 PFLOP/s
+// in runs of seconds, under the power cap (heads of 256 over 16384 keys: 458 and 527 us, 1.13 and 0.98 PFLOP/s).  A stream's
 // softmax (1 us a tile) and its two products (0.6 us) alternate, as tensor memory has no room for a second S; the
 // other stream fills most of the gaps.  Slower were: tiles of 64 keys with two buffers of S each, P announced by
 // halves, some of the exponentials by a polynomial.

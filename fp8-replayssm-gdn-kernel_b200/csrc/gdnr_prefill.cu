@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(CD_THREADS, 3) prefill_derive_kernel(const __g
 
 // ---------------------------------------------------------------- chunked form, second kernel, few heads
 // Bound by the chain of chunks and the instructions of the one warp on each scheduler: 8192 tokens
-// of 32 heads 0.36 ms, 2.8 us a chunk, tensor cores 47 % busy.  (Four warps to 16 rows: 0.52 ms.)
+// of 32 heads 0.36 ms, 2.8 us a chunk, tensor cores 53 % busy.  (Four warps to 16 rows: 0.52 ms.)
 // Four CTAs a head with 32 value rows each; two warps share 16 rows: each
 // has half of S's key columns, X and S Q^T are added up through shared memory, both solve for N, and each
 // updates its half of S and makes the output of half the tokens.  A fifth warp requests the chunks.
@@ -961,8 +961,8 @@ __global__ void __launch_bounds__(CS_THREADS, 1) prefill_scan_kernel(const __gri
 //   warps: weighted N as three parts   | S += it times K
 // and beside it N as two parts, N P^T, and the output of the chunk before.
 // 3.4 us a chunk (all 128 rows on warp-level tiles: 7.2 us); 12 prompts of up to 2047 tokens, 32 heads: 0.12 ms of
-// 0.17.  Bound by the 56 products of a chunk, 90 to 150 cycles each (64 at the full rate: the warps' loads and stores
-// of tensor memory run beside them), and the conversions between.  Slower were: sixteen warps; the output
+// 0.17.  Bound by the 56 products of a chunk, in four groups one after another (the tensor cores are busy 28 % of the time:
+// their A operands come from tensor memory, beside the warps' loads and stores there), and the conversions between.  Slower were: sixteen warps; the output
 // taken out before X or after R; P T from the first kernel, which saves the N P^T products, was even (3.3 us a chunk,
 // 13 us more for the images).
 struct CtStage {  // one chunk

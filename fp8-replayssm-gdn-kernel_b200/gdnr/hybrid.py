@@ -60,6 +60,10 @@ def gdn_prefill(
     ``GDNR_DEVERR_BAD_SLOT``; the others must be distinct.  An empty sequence leaves its
     state as it is (zeros if it starts from zeros).
 
+    ``max_seqlen`` (the mean length where it is 0) decides for the whole call: up to 20 tokens token by
+    token, else in chunks of 64, with a workspace of 21568 bytes for each of the ``T // 64 + N`` chunks of
+    each value head.  Many single tokens beside a long prompt are better off in a call of their own.
+
     The state can be handed to the decode step with :meth:`gdnr.ReplayState.load_state`.
     """
     if out is None:

@@ -259,7 +259,13 @@ int gdnr_bf16_step(const gdnr_bf16_step_args* args, void* stream);
  * slot state_indices[n]; an index <= 0 is the null slot (out rows are zeros, no state is
  * touched), one >= slots likewise and reported as GDNR_DEVERR_BAD_SLOT; the non-null ones
  * must be distinct.  Without it sequence n uses slot n.  has_initial[n] == 0: the
- * sequence starts from the zero state and its slot is only written. */
+ * sequence starts from the zero state and its slot is only written.
+ *
+ * All sequences of a call go one way, token by token or in chunks of 64 tokens; max_seqlen
+ * decides (more than 20: chunks), or the mean length where it is 0.  In chunks, single tokens
+ * beside a long prompt cost a chunk each: give them a call of their own where they are many.
+ * A value that is not finite spoils its sequence's rows from its chunk on, earlier tokens of that
+ * chunk among them. */
 typedef struct {
   gdnr_tensor mixed_qkv;     /* [T, 2*H*K + HV*V] BF16, raw q | k | v */
   gdnr_tensor a, b;          /* [T,HV] BF16|F16|F32 */
@@ -279,8 +285,9 @@ typedef struct {
 } gdnr_prefill_args;
 
 int gdnr_gdn_prefill(const gdnr_prefill_args* args, void* stream);
-/* Workspace bytes of gdnr_gdn_prefill for T tokens of N sequences (about 11 KB a token
- * at 32 value heads; none for a few tokens a sequence). */
+/* Workspace bytes of gdnr_gdn_prefill for T tokens of N sequences: in chunks 21568 bytes for each of
+ * (T / 64 + N) chunks of each value head (at 32 heads 11 KB a token and 690 KB a sequence), none token
+ * by token. */
 int64_t gdnr_gdn_prefill_workspace(int64_t tokens, int64_t sequences, int32_t value_heads, int32_t max_seqlen);
 
 /* ---- gdnr_qk_norm_rope_append --------------------------------------------
@@ -337,7 +344,8 @@ typedef struct {
 } gdnr_attn_args;
 
 int gdnr_paged_attention(const gdnr_attn_args* args, void* stream);
-/* Workspace bytes of gdnr_paged_attention on the current device for head dim D. */
+/* Workspace bytes of gdnr_paged_attention on the current device for head dim D, whatever the batch: every
+ * multiprocessor's parts of units that are cut (148 of them: 30, 59 and 78 MB for D = 64, 128 and 256). */
 int64_t gdnr_paged_attention_workspace(int32_t head_dim);
 
 /* ---- misc --------------------------------------------------------------- */
