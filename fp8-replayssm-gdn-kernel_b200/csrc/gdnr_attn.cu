@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(32 * WM * WN + 32)
         }
 #pragma unroll
       for (int kk = 0; kk < NT / 2; ++kk) {
-        // weights are rounded to bf16 for the tensor cores; their sum is taken before that
+        // Weights are rounded to bf16 for the tensor cores; their sum is taken before that.  (As two bf16 each, which would leave the
+        // output's own rounding only: 64 single tokens 1 to 5 % slower, drafts up to 20 %.)
         const uint32_t a[4] = {cvt_bf16x2(s[2 * kk][0], s[2 * kk][1]), cvt_bf16x2(s[2 * kk][2], s[2 * kk][3]),
                                cvt_bf16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]), cvt_bf16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
 #pragma unroll
