@@ -56,9 +56,11 @@ typedef enum {
 
 /* Bits of the device error word (see error_flag below). */
 #define GDNR_DEVERR_WAIT_TIMEOUT 0x1u /* a bounded mbarrier wait gave up */
-#define GDNR_DEVERR_BAD_POS 0x2u      /* fused step: pos[b] outside [0, L) */
-#define GDNR_DEVERR_BAD_HINT 0x4u     /* flush_hint NONE but a sequence's ring was full */
-#define GDNR_DEVERR_BAD_SLOT 0x8u     /* packed decode: state_indices[i] >= slots */
+#define GDNR_DEVERR_BAD_POS 0x2u      /* fused step: pos[b] outside [0, L); append: positions[t] outside the table */
+#define GDNR_DEVERR_BAD_HINT 0x4u     /* flush_hint NONE but a sequence's ring was full; attention: a sequence
+                                         longer than max_seqlen */
+#define GDNR_DEVERR_BAD_SLOT 0x8u     /* a slot or page outside its pool (packed decode, prompt operators), a
+                                         length outside its block table */
 #define GDNR_DEVERR_LAYOUT 0x10u      /* a kernel's shared memory did not fit its layout (a launch
                                          configuration fault of the library): nothing was done */
 
